@@ -38,6 +38,8 @@ fn main() {
         let obj = out.join(format!("{s}.o"));
         let ok = Command::new(&hipcc)
             .args(["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-fno-gpu-rdc", "-x", "hip", "-c"])
+            // no packed-f32 instructions, as in build.py
+            .args(["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"])
             .arg(csrc.join(s))
             .arg("-o")
             .arg(&obj)
