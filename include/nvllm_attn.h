@@ -239,6 +239,89 @@ int nvllm_qk_norm_rope_cache_f32(const void *q, const void *k, const void *v, vo
                                  int num_heads, int num_kv_heads, int head_dim, int block_size,
                                  int64_t num_cache_blocks, nvllm_stream_t stream);
 
+/* ======================================================================== */
+/* 8-bit KV cache                                                           */
+/* ======================================================================== */
+
+/* The paged cache at one byte a value (no counterpart in the reference, whose cache is bf16 / f32):
+ * half the bytes of a decode step, twice the tokens in the same memory.
+ *   k/v cache   uint8 [num_blocks, block_size, num_kv_heads, head_dim]   codes
+ *   k/v scales  f32   [num_blocks, num_kv_heads]                         one per block and kv head
+ *   value = code * scale
+ * format 0 = int8: codes are integers in -127 .. 127; format 1 = E4M3 (OCP): codes are its numbers,
+ * +-448 at most.  dtype (0 bf16, 1 f32) is that of the other tensors.  head_dim <= 256, block_size <=
+ * 256.  A fresh cache is all zeros, codes and scales.
+ *
+ * What a write does to a block.  Scales are powers of two, the smallest with max|x| <= top * scale
+ * (top 127 or 448; 0 for zeros; 2^-126 at least).  A call that writes the block's row 0 BEGINS the
+ * block: its scale comes from the rows of that call, what the block held before is gone.  Any other
+ * call keeps the rows it does not write, and the scale if it suffices; if its rows need a larger one,
+ * the kept codes are rounded to that.  All roundings are to nearest, ties to even; x / scale and code *
+ * scale are exact, so a write has one right answer, bit for bit.  A NaN is stored as E4M3's NaN, and as
+ * 0 in int8; what is infinite or beyond 2^127 saturates and takes no part in the scale.
+ * The slot mapping may name slots in any order; of tokens that name the same slot the last one is
+ * written; a negative slot, or one past the pool, skips its token.  Two calls that run at the same
+ * time must not write the same block. */
+
+/* Workspace of the two writers below: 0 up to 4096 tokens, else 4 bytes per slot of the pool.  Its
+ * contents need no preparation and mean nothing between calls; calls that overlap in time need one
+ * each.  A smaller one (or one not 16-byte aligned) is NVLLM_ERR_CONFIG. */
+size_t nvllm_kv8_write_workspace_bytes(int64_t num_tokens, int block_size, int64_t num_cache_blocks);
+
+/* nvllm_reshape_and_cache_* with quantisation: key, value [num_tokens, num_kv_heads, head_dim]. */
+int nvllm_reshape_and_cache_kv8(const void *key, const void *value, void *k_cache, void *v_cache,
+                                float *k_scales, float *v_scales, const int64_t *slot_mapping,
+                                void *workspace, size_t workspace_bytes, int64_t num_tokens,
+                                int num_kv_heads, int head_dim, int block_size,
+                                int64_t num_cache_blocks, int format, int dtype,
+                                nvllm_stream_t stream);
+
+/* nvllm_qk_norm_rope_cache_* with quantisation: the rotated K and V go into the 8-bit cache, rounded
+ * once, from f32 (from f64 where the tensors are f32), not by way of k_out.  q_out may be q; k_out
+ * (optional) must not overlap k. */
+int nvllm_qk_norm_rope_cache_kv8(const void *q, const void *k, const void *v, void *q_out,
+                                 void *k_out, const void *q_weight, const void *k_weight, float eps,
+                                 const void *cos_cache, const void *sin_cache,
+                                 int64_t max_positions, const int32_t *positions, void *k_cache,
+                                 void *v_cache, float *k_scales, float *v_scales,
+                                 const int64_t *slot_mapping, void *workspace,
+                                 size_t workspace_bytes, int64_t num_tokens, int num_heads,
+                                 int num_kv_heads, int head_dim, int block_size,
+                                 int64_t num_cache_blocks, int format, int dtype,
+                                 nvllm_stream_t stream);
+
+/* nvllm_gather_cache_blocks, dequantised: k_out[i] = the values of block block_ids[i] (device int32
+ * [num_ids]), [num_ids, block_size, num_kv_heads, head_dim] in dtype; v_out likewise unless NULL
+ * (then v_cache and v_scales may be NULL too).  An id outside the pool gives zeros.  Exact in bf16
+ * and f32 alike. */
+int nvllm_gather_cache_blocks_kv8(const void *k_cache, const void *v_cache, const float *k_scales,
+                                  const float *v_scales, const int32_t *block_ids, int64_t num_ids,
+                                  void *k_out, void *v_out, int64_t num_cache_blocks,
+                                  int block_size, int num_kv_heads, int head_dim, int format,
+                                  int dtype, nvllm_stream_t stream);
+
+/* nvllm_paged_attn_* over the 8-bit cache: same tables, lengths, mask, clamps and output; a query that
+ * sees no key (context_len < num_new_tokens) gives zeros.  Scales may be any finite numbers >= 0.
+ * `workspace` as there, sized by nvllm_paged_attn_kv8_workspace_bytes for the same shape and dtype
+ * with the launch device current. */
+int nvllm_paged_attn_kv8(const void *q, const void *k_cache, const void *v_cache,
+                         const float *k_scales, const float *v_scales, const int32_t *block_tables,
+                         const int32_t *context_lens, void *out, void *workspace,
+                         size_t workspace_bytes, int num_seqs, int num_new_tokens, int num_heads,
+                         int num_kv_heads, int head_dim, int block_size, int max_blocks_per_seq,
+                         int64_t num_cache_blocks, float scale, int format, int dtype,
+                         nvllm_stream_t stream);
+size_t nvllm_paged_attn_kv8_workspace_bytes(int num_seqs, int num_new_tokens, int num_heads,
+                                            int num_kv_heads, int head_dim, int block_size,
+                                            int max_blocks_per_seq, int dtype);
+/* Which kernel a launch shape runs (a pure query, as nvllm_paged_attn_path): 2 = generic. */
+int nvllm_paged_attn_kv8_path(int num_seqs, int num_new_tokens, int num_heads, int num_kv_heads,
+                              int head_dim, int block_size, int max_blocks_per_seq, int dtype);
+
+/* Bytes of ONE layer's K (or V) in the 8-bit cache, codes and scales; -1 on a negative dimension. */
+int64_t nvllm_kv_cache_kv8_layer_bytes(int64_t num_blocks, int64_t block_size,
+                                       int64_t num_kv_heads, int64_t head_dim);
+
 /* Replaces: flash_attention_get_last_error (kernels/flash_attn_fwd.cu:540-543).
  * Thread-local; never NULL. */
 const char *nvllm_get_last_error(void);

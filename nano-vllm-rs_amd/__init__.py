@@ -4,7 +4,8 @@ Python here is only the harness-side mirror of the C ABI in
 include/nvllm_attn.h: ctypes bindings (`capi`), the host structures
 (`core`: BlockTable, BlockManager, hash_token_block, ...) and the
 reference-shaped operators (`attention`: flash_attention, prefill_attention,
-paged_attention, write_kv_to_cache) over torch device tensors.  All compute
+paged_attention, write_kv_to_cache) over torch device tensors, with the 8-bit
+KV cache's in `kv8`.  All compute
 runs in libnvllm_attn.so (hand-written gfx950 HIP + C++ host code); nothing in
 this package falls back to PyTorch or to the CPU oracle.
 """
@@ -21,4 +22,8 @@ from .attention import (  # noqa: F401
     FlashAttentionConfig, flash_attention, prefill_attention, paged_attention,
     paged_attention_batched, paged_attention_path, validate_tables, write_kv_to_cache, reshape_and_cache, RotaryEmbedding,
     qk_norm_rope_cache,
+)
+from .kv8 import (  # noqa: F401
+    reshape_and_cache_kv8, qk_norm_rope_cache_kv8, gather_cache_blocks_kv8, paged_attention_kv8,
+    paged_attention_kv8_path,
 )

@@ -19,7 +19,7 @@ import numpy as np
 import torch
 
 from . import capi
-from .core import BlockTable, ConfigError, LayerKVCache, check
+from .core import KV8_FORMATS, BlockTable, ConfigError, LayerKVCache, TensorError, check
 
 _DT = {torch.bfloat16: 0, torch.float32: 1}
 
@@ -45,6 +45,12 @@ def _dtype_code(t):
     if t.dtype not in _DT:
         raise ConfigError(capi.NVLLM_ERR_UNSUPPORTED, "dtype must be bfloat16 or float32")
     return _DT[t.dtype]
+
+
+def _require_wide(*caches):
+    for c in caches:
+        if c.dtype in KV8_FORMATS:
+            raise ConfigError(capi.NVLLM_ERR_UNSUPPORTED, "an 8-bit cache takes the *_kv8 operators")
 
 
 class FlashAttentionConfig:
@@ -100,13 +106,15 @@ def prefill_attention(query, key, value, num_heads, num_kv_heads, scale, causal)
 
 def paged_attention(query, kv_cache, block_table, context_len, num_heads, num_kv_heads, head_dim,
                     scale):
-    """paged.rs:117-126: ONE sequence, host BlockTable, the layer's cache -> [B,T,Hq*D]."""
+    """paged.rs:117-126: ONE sequence, host BlockTable, the layer's cache (8-bit ones too) -> [B,T,Hq*D]."""
     assert isinstance(kv_cache, LayerKVCache) and isinstance(block_table, BlockTable)
     kc, vc = kv_cache.key_cache(), kv_cache.value_cache()
     _require_device(query, kc, vc)
     B, T, Hq, D = query.shape
     if Hq != num_heads or D != head_dim or kc.shape[2] != num_kv_heads:
         raise ConfigError(capi.NVLLM_ERR_CONFIG, "shape mismatch")
+    if kc.dtype in KV8_FORMATS:
+        return _paged_attention_kv8_seq(query, kv_cache, block_table, context_len, scale)
     out = torch.empty((B, T, Hq * D), dtype=query.dtype, device=query.device)
     need = capi.lib().nvllm_paged_attention_seq_scratch_bytes(
         block_table.num_blocks(), T, Hq, num_kv_heads, D, block_table.block_size())
@@ -116,6 +124,30 @@ def paged_attention(query, kv_cache, block_table, context_len, num_heads, num_kv
         num_kv_heads, D, float(scale), _dtype_code(query), _ptr(out), _ptr(scratch),
         scratch.numel(), _stream()))
     return out
+
+
+def _paged_attention_kv8_seq(query, kv_cache, block_table, context_len, scale):
+    """paged_attention on an 8-bit cache: the checks of nvllm_paged_attention_seq, then the batched
+    operator over the one table (uploaded here)."""
+    from . import kv8
+    kc = kv_cache.key_cache()
+    ids = block_table.get_physical_block_ids()
+    if not ids:  # paged.rs:133-137
+        raise ConfigError(capi.NVLLM_ERR_CONFIG, "BlockTable is empty - no blocks allocated")
+    if block_table.block_size() != kc.shape[1]:
+        raise ConfigError(capi.NVLLM_ERR_CONFIG, "block_size mismatch")
+    if query.shape[0] != 1:
+        raise TensorError(capi.NVLLM_ERR_TENSOR, "paged_attention: query batch must be 1")
+    if max(ids) >= kc.shape[0]:
+        raise TensorError(capi.NVLLM_ERR_TENSOR, "paged_attention: block id out of range")
+    if not 0 < context_len <= len(ids) * kc.shape[1]:
+        raise TensorError(capi.NVLLM_ERR_TENSOR, "paged_attention: context_len exceeds allocated blocks")
+    if query.shape[1] > context_len:
+        raise TensorError(capi.NVLLM_ERR_TENSOR, "paged_attention: num_new_tokens > context_len")
+    table = torch.tensor([ids], dtype=torch.int32).to(query.device)
+    lens = torch.tensor([context_len], dtype=torch.int32).to(query.device)
+    return kv8.paged_attention_kv8(query, kc, kv_cache.value_cache(), kv_cache.key_scales(), kv_cache.value_scales(),
+                                   table, lens, scale)
 
 
 PAGED_PATHS = ("decode", "k1_paged", "generic", "paged_mid")
@@ -150,6 +182,7 @@ def paged_attention_batched(query, key_cache, value_cache, block_tables, context
     """Batched form (nvllm_paged_attn_*): query [num_seqs,T,Hq,D], block_tables int32
     [num_seqs,max_blocks], context_lens int32 [num_seqs] -> [num_seqs,T,Hq*D]."""
     _require_device(query, key_cache, value_cache, block_tables, context_lens)
+    _require_wide(key_cache, value_cache)
     N, T, Hq, D = query.shape
     nb, bs, Hkv, _ = key_cache.shape
     assert block_tables.dtype == torch.int32 and context_lens.dtype == torch.int32
@@ -171,6 +204,7 @@ def reshape_and_cache(key, value, key_cache, value_cache, slot_mapping):
     """Batched KV write (nvllm_reshape_and_cache_*): key/value [num_tokens,Hkv,D],
     slot_mapping int64 [num_tokens] ON DEVICE; in place."""
     _require_device(key, value, key_cache, value_cache, slot_mapping)
+    _require_wide(key_cache, value_cache)
     assert slot_mapping.dtype == torch.int64
     n, Hkv, D = key.shape
     nb, bs = key_cache.shape[0], key_cache.shape[1]
@@ -211,6 +245,7 @@ def qk_norm_rope_cache(query, key, value, q_weight, k_weight, eps, rotary, posit
     Returns q_out (query itself unless q_out is given)."""
     _require_device(query, key, value, q_weight, k_weight, positions, key_cache, value_cache,
                     slot_mapping)
+    _require_wide(key_cache, value_cache)
     assert positions.dtype == torch.int32 and slot_mapping.dtype == torch.int64
     n, Hq, D = query.shape
     Hkv = key.shape[1]
@@ -232,6 +267,7 @@ def write_kv_to_cache(key, value, key_cache, value_cache, slot_mapping, block_si
     """paged.rs:208-215: key/value [1,S,Hkv,D], HOST slot mapping (list of ints).
     Updates the caches in place and returns them."""
     _require_device(key, value, key_cache, value_cache)
+    _require_wide(key_cache, value_cache)
     _, S, Hkv, D = key.shape
     slots = np.ascontiguousarray(slot_mapping, dtype=np.int64)
     scratch = torch.empty(max(S, 1) * 8, dtype=torch.uint8, device=key.device)

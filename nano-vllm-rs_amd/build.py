@@ -22,8 +22,11 @@ SOURCES = [
     "paged_attn_mid.hip",
     "flash_attn.hip",
     "flash_attn_mfma.hip",
+    "capi_kv8.cpp",
+    "kv8_write.hip",
+    "paged_attn_kv8.hip",
 ]
-HEADERS = ["nvllm_host.hpp", "nvllm_sched.hpp", "nvllm_kernels.hpp", os.path.join("..", "..", "include", "nvllm_attn.h")]
+HEADERS = ["nvllm_host.hpp", "nvllm_sched.hpp", "nvllm_kernels.hpp", "kv8_common.hpp", os.path.join("..", "..", "include", "nvllm_attn.h")]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-function",
          "-fno-gpu-rdc",

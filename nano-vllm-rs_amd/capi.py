@@ -38,6 +38,14 @@ SIGNATURES = {
     "nvllm_reshape_and_cache_f32": (_i, [_vp, _vp, _vp, _vp, _vp, _i64, _i, _i, _i, _i64, _vp]),
     "nvllm_qk_norm_rope_cache_bf16": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _f, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _i, _i, _i, _i, _i64, _vp]),
     "nvllm_qk_norm_rope_cache_f32": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _f, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _i, _i, _i, _i, _i64, _vp]),
+    "nvllm_kv8_write_workspace_bytes": (_sz, [_i64, _i, _i64]),
+    "nvllm_reshape_and_cache_kv8": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _i64, _i, _i, _i, _i64, _i, _i, _vp]),
+    "nvllm_qk_norm_rope_cache_kv8": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _f, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _i64, _i, _i, _i, _i, _i64, _i, _i, _vp]),
+    "nvllm_gather_cache_blocks_kv8": (_i, [_vp, _vp, _vp, _vp, _vp, _i64, _vp, _vp, _i64, _i, _i, _i, _i, _i, _vp]),
+    "nvllm_paged_attn_kv8": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _i, _i, _i, _i, _i, _i, _i, _i64, _f, _i, _i, _vp]),
+    "nvllm_paged_attn_kv8_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i, _i, _i]),
+    "nvllm_paged_attn_kv8_path": (_i, [_i, _i, _i, _i, _i, _i, _i, _i]),
+    "nvllm_kv_cache_kv8_layer_bytes": (_i64, [_i64, _i64, _i64, _i64]),
     "nvllm_rope_cache_f32": (_i, [_i64, _i64, _d, _vp, _vp]),
     "nvllm_get_last_error": (_c.c_char_p, []),
     "nvllm_synchronize": (_i, []),

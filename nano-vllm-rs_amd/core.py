@@ -209,8 +209,22 @@ class BlockManager:
         capi.lib().nvllm_block_manager_reset(self._h)
 
 
+class _Kv8Formats(dict):
+    """cache dtype -> format code of the 8-bit entries (filled on first use: torch is imported late)"""
+
+    def __contains__(self, dtype):
+        if not self:
+            import torch
+            self.update({torch.int8: 0, torch.float8_e4m3fn: 1})
+        return dict.__contains__(self, dtype)
+
+
+KV8_FORMATS = _Kv8Formats()
+
+
 class KVCacheConfig:
-    """kv_cache.rs:21-71 (dtype: a torch dtype; the reference defaults to F32, :51)."""
+    """kv_cache.rs:21-71 (dtype: a torch dtype; the reference defaults to F32, :51).  torch.int8 and
+    torch.float8_e4m3fn make an 8-bit cache (module `kv8`): codes and a scale for each block and head."""
 
     def __init__(self, num_blocks, block_size, num_kv_heads, head_dim, num_layers, dtype=None):
         import torch
@@ -233,13 +247,18 @@ class KVCacheConfig:
         return codes[self.dtype]
 
     def layer_cache_size_bytes(self):
-        """kv_cache.rs:62-65 (nvllm_kv_cache_layer_bytes)."""
+        """kv_cache.rs:62-65 (nvllm_kv_cache_layer_bytes); codes and scales of an 8-bit cache."""
+        if self.dtype in KV8_FORMATS:
+            return int(capi.lib().nvllm_kv_cache_kv8_layer_bytes(self.num_blocks, self.block_size,
+                                                                 self.num_kv_heads, self.head_dim))
         return int(capi.lib().nvllm_kv_cache_layer_bytes(self.num_blocks, self.block_size,
                                                          self.num_kv_heads, self.head_dim,
                                                          self._dtype_code()))
 
     def total_cache_size_bytes(self):
         """kv_cache.rs:68-70 (nvllm_kv_cache_total_bytes)."""
+        if self.dtype in KV8_FORMATS:
+            return 2 * self.num_layers * self.layer_cache_size_bytes()
         return int(capi.lib().nvllm_kv_cache_total_bytes(self.num_blocks, self.block_size,
                                                          self.num_kv_heads, self.head_dim,
                                                          self.num_layers, self._dtype_code()))
@@ -247,7 +266,7 @@ class KVCacheConfig:
 
 class LayerKVCache:
     """kv_cache.rs:75-206: zero-initialised K and V [num_blocks, block_size, Hkv, D],
-    resident in HBM (torch only provides the allocation)."""
+    resident in HBM (torch only provides the allocation).  An 8-bit cache has scales beside them."""
 
     def __init__(self, config, device):
         import torch
@@ -255,6 +274,10 @@ class LayerKVCache:
         self.config = config
         self._key_cache = torch.zeros(shape, dtype=config.dtype, device=device)
         self._value_cache = torch.zeros(shape, dtype=config.dtype, device=device)
+        self._key_scales = self._value_scales = None
+        if config.dtype in KV8_FORMATS:
+            self._key_scales = torch.zeros((shape[0], shape[2]), dtype=torch.float32, device=device)
+            self._value_scales = torch.zeros_like(self._key_scales)
 
     def key_cache(self):
         return self._key_cache
@@ -262,11 +285,29 @@ class LayerKVCache:
     def value_cache(self):
         return self._value_cache
 
+    def key_scales(self):
+        """f32 [num_blocks, Hkv] of an 8-bit cache, else None"""
+        return self._key_scales
+
+    def value_scales(self):
+        return self._value_scales
+
     def _gather(self, cache, block_ids):
         import torch
         if len(block_ids) == 0:  # kv_cache.rs:124-126
             raise ConfigError(capi.NVLLM_ERR_CONFIG, "block_ids cannot be empty")
         c = self.config
+        if c.dtype in KV8_FORMATS:  # the values, in bfloat16 (which holds them exactly)
+            scales = self._key_scales if cache is self._key_cache else self._value_scales
+            ids = torch.tensor([int(b) for b in block_ids], dtype=torch.int32, device=cache.device)
+            out = torch.empty((len(block_ids), c.block_size, c.num_kv_heads, c.head_dim), dtype=torch.bfloat16,
+                              device=cache.device)
+            st = torch.cuda.current_stream(cache.device).cuda_stream
+            with torch.cuda.device(cache.device):
+                check(capi.lib().nvllm_gather_cache_blocks_kv8(
+                    cache.data_ptr(), None, scales.data_ptr(), None, ids.data_ptr(), len(block_ids), out.data_ptr(),
+                    None, c.num_blocks, c.block_size, c.num_kv_heads, c.head_dim, KV8_FORMATS[c.dtype], 0, st))
+            return out
         ids = torch.tensor([int(b) for b in block_ids], dtype=torch.int32, device=cache.device)
         out = torch.empty((len(block_ids), c.block_size, c.num_kv_heads, c.head_dim), dtype=c.dtype,
                           device=cache.device)

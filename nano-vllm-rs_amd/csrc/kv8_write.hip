@@ -1,0 +1,361 @@
+// kv8_write.hip -- writing and reading the 8-bit KV cache (gfx950): the quantising forms of
+// reshape_and_cache (K4), of the producer (K5), and of the block gather.
+//
+// The number formats and the scale's formula are in kv8_common.hpp.  What a write does to a block:
+// let W be the rows (slots of the block) that the call writes and need = scale_of(max |x| over W).
+//   W holds the block's row 0:  scale' = need.  The block begins; what it held is gone.
+//   otherwise:                  scale' = max(scale, need).  If that grew, the codes of the rows not
+//                               in W are rounded to the new scale.
+//   code(x) = round(x / scale') for the rows in W.
+// Blocks are filled in order (BlockTable::get_slot_mapping, reference src/core/block.rs:269-283), so
+// row 0 is written exactly when a block comes fresh from the allocator: no call has to reset scales.
+//
+// The scale couples all tokens that a call puts into one block, and a slot mapping may name them in
+// any order.  So each block gets ONE owner: the token that writes its lowest row in this call.  The
+// owner's wave finds the block's other tokens, takes the maximum, and writes codes and scale; no
+// atomics on the cache, and of tokens that name the same slot the last one wins, as in a sequential
+// loop (the reference's, src/attention/paged.rs:231-262).
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+#include "kv8_common.hpp"
+
+namespace nvllm {
+namespace kernels {
+
+namespace {
+
+using namespace kv8;
+
+constexpr int kThreads = 256;
+constexpr int kWaves = kThreads / 64;
+constexpr int kMaxChunk = 16;  // tokens a workgroup looks after
+
+// Up to this many tokens every workgroup reads the whole slot mapping to find its blocks' tokens;
+// above, a launch in front leaves slot -> token in the workspace.
+constexpr int64_t kScanTokens = 4096;
+
+// slot -> token for every slot the call writes.  Nothing is cleared first: an entry counts only if
+// the token it names writes that very slot, so whatever else the workspace holds is seen through.
+// The last token that names a slot wins, by compare-and-swap.
+__global__ __launch_bounds__(kThreads) void kv8_index_kernel(const int64_t *__restrict__ slots, int n,
+                                                             int64_t num_slots, int32_t *index) {
+    const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+    if (i >= n) return;
+    const int t = (int)i;
+    const int64_t s = slots[t];
+    if (s < 0 || s >= num_slots) return;
+    int seen = index[s];
+    while (!(seen >= t && seen < n && slots[seen] == s)) {
+        const int was = atomicCAS(index + s, seen, t);
+        if (was == seen) break;
+        seen = was;
+    }
+}
+
+// The blocks that the chunk's tokens own.  LDS: map[c * bs + o] = the token of this call that writes
+// row o of token c's block (-1: none), owner[0 .. count) = the chunk's owning tokens.
+struct Chunk {
+    int *map;
+    int *owner;
+    int64_t *block;  // block id of each token of the chunk, -1 where its slot is not valid
+};
+
+__device__ __forceinline__ int find_blocks(const Chunk &ch, const int64_t *__restrict__ slots, int n, int t0,
+                                           int chunk, int bs, int64_t num_slots,
+                                           const int32_t *__restrict__ index) {
+    __shared__ int count;
+    const int tid = threadIdx.x;
+    if (tid < chunk) {
+        int64_t b = -1;
+        if (t0 + tid < n) {
+            const int64_t s = slots[t0 + tid];
+            if (s >= 0 && s < num_slots) b = s / bs;
+        }
+        ch.block[tid] = b;
+    }
+    if (tid == 0) count = 0;
+    if (index) {
+        __syncthreads();
+        for (int i = tid; i < chunk * bs; i += kThreads) {
+            const int c = i / bs;
+            const int64_t b = ch.block[c];
+            int e = -1;
+            if (b >= 0) {
+                const int64_t s = b * bs + (i - c * bs);
+                e = index[s];
+                if (e < 0 || e >= n || slots[e] != s) e = -1;
+            }
+            ch.map[i] = e;
+        }
+    } else {
+        for (int i = tid; i < chunk * bs; i += kThreads) ch.map[i] = -1;
+        __syncthreads();
+        for (int t = tid; t < n; t += kThreads) {
+            const int64_t s = slots[t];
+            if (s < 0 || s >= num_slots) continue;
+            const int64_t b = s / bs;
+            for (int c = 0; c < chunk; ++c)
+                if (ch.block[c] == b) atomicMax(ch.map + c * bs + (int)(s - b * bs), t);
+        }
+    }
+    __syncthreads();
+    if (tid < chunk && ch.block[tid] >= 0) {
+        int o = 0;
+        while (o < bs - 1 && ch.map[tid * bs + o] < 0) ++o;
+        if (ch.map[tid * bs + o] == t0 + tid) ch.owner[atomicAdd(&count, 1)] = tid;
+    }
+    __syncthreads();
+    return count;
+}
+
+// Scale and codes of one (block, kv head) of K or V by one wave, any head_dim and block_size.
+// row(t) is called by the whole wave and returns a functor d -> value of token t's row.
+template <Kv8Format F, typename Row>
+__device__ __forceinline__ void write_unit(const int *map, int bs, int D, int Hkv, int64_t block, int head,
+                                           unsigned char *cache, float *scales, const Row &row) {
+    const int lane = threadIdx.x & 63;
+    float amax = 0.0f;
+    for (int o = 0; o < bs; ++o) {
+        const int t = map[o];
+        if (t < 0) continue;
+        const auto x = row(t);
+        for (int d = lane; d < D; d += 64) amax = fmaxf(amax, finite_abs(x(d)));
+    }
+    const float need = scale_of<F>(wave_max(amax));
+    const bool begins = map[0] >= 0;
+    float *sp = scales + block * Hkv + head;
+    const float was = begins ? 0.0f : *sp;
+    const float s = fmaxf(was, need);
+    const float inv = inverse_scale(s);
+    unsigned char *base = cache + (block * bs * Hkv + head) * (int64_t)D;
+    for (int o = 0; o < bs; ++o) {
+        unsigned char *out = base + (int64_t)o * Hkv * D;
+        const int t = map[o];
+        if (t >= 0) {
+            const auto x = row(t);
+            for (int d = lane; d < D; d += 64) out[d] = encode1<F>(x(d) * inv);
+        } else if (!begins && s > was) {
+            const float ratio = was * inv;
+            for (int d = lane; d < D; d += 64) out[d] = (unsigned char)rescale4<F>(out[d], ratio);
+        }
+    }
+    if (lane == 0 && (begins || s > was)) *sp = s;
+}
+
+// Norm and rotation of one row by one wave: x / sqrt(mean(x^2) + eps) * weight, then the rotation of
+// the pairs (d, d + D/2).  AT: f32 for bf16 tensors; f64 for f32 ones, where a value that f32 leaves on the other
+// side of a code's border would show as a whole step.
+template <typename ET, typename AT> struct RotatedRow {
+    const ET *x, *w, *c, *s;
+    int half;
+    AT inv;
+    __device__ __forceinline__ AT operator()(int d) const {
+        const int lo = d < half ? d : d - half;
+        const AT a = (AT)to_f32(x[lo]) * inv * (AT)to_f32(w[lo]);
+        const AT b = (AT)to_f32(x[lo + half]) * inv * (AT)to_f32(w[lo + half]);
+        return d < half ? a * (AT)to_f32(c[d]) - b * (AT)to_f32(s[d]) : b * (AT)to_f32(c[d]) + a * (AT)to_f32(s[d]);
+    }
+};
+
+template <typename ET, typename AT>
+__device__ __forceinline__ RotatedRow<ET, AT> rotated_row(const ET *x, const ET *w, const ET *cos_cache,
+                                                          const ET *sin_cache, int pos, int max_pos, int D, float eps) {
+    const int lane = threadIdx.x & 63;
+    pos = pos < 0 ? 0 : (pos >= max_pos ? max_pos - 1 : pos);  // never read outside the tables
+    AT ss = 0;
+    for (int d = lane; d < D; d += 64) ss += (AT)to_f32(x[d]) * (AT)to_f32(x[d]);
+#pragma unroll
+    for (int m = 32; m > 0; m >>= 1) ss += __shfl_xor(ss, m);
+    return {x, w, cos_cache + (int64_t)pos * D, sin_cache + (int64_t)pos * D, D / 2,
+            (AT)1 / (AT)sqrt((AT)(ss / (AT)D + (AT)eps))};
+}
+
+template <typename ET> struct PlainRow {
+    const ET *x;
+    __device__ __forceinline__ float operator()(int d) const { return to_f32(x[d]); }
+};
+
+// Any head_dim and block_size.  Workgroups [0, row_blocks) normalise and rotate rows of Q (and of K
+// to k_out, if asked), one a wave; the rest look after `chunk` tokens' cache blocks each.
+template <typename ET, Kv8Format F, bool PRODUCER>
+__global__ __launch_bounds__(kThreads) void kv8_write_generic_kernel(const Kv8WriteArgs a, int chunk, int row_blocks,
+                                                                     bool indexed) {
+    typedef typename std::conditional<sizeof(ET) == 4, double, float>::type AT;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int D = a.head_dim, Hkv = a.num_kv_heads, Hq = a.num_heads;
+    const ET *key = static_cast<const ET *>(a.key), *value = static_cast<const ET *>(a.value);
+    if constexpr (PRODUCER) {
+        if ((int)blockIdx.x < row_blocks) {
+            const int heads = Hq + (a.k_out ? Hkv : 0);
+            const int64_t r = (int64_t)blockIdx.x * kWaves + wave;
+            const int64_t t = r / heads;
+            if (t >= a.num_tokens) return;
+            const int h = (int)(r - t * heads);
+            const ET *x = h < Hq ? static_cast<const ET *>(a.q) + (t * Hq + h) * D : key + (t * Hkv + h - Hq) * D;
+            ET *y = h < Hq ? static_cast<ET *>(a.q_out) + (t * Hq + h) * D
+                           : static_cast<ET *>(a.k_out) + (t * Hkv + h - Hq) * D;
+            const auto row = rotated_row<ET, AT>(x, static_cast<const ET *>(h < Hq ? a.q_weight : a.k_weight),
+                                                 static_cast<const ET *>(a.cos_cache),
+                                                 static_cast<const ET *>(a.sin_cache), a.positions[t], a.max_positions,
+                                                 D, a.eps);
+            for (int d = lane; d < D / 2; d += 64) {  // both of a pair are read before either is written: y may be x
+                const ET lo = static_cast<ET>((float)row(d)), hi = static_cast<ET>((float)row(d + D / 2));
+                y[d] = lo;
+                y[d + D / 2] = hi;
+            }
+            return;
+        }
+    }
+    extern __shared__ int dyn[];
+    __shared__ int owner[kMaxChunk];
+    __shared__ int64_t block[kMaxChunk];
+    const Chunk ch{dyn, owner, block};
+    const int bs = a.block_size, n = (int)a.num_tokens, t0 = ((int)blockIdx.x - row_blocks) * chunk;
+    const int count = find_blocks(ch, a.slot_mapping, n, t0, chunk, bs, a.num_cache_blocks * bs,
+                                  indexed ? a.workspace : nullptr);
+    for (int u = wave; u < count * Hkv * 2; u += kWaves) {
+        const int i = u / (2 * Hkv), head = u % Hkv;
+        const bool is_v = (u / Hkv) & 1;
+        const int c = owner[i];
+        const int *map = dyn + c * bs;
+        unsigned char *cache = static_cast<unsigned char *>(is_v ? a.v_cache : a.k_cache);
+        float *scales = is_v ? a.v_scales : a.k_scales;
+        if (PRODUCER && !is_v)
+            write_unit<F>(map, bs, D, Hkv, block[c], head, cache, scales, [&](int t) {
+                return rotated_row<ET, AT>(key + ((int64_t)t * Hkv + head) * D, static_cast<const ET *>(a.k_weight),
+                                           static_cast<const ET *>(a.cos_cache), static_cast<const ET *>(a.sin_cache),
+                                           a.positions[t], a.max_positions, D, a.eps);
+            });
+        else
+            write_unit<F>(map, bs, D, Hkv, block[c], head, cache, scales, [&](int t) {
+                return PlainRow<ET>{(is_v ? value : key) + ((int64_t)t * Hkv + head) * D};
+            });
+    }
+}
+
+template <typename ET, Kv8Format F>
+hipError_t launch_generic(const Kv8WriteArgs &a, bool indexed, hipStream_t stream) {
+    int chunk = kMaxChunk;
+    while (chunk > 1 && a.num_tokens / chunk < 512) chunk /= 2;
+    const int64_t chunks = (a.num_tokens + chunk - 1) / chunk;
+    const size_t lds = (size_t)chunk * a.block_size * sizeof(int);
+    if (a.q) {
+        const int64_t rows = a.num_tokens * (a.num_heads + (a.k_out ? a.num_kv_heads : 0));
+        const int64_t row_blocks = (rows + kWaves - 1) / kWaves;
+        if (row_blocks + chunks > 0x7fffffffLL) return hipErrorInvalidValue;
+        kv8_write_generic_kernel<ET, F, true><<<dim3((unsigned)(row_blocks + chunks)), dim3(kThreads), lds, stream>>>(
+            a, chunk, (int)row_blocks, indexed);
+    } else {
+        kv8_write_generic_kernel<ET, F, false><<<dim3((unsigned)chunks), dim3(kThreads), lds, stream>>>(a, chunk, 0,
+                                                                                                     indexed);
+    }
+    return hipGetLastError();
+}
+
+// Read-back of whole blocks: out[i] = codes of block ids[i] times its scales, in bf16 (exact) or f32.
+// Eight values a thread (D a multiple of 8), else one; blockIdx.y takes K and V.
+// Ids outside the pool give zeros.
+template <typename ET, Kv8Format F, int V>
+__global__ __launch_bounds__(256) void kv8_gather_kernel(const unsigned char *__restrict__ k_cache,
+                                                         const unsigned char *__restrict__ v_cache,
+                                                         const float *__restrict__ k_scales,
+                                                         const float *__restrict__ v_scales,
+                                                         const int32_t *__restrict__ ids, ET *__restrict__ k_out,
+                                                         ET *__restrict__ v_out, int64_t total, int block_vec,
+                                                         int Hkv, int D, int64_t num_cache_blocks) {
+    const int64_t g = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (g >= total) return;
+    const bool is_v = blockIdx.y;
+    const unsigned char *cache = is_v ? v_cache : k_cache;
+    ET *out = (is_v ? v_out : k_out) + g * V;
+    const int64_t i = total <= 0xffffffffLL ? (int64_t)((unsigned)g / (unsigned)block_vec) : g / block_vec;
+    const int idx = (int)(g - i * block_vec) * V;
+    const int64_t id = ids[i];
+    float x[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) x[j] = 0.0f;
+    if (id >= 0 && id < num_cache_blocks) {
+        const float s = (is_v ? v_scales : k_scales)[id * Hkv + (idx / D) % Hkv];
+        const unsigned char *p = cache + id * ((int64_t)block_vec * V) + idx;
+        if constexpr (V == 8) {
+            const u32x2 w = *reinterpret_cast<const u32x2 *>(p);
+            decode4<F>(w[0], x);
+            decode4<F>(w[1], x + 4);
+        } else {
+            x[0] = decode1<F>(*p);
+        }
+#pragma unroll
+        for (int j = 0; j < V; ++j) x[j] *= s;
+    }
+    if constexpr (V == 8 && sizeof(ET) == 2) {
+        const u32x4 y = {pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]),
+                         pack_bf16x2(x[6], x[7])};
+        __builtin_nontemporal_store(y, reinterpret_cast<u32x4 *>(out));
+    } else if constexpr (V == 8) {
+        __builtin_nontemporal_store(f32x4{x[0], x[1], x[2], x[3]}, reinterpret_cast<f32x4 *>(out));
+        __builtin_nontemporal_store(f32x4{x[4], x[5], x[6], x[7]}, reinterpret_cast<f32x4 *>(out) + 1);
+    } else {
+        *out = static_cast<ET>(x[0]);
+    }
+}
+
+template <typename ET, Kv8Format F, int V>
+hipError_t launch_gather(const void *k_cache, const void *v_cache, const float *k_scales, const float *v_scales,
+                         const int32_t *ids, int64_t num_ids, void *k_out, void *v_out, int64_t num_cache_blocks,
+                         int block_size, int Hkv, int D, hipStream_t stream) {
+    const int64_t vec = (int64_t)block_size * Hkv * D / V, total = num_ids * vec, blocks = (total + 255) / 256;
+    if (vec * V > 0x7fffffffLL || blocks > 0x7fffffffLL) return hipErrorInvalidValue;
+    kv8_gather_kernel<ET, F, V><<<dim3((unsigned)blocks, v_out ? 2 : 1), dim3(256), 0, stream>>>(
+        static_cast<const unsigned char *>(k_cache), static_cast<const unsigned char *>(v_cache), k_scales, v_scales,
+        ids, static_cast<ET *>(k_out), static_cast<ET *>(v_out), total, (int)vec, Hkv, D, num_cache_blocks);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+size_t kv8_write_workspace_bytes(int64_t num_tokens, int block_size, int64_t num_cache_blocks) {
+    return num_tokens > kScanTokens ? (size_t)num_cache_blocks * block_size * sizeof(int32_t) : 0;
+}
+
+hipError_t launch_kv8_write(DType dt, Kv8Format fmt, const Kv8WriteArgs &a, hipStream_t stream) {
+    if (a.num_tokens <= 0) return hipSuccess;
+    const bool indexed = kv8_write_workspace_bytes(a.num_tokens, a.block_size, a.num_cache_blocks) > 0;
+    if (indexed) {
+        if (!a.workspace) return hipErrorInvalidValue;
+        kv8_index_kernel<<<dim3((unsigned)((a.num_tokens + kThreads - 1) / kThreads)), dim3(kThreads), 0, stream>>>(
+            a.slot_mapping, (int)a.num_tokens, a.num_cache_blocks * a.block_size, a.workspace);
+        const hipError_t err = hipGetLastError();
+        if (err != hipSuccess) return err;
+    }
+    if (dt == DType::BF16)
+        return fmt == Kv8Format::Int8 ? launch_generic<__bf16, Kv8Format::Int8>(a, indexed, stream)
+                                      : launch_generic<__bf16, Kv8Format::E4M3>(a, indexed, stream);
+    return fmt == Kv8Format::Int8 ? launch_generic<float, Kv8Format::Int8>(a, indexed, stream)
+                                  : launch_generic<float, Kv8Format::E4M3>(a, indexed, stream);
+}
+
+hipError_t launch_kv8_gather(DType dt, Kv8Format fmt, const void *k_cache, const void *v_cache,
+                             const float *k_scales, const float *v_scales, const int32_t *ids, int64_t num_ids,
+                             void *k_out, void *v_out, int64_t num_cache_blocks, int block_size, int num_kv_heads,
+                             int head_dim, hipStream_t stream) {
+    if (num_ids <= 0) return hipSuccess;
+    const auto at = [](const void *p, unsigned n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; };
+    const bool wide = head_dim % 8 == 0 && at(k_cache, 8) && at(v_cache, 8) && at(k_out, 16) && at(v_out, 16);
+#define NVLLM_KV8_GATHER(ET, F)                                                                                  \
+    return wide ? launch_gather<ET, F, 8>(k_cache, v_cache, k_scales, v_scales, ids, num_ids, k_out, v_out,      \
+                                          num_cache_blocks, block_size, num_kv_heads, head_dim, stream)          \
+                : launch_gather<ET, F, 1>(k_cache, v_cache, k_scales, v_scales, ids, num_ids, k_out, v_out,      \
+                                          num_cache_blocks, block_size, num_kv_heads, head_dim, stream)
+    if (dt == DType::BF16) {
+        if (fmt == Kv8Format::Int8) NVLLM_KV8_GATHER(__bf16, Kv8Format::Int8);
+        NVLLM_KV8_GATHER(__bf16, Kv8Format::E4M3);
+    }
+    if (fmt == Kv8Format::Int8) NVLLM_KV8_GATHER(float, Kv8Format::Int8);
+    NVLLM_KV8_GATHER(float, Kv8Format::E4M3);
+#undef NVLLM_KV8_GATHER
+}
+
+}  // namespace kernels
+}  // namespace nvllm

@@ -82,6 +82,45 @@ struct QkNormRopeCacheArgs {
 };
 hipError_t launch_qk_norm_rope_cache(DType dt, const QkNormRopeCacheArgs &a, hipStream_t stream);
 
+// 8-bit KV cache: number format of the codes (kv8_common.hpp)
+enum class Kv8Format : int { Int8 = 0, E4M3 = 1 };
+constexpr int kKv8MaxBlockSize = 256;
+
+// K4 / K5 with quantisation, and the read-back (kv8_write.hip)
+struct Kv8WriteArgs {
+    const void *key;
+    const void *value;
+    void *k_cache;
+    void *v_cache;
+    float *k_scales;
+    float *v_scales;
+    const int64_t *slot_mapping;
+    int32_t *workspace;  // slot -> token, where kv8_write_workspace_bytes() > 0
+    int64_t num_tokens;
+    int num_kv_heads;
+    int head_dim;
+    int block_size;
+    int64_t num_cache_blocks;
+    // producer only (q == nullptr: plain write)
+    const void *q;
+    void *q_out;
+    void *k_out;  // optional
+    const void *q_weight;
+    const void *k_weight;
+    float eps;
+    const void *cos_cache;
+    const void *sin_cache;
+    int max_positions;
+    const int32_t *positions;
+    int num_heads;
+};
+size_t kv8_write_workspace_bytes(int64_t num_tokens, int block_size, int64_t num_cache_blocks);
+hipError_t launch_kv8_write(DType dt, Kv8Format fmt, const Kv8WriteArgs &a, hipStream_t stream);
+hipError_t launch_kv8_gather(DType dt, Kv8Format fmt, const void *k_cache, const void *v_cache,
+                             const float *k_scales, const float *v_scales, const int32_t *ids,
+                             int64_t num_ids, void *k_out, void *v_out, int64_t num_cache_blocks,
+                             int block_size, int num_kv_heads, int head_dim, hipStream_t stream);
+
 // K2/K2b/K3: paged_attn.hip
 struct PagedAttnArgs {
     const void *q;
@@ -125,6 +164,12 @@ hipError_t launch_paged_attn(DType dt, const PagedAttnArgs &a, hipStream_t strea
 constexpr size_t kNoAllocScratchBytes = (size_t)32 << 20;
 hipError_t launch_paged_attn_noalloc(DType dt, const PagedAttnArgs &a, hipStream_t stream);
 hipError_t noalloc_prepare_device();  // looks the scratch address of the current device up once
+// attention over the 8-bit cache (paged_attn_kv8.hip); `a.k_cache` / `a.v_cache` hold codes
+enum class PagedKv8Path : int { Decode = 0, Generic = 2 };
+PagedKv8Path paged_attn_kv8_path(DType dt, const PagedAttnArgs &a);
+size_t paged_attn_kv8_workspace_bytes(DType dt, const PagedAttnArgs &a);
+hipError_t launch_paged_attn_kv8(DType dt, Kv8Format fmt, const PagedAttnArgs &a, const float *k_scales,
+                                 const float *v_scales, hipStream_t stream);
 // K1 over the paged cache (flash_attn_mfma.hip): chunked prefill / verify with more than 32 query
 // rows per kv head; launch_paged_attn dispatches to it
 bool flash_attn_paged_supported(DType dt, const PagedAttnArgs &a);

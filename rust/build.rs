@@ -17,6 +17,9 @@ const SOURCES: &[&str] = &[
     "paged_attn_mid.hip",
     "flash_attn.hip",
     "flash_attn_mfma.hip",
+    "capi_kv8.cpp",
+    "kv8_write.hip",
+    "paged_attn_kv8.hip",
 ];
 
 fn main() {

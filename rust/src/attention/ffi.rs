@@ -68,6 +68,14 @@ extern "C" {
     pub fn nvllm_gather_cache_blocks(cache: *const c_void, block_ids: *const i32, num_ids: i64, out: *mut c_void, num_cache_blocks: i64, block_size: c_int, num_kv_heads: c_int, head_dim: c_int, dtype: c_int, stream: Stream) -> c_int;
     pub fn nvllm_qk_norm_rope_cache_bf16(q: *const c_void, k: *const c_void, v: *const c_void, q_out: *mut c_void, k_out: *mut c_void, q_weight: *const c_void, k_weight: *const c_void, eps: f32, cos_cache: *const c_void, sin_cache: *const c_void, max_positions: i64, positions: *const i32, k_cache: *mut c_void, v_cache: *mut c_void, slot_mapping: *const i64, num_tokens: i64, num_heads: c_int, num_kv_heads: c_int, head_dim: c_int, block_size: c_int, num_cache_blocks: i64, stream: Stream) -> c_int;
     pub fn nvllm_qk_norm_rope_cache_f32(q: *const c_void, k: *const c_void, v: *const c_void, q_out: *mut c_void, k_out: *mut c_void, q_weight: *const c_void, k_weight: *const c_void, eps: f32, cos_cache: *const c_void, sin_cache: *const c_void, max_positions: i64, positions: *const i32, k_cache: *mut c_void, v_cache: *mut c_void, slot_mapping: *const i64, num_tokens: i64, num_heads: c_int, num_kv_heads: c_int, head_dim: c_int, block_size: c_int, num_cache_blocks: i64, stream: Stream) -> c_int;
+    pub fn nvllm_kv8_write_workspace_bytes(num_tokens: i64, block_size: c_int, num_cache_blocks: i64) -> usize;
+    pub fn nvllm_reshape_and_cache_kv8(key: *const c_void, value: *const c_void, k_cache: *mut c_void, v_cache: *mut c_void, k_scales: *mut f32, v_scales: *mut f32, slot_mapping: *const i64, workspace: *mut c_void, workspace_bytes: usize, num_tokens: i64, num_kv_heads: c_int, head_dim: c_int, block_size: c_int, num_cache_blocks: i64, format: c_int, dtype: c_int, stream: Stream) -> c_int;
+    pub fn nvllm_qk_norm_rope_cache_kv8(q: *const c_void, k: *const c_void, v: *const c_void, q_out: *mut c_void, k_out: *mut c_void, q_weight: *const c_void, k_weight: *const c_void, eps: f32, cos_cache: *const c_void, sin_cache: *const c_void, max_positions: i64, positions: *const i32, k_cache: *mut c_void, v_cache: *mut c_void, k_scales: *mut f32, v_scales: *mut f32, slot_mapping: *const i64, workspace: *mut c_void, workspace_bytes: usize, num_tokens: i64, num_heads: c_int, num_kv_heads: c_int, head_dim: c_int, block_size: c_int, num_cache_blocks: i64, format: c_int, dtype: c_int, stream: Stream) -> c_int;
+    pub fn nvllm_gather_cache_blocks_kv8(k_cache: *const c_void, v_cache: *const c_void, k_scales: *const f32, v_scales: *const f32, block_ids: *const i32, num_ids: i64, k_out: *mut c_void, v_out: *mut c_void, num_cache_blocks: i64, block_size: c_int, num_kv_heads: c_int, head_dim: c_int, format: c_int, dtype: c_int, stream: Stream) -> c_int;
+    pub fn nvllm_paged_attn_kv8(q: *const c_void, k_cache: *const c_void, v_cache: *const c_void, k_scales: *const f32, v_scales: *const f32, block_tables: *const i32, context_lens: *const i32, out: *mut c_void, workspace: *mut c_void, workspace_bytes: usize, num_seqs: c_int, num_new_tokens: c_int, num_heads: c_int, num_kv_heads: c_int, head_dim: c_int, block_size: c_int, max_blocks_per_seq: c_int, num_cache_blocks: i64, scale: f32, format: c_int, dtype: c_int, stream: Stream) -> c_int;
+    pub fn nvllm_paged_attn_kv8_workspace_bytes(num_seqs: c_int, num_new_tokens: c_int, num_heads: c_int, num_kv_heads: c_int, head_dim: c_int, block_size: c_int, max_blocks_per_seq: c_int, dtype: c_int) -> usize;
+    pub fn nvllm_paged_attn_kv8_path(num_seqs: c_int, num_new_tokens: c_int, num_heads: c_int, num_kv_heads: c_int, head_dim: c_int, block_size: c_int, max_blocks_per_seq: c_int, dtype: c_int) -> c_int;
+    pub fn nvllm_kv_cache_kv8_layer_bytes(num_blocks: i64, block_size: i64, num_kv_heads: i64, head_dim: i64) -> i64;
     pub fn nvllm_get_last_error() -> *const c_char;
     pub fn nvllm_synchronize() -> c_int;
     pub fn nvllm_kv_cache_layer_bytes(num_blocks: i64, block_size: i64, num_kv_heads: i64, head_dim: i64, dtype: c_int) -> i64;
