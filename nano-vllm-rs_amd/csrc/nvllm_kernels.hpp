@@ -159,6 +159,9 @@ hipError_t launch_paged_attn_mid(const PagedAttnArgs &a, hipStream_t stream);
 // what THIS launch needs (<= paged_attn_workspace_bytes of its shape: 0 when the generic kernel runs)
 size_t paged_attn_launch_workspace_bytes(DType dt, const PagedAttnArgs &a);
 hipError_t launch_paged_attn(DType dt, const PagedAttnArgs &a, hipStream_t stream);
+// split-K partials (f32 O [rows, splits, 128], then (m, l) [rows, splits, 2]) -> bf16 rows
+hipError_t launch_paged_attn_merge(const float *ws_o, const float *ws_ml, void *out, int64_t rows, int splits,
+                                   hipStream_t stream);
 // the same launch with the split-K scratch in a file-scope device array of paged_attn.hip
 // (a.workspace is ignored); launches that need more than kNoAllocScratchBytes are refused
 constexpr size_t kNoAllocScratchBytes = (size_t)32 << 20;

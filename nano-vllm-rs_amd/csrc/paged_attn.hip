@@ -801,6 +801,13 @@ size_t paged_attn_launch_workspace_bytes(DType dt, const PagedAttnArgs &a) {
                                       a.block_size, a.max_blocks_per_seq);
 }
 
+hipError_t launch_paged_attn_merge(const float *ws_o, const float *ws_ml, void *out, int64_t rows, int splits,
+                                   hipStream_t stream) {
+    paged_attn_merge_kernel<<<dim3((unsigned)rows), dim3(256), 0, stream>>>(ws_o, ws_ml, static_cast<__bf16 *>(out),
+                                                                            rows, splits);
+    return hipGetLastError();
+}
+
 hipError_t launch_paged_attn(DType dt, const PagedAttnArgs &a, hipStream_t stream) {
     if (a.num_seqs <= 0) return hipSuccess;
     if (launch_policy().paged_mid > 0 && use_mid(dt, a)) return launch_paged_attn_mid(a, stream);
@@ -847,12 +854,7 @@ hipError_t launch_paged_attn(DType dt, const PagedAttnArgs &a, hipStream_t strea
 #undef NVLLM_PAGED_CASE
         hipError_t err = hipGetLastError();
         if (err != hipSuccess) return err;
-        if (splits > 1) {
-            const dim3 grid((unsigned)rows), block(256);
-            paged_attn_merge_kernel<<<grid, block, 0, stream>>>(
-                ws_o, ws_ml, static_cast<__bf16 *>(a.out), (int64_t)rows, splits);
-            err = hipGetLastError();
-        }
+        if (splits > 1) err = launch_paged_attn_merge(ws_o, ws_ml, a.out, (int64_t)rows, splits, stream);
         return err;
     }
     if (use_mid(dt, a)) return launch_paged_attn_mid(a, stream);

@@ -135,7 +135,7 @@ __global__ __launch_bounds__(256) void paged_attn_kv8_generic_kernel(
         L += f * l_s[w];
         y += f * o_s[w][d];
     }
-    if (d < D) out[orow + d] = static_cast<ET>(L > 0.0f ? y / L : 0.0f);
+    if (d < D) out[orow + d] = static_cast<ET>(L == 0.0f ? 0.0f : y / L);  // no key seen: zeros
 }
 
 template <typename ET, Kv8Format F>
@@ -152,15 +152,453 @@ hipError_t launch_generic(const PagedAttnArgs &a, const float *ks, const float *
     return hipGetLastError();
 }
 
+// ---------------------------------------------------------------------------
+// Decode path: bf16, head_dim 128, block_size 16, up to 48 query rows (T * Hq/Hkv) per kv head.
+//
+// Bound by HBM: a cached token costs 2 * Hkv * 128 bytes, half of the bf16 cache's.  The work is cut as
+// in paged_attn.hip: grid (splits, sequences, kv-head groups), one wave per kv head of a workgroup, all
+// query rows of the head in one wave, no barriers; HPB waves walk the same table entries, so together
+// they read whole blocks.  What one byte a value changes:
+//   tile    32 keys (2 blocks), 8 KiB.  NBUF tiles in registers, all but one of them on their way;
+//   K       8 lanes x 16 B read a 128-byte row, 8 rows an instruction; through the wave's LDS image (16-byte
+//           chunk ch of row r at position ch ^ (r & 7): 8 rows x 1 chunk and 1 row x 8 chunks both touch
+//           all banks once).  A lane reads chunks 4i + g of row c: 16 dims = two MFMA k-steps of 8, so the
+//           dims are in an order of their own and Q's fragments follow it;
+//   V       the same image; ds_read_b64_tr_b8 gives a lane 8 keys of one dim.  Group g takes the keys that
+//           its scores are for (4g .. 4g+3 of two blocks), so P needs no lane movement;
+//   codes   become bf16 in registers, exactly (v_cvt_scalef32_pk_bf16_fp8, two a instruction; int8 by way of
+//           f32), and go to mfma_f32_16x16x32_bf16;
+//   scales  lane l of the wave holds id, K scale and V scale of block l of a run of 64; v_readlane makes
+//           them scalars at the tile that needs them.  The next run's are loaded 32 tiles ahead.
+// ---------------------------------------------------------------------------
+typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
+typedef __attribute__((ext_vector_type(2))) int i32x2;
+
+constexpr int kD = 128;
+constexpr int kBS = 16;
+constexpr int kTileBlocks = 2;
+constexpr int kTileKeys = kTileBlocks * kBS;
+constexpr int kImage = kTileKeys * kD;  // 4 KiB: one tile of K or of V
+constexpr int kRun = 64;                // blocks whose ids and scales a wave holds at once
+constexpr int kMaxDecodeRows = 48;
+
+__device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// 8 codes -> 8 bf16, exact
+template <Kv8Format F> __device__ __forceinline__ bf16x8 widen8(unsigned w0, unsigned w1) {
+    u32x4 r;
+    if constexpr (F == Kv8Format::E4M3) {
+        r[0] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w0, 1.0f, false));
+        r[1] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w0, 1.0f, true));
+        r[2] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w1, 1.0f, false));
+        r[3] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w1, 1.0f, true));
+    } else {
+        float x[8];
+        decode4<F>(w0, x);
+        decode4<F>(w1, x + 4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r[i] = pack_bf16x2(x[2 * i], x[2 * i + 1]);
+    }
+    return __builtin_bit_cast(bf16x8, r);
+}
+
+// hipcc leaves too few wait states between the last matrix instruction of a basic block and a read of
+// its result in the next one (seen here as wrong values of one accumulator register; tests/mfma_waits.py
+// finds such places in the assembly).  Behind code whose results leave a block: 8 wait states.
+__device__ __forceinline__ void settle() {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_nop 7");
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+struct Tile {
+    u32x4 k[kTileBlocks][2], v[kTileBlocks][2];  // [block][rows 0-7, 8-15]
+    float ks[kTileBlocks], vs[kTileBlocks];      // wave-uniform
+};
+
+// byte c of the result is 0xff where byte c of w is an E4M3 NaN (0x7f, 0xff)
+__device__ __forceinline__ unsigned nan_bytes(unsigned w) {
+    const unsigned t = (w & 0x7f7f7f7fu) + 0x01010101u;  // bit 7 of a byte: its low seven bits were all ones
+    return ((t & 0x80808080u) >> 7) * 0xffu;
+}
+
+template <Kv8Format F, int NQT, int HPB, int NBUF>
+__global__ __launch_bounds__(64 * HPB, NQT == 1 ? 2 : 1) void paged_attn_kv8_decode_kernel(
+    const __bf16 *__restrict__ q, const unsigned char *__restrict__ k_cache, const unsigned char *__restrict__ v_cache,
+    const float *__restrict__ k_scales, const float *__restrict__ v_scales, const int32_t *__restrict__ block_tables,
+    const int32_t *__restrict__ context_lens, __bf16 *__restrict__ out, float *__restrict__ ws_o,
+    float *__restrict__ ws_ml, int T, int Hq, int Hkv, int max_blocks_per_seq, int64_t num_cache_blocks,
+    float scale_log2e, int num_splits, int blocks_per_split, bool stream) {
+    __shared__ __attribute__((aligned(16))) unsigned char lds_all[HPB * 2 * kImage];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int g = lane >> 4, c = lane & 15;
+    const int split = blockIdx.x, seq = blockIdx.y;
+    const int kvh = blockIdx.z * HPB + wave;
+    if (kvh >= Hkv) return;  // whole wave; no barriers are used anywhere
+
+    const int G = Hq / Hkv, R = T * G;
+    int ctx = context_lens[seq];
+    const int64_t cap = (int64_t)max_blocks_per_seq * kBS;
+    if (ctx > cap) ctx = (int)cap;  // never read past the table row
+    const int nblk_seq = ctx > 0 ? (int)(((int64_t)ctx + kBS - 1) / kBS) : 0;
+    const int blk_begin = split * blocks_per_split;
+    int blk_end = blk_begin + blocks_per_split;
+    if (blk_end > nblk_seq) blk_end = nblk_seq;
+    const int ntiles = blk_end > blk_begin ? (blk_end - blk_begin + kTileBlocks - 1) / kTileBlocks : 0;
+    unsigned char *lds_k = lds_all + wave * 2 * kImage, *lds_v = lds_k + kImage;
+    const int32_t *table = block_tables + (int64_t)seq * max_blocks_per_seq;
+
+    // Q^T fragments (B operand): k-step 2i + h of lane (g, c) holds Q[row c][16 (4i + g) + 8h .. + 7]
+    bf16x8 qf[NQT][4];
+    int t_of_row[NQT];
+#pragma unroll
+    for (int qt = 0; qt < NQT; ++qt) {
+        const int r = qt * 16 + c;
+        const int t = r < R ? r / G : 0, hg = r < R ? r - t * G : 0;
+        t_of_row[qt] = t;
+        const __bf16 *qrow = q + (((int64_t)seq * T + t) * Hq + kvh * G + hg) * kD;
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            u32x4 x = {0u, 0u, 0u, 0u};
+            if (r < R) x = *reinterpret_cast<const u32x4 *>(qrow + 16 * (4 * (s >> 1) + g) + 8 * (s & 1));
+            qf[qt][s] = __builtin_bit_cast(bf16x8, x);
+        }
+    }
+
+    const int64_t block_bytes = (int64_t)kBS * Hkv * kD;
+    const unsigned row_stride = (unsigned)Hkv * kD;
+    const int lr = lane >> 3, lch = lane & 7;
+    const unsigned lane_off = (unsigned)lr * row_stride + (unsigned)kvh * kD + 16u * lch;
+    const unsigned wr = (unsigned)(lr * kD + 16 * (lch ^ lr));                    // + 2048 b + 1024 i
+    const unsigned krd0 = (unsigned)(c * kD + 16 * (g ^ (c & 7)));                // + 2048 b, chunk g
+    const unsigned krd1 = (unsigned)(c * kD + 16 * ((4 + g) ^ (c & 7)));          // chunk 4 + g
+    const int tr_q = c >> 1;                                                      // transposed read: its row
+    const int tr_row = (tr_q < 4 ? 0 : kBS) + 4 * g + (tr_q & 3);
+    const unsigned tr_base = (unsigned)(tr_row * kD + 8 * (c & 1));
+    const unsigned tr_sw = (unsigned)(tr_row & 7);
+
+    // ids and scales of the runs of 64 blocks.  Past the split's end: the last id (read, and masked), scale 0
+    auto run_ids = [&](int base) -> int {
+        int j = base + lane;
+        if (j >= blk_end) j = blk_end - 1;
+        return table[j];
+    };
+    auto clamp_id = [&](int id) -> int64_t {
+        int64_t x = id;
+        if (x < 0) x = 0;
+        if (x >= num_cache_blocks) x = num_cache_blocks - 1;
+        return x;
+    };
+    int id = 0, id_n = 0, id_nn = 0;
+    float ks = 0.f, vs = 0.f, ks_n = 0.f, vs_n = 0.f;
+    auto run_scales = [&](int base, int ids, float &a, float &b) {
+        const int64_t at = clamp_id(ids) * Hkv + kvh;
+        a = k_scales[at];
+        b = v_scales[at];
+        if (base + lane >= blk_end) a = b = 0.0f;
+    };
+    auto load_tile = [&](Tile &tl, int t) {
+        const int j = (kTileBlocks * t) & (kRun - 1);
+#pragma unroll
+        for (int b = 0; b < kTileBlocks; ++b) {
+            tl.ks[b] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, ks), j + b));
+            tl.vs[b] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, vs), j + b));
+        }
+        int64_t at[kTileBlocks];
+#pragma unroll
+        for (int b = 0; b < kTileBlocks; ++b) at[b] = clamp_id(__builtin_amdgcn_readlane(id, j + b)) * block_bytes;
+#pragma unroll
+        for (int b = 0; b < kTileBlocks; ++b)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const u32x4 *p = reinterpret_cast<const u32x4 *>(k_cache + at[b] + lane_off + (size_t)(8 * i) * row_stride);
+                tl.k[b][i] = stream ? __builtin_nontemporal_load(p) : *p;
+            }
+#pragma unroll
+        for (int b = 0; b < kTileBlocks; ++b)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const u32x4 *p = reinterpret_cast<const u32x4 *>(v_cache + at[b] + lane_off + (size_t)(8 * i) * row_stride);
+                tl.v[b][i] = stream ? __builtin_nontemporal_load(p) : *p;
+            }
+        if (j == kRun - kTileBlocks) {  // the run's last tile: on to the next
+            const int base = blk_begin + kTileBlocks * (t + 1);
+            id = id_n;
+            ks = ks_n;
+            vs = vs_n;
+            id_n = id_nn;
+            run_scales(base + kRun, id_n, ks_n, vs_n);
+            id_nn = run_ids(base + 2 * kRun);
+        }
+    };
+
+    float m_run[NQT], l_run[NQT];
+    f32x4 acc[NQT][8];
+#pragma unroll
+    for (int qt = 0; qt < NQT; ++qt) {
+        m_run[qt] = -INFINITY;
+        l_run[qt] = 0.0f;
+#pragma unroll
+        for (int dt = 0; dt < 8; ++dt) acc[qt][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    const int first_masked = ctx - (T - 1);  // first key that some query row cannot see
+
+    // A operand of P.V: 8 keys (4g .. 4g+3 of both blocks) of dim 16 dt + c
+    auto v_fragment = [&](int dt) -> bf16x8 {
+        typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
+        const i32x2 w =
+            __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i32x2 *)(lds_v + tr_base + 16u * ((unsigned)dt ^ tr_sw)));
+        return widen8<F>((unsigned)w[0], (unsigned)w[1]);
+    };
+    // A NaN among the values of keys that some rows must not see: 0 * NaN would reach those rows.  Which
+    // (dim, row) pairs do see one is a product of zeros and ones; they become NaN here, and the code 0.
+    auto mark_nan = [&](Tile &tl, int t) {
+        const int blk0 = blk_begin + kTileBlocks * t, key0 = blk0 * kBS;
+#pragma unroll
+        for (int b = 0; b < kTileBlocks; ++b)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                u32x4 one;
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    const unsigned n = nan_bytes(tl.v[b][i][w]);
+                    one[w] = n & 0x38383838u;  // 1.0
+                    tl.v[b][i][w] &= ~n;
+                }
+                *reinterpret_cast<u32x4 *>(lds_v + wr + 2048 * b + 1024 * i) = one;
+            }
+        u32x4 see[NQT];
+#pragma unroll
+        for (int qt = 0; qt < NQT; ++qt)
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) {
+                const int key = key0 + (e >> 2) * kBS + 4 * g + (e & 3), last = ctx - T + t_of_row[qt];
+                see[qt][e >> 1] = (key <= last ? 0x3f80u : 0u) | (key + 1 <= last ? 0x3f800000u : 0u);
+            }
+#pragma unroll
+        for (int dt = 0; dt < 8; ++dt) {
+            const bf16x8 one = v_fragment(dt);
+#pragma unroll
+            for (int qt = 0; qt < NQT; ++qt) {
+                const f32x4 hit = __builtin_amdgcn_mfma_f32_16x16x32_bf16(one, __builtin_bit_cast(bf16x8, see[qt]),
+                                                                          f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[qt][dt][e] = hit[e] > 0.0f ? __builtin_nanf("") : acc[qt][dt][e];
+            }
+        }
+    };
+
+    auto compute_tile = [&](Tile &tl, int t) {
+        const int blk0 = blk_begin + kTileBlocks * t, key0 = blk0 * kBS;
+        const bool tail = key0 + kTileKeys > first_masked || blk0 + kTileBlocks > blk_end;
+        bool has_nan = false;
+        if (tail) {  // V rows past the context hold anything: zeros, so that 0 * them is 0
+#pragma unroll
+            for (int b = 0; b < kTileBlocks; ++b)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    if (key0 + b * kBS + 8 * i + lr >= ctx || blk0 + b >= blk_end) tl.v[b][i] = u32x4{0u, 0u, 0u, 0u};
+                    if constexpr (F == Kv8Format::E4M3) {
+                        unsigned any = 0;
+#pragma unroll
+                        for (int w = 0; w < 4; ++w) any |= nan_bytes(tl.v[b][i][w]);
+                        has_nan |= any != 0;
+                    }
+                }
+            has_nan = __any(has_nan);
+        }
+        if constexpr (F == Kv8Format::E4M3)
+            if (has_nan) mark_nan(tl, t);
+#pragma unroll
+        for (int b = 0; b < kTileBlocks; ++b)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) *reinterpret_cast<u32x4 *>(lds_k + wr + 2048 * b + 1024 * i) = tl.k[b][i];
+        // S^T = K Q^T, one 16 x 16 tile per block
+        f32x4 s[NQT][kTileBlocks];
+#pragma unroll
+        for (int b = 0; b < kTileBlocks; ++b) {
+            const u32x4 k0 = *reinterpret_cast<const u32x4 *>(lds_k + krd0 + 2048 * b);
+            const u32x4 k1 = *reinterpret_cast<const u32x4 *>(lds_k + krd1 + 2048 * b);
+            const bf16x8 a0 = widen8<F>(k0[0], k0[1]), a1 = widen8<F>(k0[2], k0[3]);
+            const bf16x8 a2 = widen8<F>(k1[0], k1[1]), a3 = widen8<F>(k1[2], k1[3]);
+#pragma unroll
+            for (int qt = 0; qt < NQT; ++qt) {
+                f32x4 x = {0.f, 0.f, 0.f, 0.f};
+                x = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a0, qf[qt][0], x, 0, 0, 0);
+                x = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a1, qf[qt][1], x, 0, 0, 0);
+                x = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a2, qf[qt][2], x, 0, 0, 0);
+                x = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a3, qf[qt][3], x, 0, 0, 0);
+                s[qt][b] = x;
+            }
+        }
+#pragma unroll
+        for (int b = 0; b < kTileBlocks; ++b)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) *reinterpret_cast<u32x4 *>(lds_v + wr + 2048 * b + 1024 * i) = tl.v[b][i];
+        // online softmax in the exp2 domain; a query row's state lives in the lanes c = row
+        bf16x8 pf[NQT];
+#pragma unroll
+        for (int qt = 0; qt < NQT; ++qt) {
+            float sv[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                sv[j] = s[qt][j >> 2][j & 3] * (tl.ks[j >> 2] * scale_log2e);
+                if (tail) {
+                    const bool see = key0 + (j >> 2) * kBS + 4 * g + (j & 3) <= ctx - T + t_of_row[qt] &&
+                                     blk0 + (j >> 2) < blk_end;
+                    sv[j] = see ? sv[j] : -INFINITY;
+                }
+            }
+            float mx = sv[0];
+#pragma unroll
+            for (int j = 1; j < 8; ++j) mx = fmaxf(mx, sv[j]);
+            mx = fmaxf(mx, __shfl_xor(mx, 16));
+            mx = fmaxf(mx, __shfl_xor(mx, 32));
+            const float m_new = fmaxf(m_run[qt], mx);
+            const float m_safe = m_new == -INFINITY ? 0.0f : m_new;
+            const float alpha = fast_exp2(m_run[qt] - m_safe);
+            float sum = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                sv[j] = fast_exp2(sv[j] - m_safe);
+                sum += sv[j];
+                sv[j] *= tl.vs[j >> 2];
+            }
+            l_run[qt] = l_run[qt] * alpha + sum;
+            m_run[qt] = m_new;
+#pragma unroll
+            for (int dt = 0; dt < 8; ++dt) acc[qt][dt] *= alpha;
+            // the matrix unit takes p in bf16: each weight off by 2^-8 at most, as the output's own rounding
+            pf[qt] = __builtin_bit_cast(bf16x8, u32x4{pack_bf16x2(sv[0], sv[1]), pack_bf16x2(sv[2], sv[3]),
+                                                      pack_bf16x2(sv[4], sv[5]), pack_bf16x2(sv[6], sv[7])});
+        }
+        // O^T += V^T P^T
+#pragma unroll
+        for (int dt = 0; dt < 8; ++dt) {
+            const bf16x8 a = v_fragment(dt);
+#pragma unroll
+            for (int qt = 0; qt < NQT; ++qt)
+                acc[qt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, pf[qt], acc[qt][dt], 0, 0, 0);
+        }
+        settle();
+    };
+
+    if (ntiles > 0) {
+        id = run_ids(blk_begin);
+        id_n = run_ids(blk_begin + kRun);
+        run_scales(blk_begin, id, ks, vs);
+        run_scales(blk_begin + kRun, id_n, ks_n, vs_n);
+        id_nn = run_ids(blk_begin + 2 * kRun);
+        Tile tl[NBUF];
+#pragma unroll
+        for (int u = 0; u < NBUF - 1; ++u)
+            if (u < ntiles) load_tile(tl[u], u);
+        for (int t = 0; t < ntiles; t += NBUF)
+#pragma unroll
+            for (int u = 0; u < NBUF; ++u)
+                if (t + u < ntiles) {
+                    if (t + u + NBUF - 1 < ntiles) load_tile(tl[(u + NBUF - 1) % NBUF], t + u + NBUF - 1);
+                    compute_tile(tl[u], t + u);
+                }
+    }
+
+#pragma unroll
+    for (int qt = 0; qt < NQT; ++qt) {
+        float l = l_run[qt];
+        l += __shfl_xor(l, 16);
+        l += __shfl_xor(l, 32);
+        const int r = qt * 16 + c;
+        if (r >= R) continue;
+        const int64_t orow = ((int64_t)seq * T + t_of_row[qt]) * Hq + kvh * G + (r - t_of_row[qt] * G);
+        if (num_splits == 1) {
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // no key seen: zeros
+            __bf16 *op = out + orow * kD + 4 * g;
+#pragma unroll
+            for (int dt = 0; dt < 8; ++dt)
+                *reinterpret_cast<u32x2 *>(op + 16 * dt) =
+                    u32x2{pack_bf16x2(acc[qt][dt][0] * inv, acc[qt][dt][1] * inv),
+                          pack_bf16x2(acc[qt][dt][2] * inv, acc[qt][dt][3] * inv)};
+        } else {
+            const int64_t prow = orow * num_splits + split;
+            float *op = ws_o + prow * kD + 4 * g;
+#pragma unroll
+            for (int dt = 0; dt < 8; ++dt) *reinterpret_cast<f32x4 *>(op + 16 * dt) = acc[qt][dt];
+            if (g == 0) {
+                ws_ml[2 * prow] = m_run[qt];
+                ws_ml[2 * prow + 1] = l;
+            }
+        }
+    }
+}
+
+bool decode_path(DType dt, const PagedAttnArgs &a) {
+    return dt == DType::BF16 && a.head_dim == kD && a.block_size == kBS &&
+           (int64_t)a.num_new_tokens * (a.num_heads / a.num_kv_heads) <= kMaxDecodeRows;
+}
+
+template <Kv8Format F, int NQT, int HPB>
+void launch_decode_as(const PagedAttnArgs &a, const float *ks, const float *vs, int splits, int bps, float *ws_o,
+                      float *ws_ml, bool stream_loads, hipStream_t stream) {
+    paged_attn_kv8_decode_kernel<F, NQT, HPB, NQT == 1 ? 3 : 4>
+        <<<dim3(splits, a.num_seqs, (a.num_kv_heads + HPB - 1) / HPB), dim3(64 * HPB), 0, stream>>>(
+            static_cast<const __bf16 *>(a.q), static_cast<const unsigned char *>(a.k_cache),
+            static_cast<const unsigned char *>(a.v_cache), ks, vs, a.block_tables, a.context_lens,
+            static_cast<__bf16 *>(a.out), ws_o, ws_ml, a.num_new_tokens, a.num_heads, a.num_kv_heads,
+            a.max_blocks_per_seq, a.num_cache_blocks, a.scale * 1.4426950408889634f, splits, bps, stream_loads);
+}
+
+template <Kv8Format F>
+hipError_t launch_decode(const PagedAttnArgs &a, const float *ks, const float *vs, hipStream_t stream) {
+    const int splits = paged_attn_num_splits(a.num_seqs, a.num_kv_heads, a.max_blocks_per_seq);
+    const size_t rows = (size_t)a.num_seqs * a.num_new_tokens * a.num_heads;
+    if (splits > 1 && (!a.workspace || a.workspace_bytes < rows * splits * (kD + 2) * sizeof(float)))
+        return hipErrorInvalidValue;
+    int bps = (a.max_blocks_per_seq + splits - 1) / splits;
+    bps = (bps + kTileBlocks - 1) / kTileBlocks * kTileBlocks;
+    float *ws_o = static_cast<float *>(a.workspace);
+    float *ws_ml = ws_o ? ws_o + rows * splits * kD : nullptr;
+    // loads that do not stay in the caches, unless what the tables reach fits the 256 MiB Infinity Cache
+    const int64_t reach = (int64_t)a.num_seqs * a.max_blocks_per_seq * 2 * kBS * a.num_kv_heads * kD;
+    const bool nt = reach > ((int64_t)256 << 20);
+    // kv heads per workgroup: up to 8 waves share a block's rows; small launches spread over the CUs
+    int hpb = a.num_kv_heads >= 8 ? 8 : (a.num_kv_heads >= 4 ? 4 : (a.num_kv_heads >= 2 ? 2 : 1));
+    while (hpb > 1 && (int64_t)splits * a.num_seqs * ((a.num_kv_heads + hpb - 1) / hpb) < device_cus()) hpb /= 2;
+    const int nqt = (a.num_new_tokens * (a.num_heads / a.num_kv_heads) + 15) / 16;
+    if (nqt > 1 && hpb > 4) hpb = 4;  // the 512-register budget of a 4-wave workgroup
+#define NVLLM_KV8_CASE(NQT, HPB) \
+    case NQT * 16 + HPB: launch_decode_as<F, NQT, HPB>(a, ks, vs, splits, bps, ws_o, ws_ml, nt, stream); break;
+    switch (nqt * 16 + hpb) {
+        NVLLM_KV8_CASE(1, 8) NVLLM_KV8_CASE(1, 4) NVLLM_KV8_CASE(1, 2) NVLLM_KV8_CASE(1, 1)
+        NVLLM_KV8_CASE(2, 4) NVLLM_KV8_CASE(2, 2) NVLLM_KV8_CASE(2, 1)
+        NVLLM_KV8_CASE(3, 4) NVLLM_KV8_CASE(3, 2) NVLLM_KV8_CASE(3, 1)
+        default: return hipErrorInvalidValue;
+    }
+#undef NVLLM_KV8_CASE
+    const hipError_t err = hipGetLastError();
+    if (err != hipSuccess || splits == 1) return err;
+    return launch_paged_attn_merge(ws_o, ws_ml, a.out, (int64_t)rows, splits, stream);
+}
+
 }  // namespace
 
-PagedKv8Path paged_attn_kv8_path(DType, const PagedAttnArgs &) { return PagedKv8Path::Generic; }
+PagedKv8Path paged_attn_kv8_path(DType dt, const PagedAttnArgs &a) {
+    return decode_path(dt, a) ? PagedKv8Path::Decode : PagedKv8Path::Generic;
+}
 
-size_t paged_attn_kv8_workspace_bytes(DType, const PagedAttnArgs &) { return 0; }
+size_t paged_attn_kv8_workspace_bytes(DType dt, const PagedAttnArgs &a) {
+    if (!decode_path(dt, a)) return 0;
+    const int splits = paged_attn_num_splits(a.num_seqs, a.num_kv_heads, a.max_blocks_per_seq);
+    if (splits <= 1) return 0;
+    return (size_t)a.num_seqs * a.num_new_tokens * a.num_heads * splits * (kD + 2) * sizeof(float);
+}
 
 hipError_t launch_paged_attn_kv8(DType dt, Kv8Format fmt, const PagedAttnArgs &a, const float *k_scales,
                                  const float *v_scales, hipStream_t stream) {
     if (a.num_seqs <= 0) return hipSuccess;
+    if (decode_path(dt, a))
+        return fmt == Kv8Format::Int8 ? launch_decode<Kv8Format::Int8>(a, k_scales, v_scales, stream)
+                                      : launch_decode<Kv8Format::E4M3>(a, k_scales, v_scales, stream);
     if (dt == DType::BF16)
         return fmt == Kv8Format::Int8 ? launch_generic<__bf16, Kv8Format::Int8>(a, k_scales, v_scales, stream)
                                       : launch_generic<__bf16, Kv8Format::E4M3>(a, k_scales, v_scales, stream);

@@ -158,6 +158,29 @@ def test_scales_far_apart_and_zero(dev, fmt, T):
     compare(call(on, 128 ** -0.5), host, 128 ** -0.5, "bf16")
 
 
+@pytest.mark.parametrize("D,bs", [(128, 16), (64, 8)])
+@pytest.mark.parametrize("T", [2, 6, 20, 70])
+def test_a_nan_reaches_only_the_queries_that_see_it(dev, T, D, bs):
+    """an E4M3 NaN in a new token's key or value: rows before that token are as without it, rows from it
+    on are NaN (all dims for a key, the one dim for a value)"""
+    rng = np.random.default_rng(T)
+    n, H, Hq = 100 + T, 2, 8
+    on, host = make(rng, "e4m3", "bf16", [n, 40 + T], T, Hq, H, D, bs, dev)
+    clean = call(on, 0.1).view(2, T, H, Hq // H, D)
+    assert bool(torch.isfinite(clean).all())
+    t = T // 2
+    pos = n - T + t
+    at = (int(host[5][0][pos // bs]), pos % bs)
+    for name, dims in (("k", slice(None)), ("v", slice(5, 6))):
+        bad = dict(on, **{name: on[name].clone()})
+        bad[name].view(torch.uint8)[at[0], at[1], 1, 5] = 0xff
+        got = call(bad, 0.1).view(2, T, H, Hq // H, D)
+        hit = torch.zeros_like(clean, dtype=torch.bool)
+        hit[0, t:, 1, :, dims] = True
+        assert torch.equal(got.isnan(), hit), name
+        assert torch.equal(got[~hit], clean[~hit]), name
+
+
 @pytest.mark.parametrize("fmt", FMT)
 @pytest.mark.parametrize("T", [1, 40])
 def test_tables_out_of_the_pool_and_lengths_past_the_row(dev, fmt, T):

@@ -104,11 +104,19 @@ def test_attend():
 def test_path_and_sizes():
     assert nv.paged_attention_kv8_path(4, 1, 4, 2, 8, 4, 3) == "generic"
     assert nv.paged_attention_kv8_path(4, 1, 16, 8, 128, 16, 3, dtype=torch.float32) == "generic"
+    for T, Hq in ((1, 8), (1, 32), (4, 32), (12, 32), (48, 8)):
+        assert nv.paged_attention_kv8_path(4, T, Hq, 8, 128, 16, 3) == "decode"
     with pytest.raises(nv.ConfigError):
         nv.paged_attention_kv8_path(4, 1, 17, 8, 128, 16, 3)
     L = C.lib()
     assert L.nvllm_paged_attn_kv8_workspace_bytes(4, 1, 4, 2, 8, 4, 3, 0) == 0
     assert L.nvllm_paged_attn_kv8_workspace_bytes(4, 1, 5, 2, 8, 4, 3, 0) == 0
+    need = L.nvllm_paged_attn_kv8_workspace_bytes(2, 1, 16, 8, 128, 16, 64, 0)
+    assert need > 0 and attend(mb=64, wsb=need - 1) == C.NVLLM_ERR_CONFIG and "needs %d" % need in C.last_error()
+    assert attend(mb=64, ws=None) == C.NVLLM_ERR_CONFIG
+    assert attend(mb=64, ws=ctypes.c_void_p(0x10008)) == C.NVLLM_ERR_CONFIG
+    for name in ("q", "kc", "vc", "out"):
+        assert attend(**{name: ctypes.c_void_p(0x10008)}) == C.NVLLM_ERR_CONFIG, name
     assert L.nvllm_kv_cache_kv8_layer_bytes(10, 16, 8, 128) == 10 * 8 * (16 * 128 + 4)
     assert L.nvllm_kv_cache_kv8_layer_bytes(10, -1, 8, 128) == -1
     for dt in (torch.int8, torch.float8_e4m3fn):
