@@ -314,7 +314,9 @@ int nvllm_paged_attn_kv8(const void *q, const void *k_cache, const void *v_cache
 size_t nvllm_paged_attn_kv8_workspace_bytes(int num_seqs, int num_new_tokens, int num_heads,
                                             int num_kv_heads, int head_dim, int block_size,
                                             int max_blocks_per_seq, int dtype);
-/* Which kernel a launch shape runs (a pure query, as nvllm_paged_attn_path): 2 = generic. */
+/* Which kernel a launch shape runs (a pure query, as nvllm_paged_attn_path).  bf16, head_dim 128,
+ * block_size 16: 0 = decode kernel, up to 48 query rows (num_new_tokens * num_heads / num_kv_heads);
+ * 1 = tile kernel, more of them.  Other shapes and f32: 2 = generic kernel. */
 int nvllm_paged_attn_kv8_path(int num_seqs, int num_new_tokens, int num_heads, int num_kv_heads,
                               int head_dim, int block_size, int max_blocks_per_seq, int dtype);
 

@@ -168,7 +168,7 @@ constexpr size_t kNoAllocScratchBytes = (size_t)32 << 20;
 hipError_t launch_paged_attn_noalloc(DType dt, const PagedAttnArgs &a, hipStream_t stream);
 hipError_t noalloc_prepare_device();  // looks the scratch address of the current device up once
 // attention over the 8-bit cache (paged_attn_kv8.hip); `a.k_cache` / `a.v_cache` hold codes
-enum class PagedKv8Path : int { Decode = 0, Generic = 2 };
+enum class PagedKv8Path : int { Decode = 0, Tile = 1, Generic = 2 };
 PagedKv8Path paged_attn_kv8_path(DType dt, const PagedAttnArgs &a);
 size_t paged_attn_kv8_workspace_bytes(DType dt, const PagedAttnArgs &a);
 hipError_t launch_paged_attn_kv8(DType dt, Kv8Format fmt, const PagedAttnArgs &a, const float *k_scales,

@@ -532,9 +532,479 @@ __global__ __launch_bounds__(64 * HPB, NQT == 1 ? 2 : 1) void paged_attn_kv8_dec
     }
 }
 
-bool decode_path(DType dt, const PagedAttnArgs &a) {
-    return dt == DType::BF16 && a.head_dim == kD && a.block_size == kBS &&
-           (int64_t)a.num_new_tokens * (a.num_heads / a.num_kv_heads) <= kMaxDecodeRows;
+// ---------------------------------------------------------------------------
+// Tile path: bf16, head_dim 128, block_size 16, any number of query rows (verify, chunked prefill).
+//
+// A workgroup of four waves owns a tile of the kv head's R = T * G packed query rows (row rho: new token
+// rho / G, head rho % G of the group) and walks the keys in tiles of 64, two workgroups per CU:
+//   KG = 1: 128 rows, 32 a wave, every wave all 64 keys;
+//   KG = 2: 64 rows; waves 0, 1 take the first 32 keys of each tile and waves 2, 3 the others, so that the
+//           four SIMDs share the work of few rows; the two halves join through LDS at the end.
+// Codes come in as in the decode kernel, but are widened to bf16 ONCE for all rows on their way into LDS
+// (two buffers of K and V, one barrier a tile); two tiles are on their way in registers and LDS while one is
+// multiplied.  S^T = K Q^T and O^T = V^T P^T with mfma_f32_32x32x16_bf16: a query row lives in the lanes
+// c and c + 32, P needs no lane movement.  LDS: row r, 16-byte chunk ch of K at position ch ^ (r & 15), of V
+// at ch ^ 2 (r & 7) (transposed reads of 4 rows x 16 dims).
+// ---------------------------------------------------------------------------
+typedef __attribute__((ext_vector_type(16))) float f32x16;
+typedef __attribute__((ext_vector_type(4))) short s16x4;
+
+constexpr int kWideRow = 2 * kD;              // bytes of a widened row
+constexpr int kBigKeys = 64;                  // keys of a tile
+constexpr int kBigBlocks = kBigKeys / kBS;
+constexpr int kWideImage = kBigKeys * kWideRow;  // 16 KiB
+constexpr float kSlack = 8.0f;  // exponents may pass the reference by this before everything is rescaled
+
+// lane l's value and lane l ^ 32's.  In asm: given the builtin the same value twice, hipcc takes its two
+// results for equal.  s_nop 1 = the wait states between a vector write and the swap; the swap itself needs
+// none before its results are read.
+__device__ __forceinline__ void swap_halves(float &a, float &b) {
+    asm volatile("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(a), "+v"(b));
+}
+__device__ __forceinline__ float half_max(float x) {
+    float a = x, b = x;
+    swap_halves(a, b);
+    return fmaxf(a, b);
+}
+__device__ __forceinline__ float half_sum(float x) {
+    float a = x, b = x;
+    swap_halves(a, b);
+    return a + b;
+}
+
+template <Kv8Format F, int KG>
+__global__ __launch_bounds__(256, 2) void paged_attn_kv8_tile_kernel(
+    const __bf16 *__restrict__ q, const unsigned char *__restrict__ k_cache, const unsigned char *__restrict__ v_cache,
+    const float *__restrict__ k_scales, const float *__restrict__ v_scales, const int32_t *__restrict__ block_tables,
+    const int32_t *__restrict__ context_lens, __bf16 *__restrict__ out, float *__restrict__ ws_o,
+    float *__restrict__ ws_ml, int T, int Hq, int Hkv, int max_blocks_per_seq, int64_t num_cache_blocks, float scale,
+    int num_splits, int blocks_per_split) {
+    constexpr int kRows = 128 / KG, NS = 2 / KG;  // rows of the workgroup; 32-key score tiles of a wave
+    __shared__ __attribute__((aligned(16))) unsigned char lds[4 * kWideImage];  // [buffer][K, V]
+    __shared__ int nan_seen;
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int h = lane >> 5, c = lane & 31;
+    const int rg = KG == 1 ? wave : (wave & 1), kg = KG == 1 ? 0 : (wave >> 1);
+    const int seq = blockIdx.x / Hkv, kvh = blockIdx.x % Hkv;
+    const int row0 = (gridDim.y - 1 - blockIdx.y) * kRows;  // the tiles with the longest walks first
+    const int split = blockIdx.z;
+    const int G = Hq / Hkv, R = T * G;
+    int ctx = context_lens[seq];
+    const int64_t cap = (int64_t)max_blocks_per_seq * kBS;
+    if (ctx > cap) ctx = (int)cap;  // never read past the table row
+    const int row_last = row0 + kRows < R ? row0 + kRows - 1 : R - 1;
+    // keys that some row of the tile sees: [0, keys); all its rows see [0, keys_all)
+    const int64_t seen = (int64_t)ctx - T + row_last / G + 1;
+    const int keys = seen > 0 ? (int)seen : 0;
+    const int keys_all = ctx - T + row0 / G + 1;
+    const int blk_begin = split * blocks_per_split;
+    int blk_end = blk_begin + blocks_per_split;
+    if (blk_end > (keys + kBS - 1) / kBS) blk_end = (keys + kBS - 1) / kBS;
+    const int ntiles = blk_end > blk_begin ? (blk_end - blk_begin + kBigBlocks - 1) / kBigBlocks : 0;
+    const int32_t *table = block_tables + (int64_t)seq * max_blocks_per_seq;
+
+    // this lane's query row, as B operand: k-step s holds Q[row][16 s + 8 h .. + 7]
+    const int row = row0 + 32 * rg + c;
+    const bool live = row < R;
+    const int t_row = live ? row / G : 0;
+    const int64_t orow = ((int64_t)seq * T + t_row) * Hq + kvh * G + (live ? row - t_row * G : 0);
+    const int last = ctx - T + t_row;  // last key it sees
+    const bool works = row0 + 32 * rg < R;  // wave-uniform: waves without rows only stage
+    bf16x8 qf[8];
+    const unsigned flip = scale < 0.0f ? 0x80008000u : 0u;  // a negative scale moves into Q: factors stay >= 0
+#pragma unroll
+    for (int s = 0; s < 8; ++s) {
+        u32x4 x = {0u, 0u, 0u, 0u};
+        if (live) x = *reinterpret_cast<const u32x4 *>(q + orow * kD + 16 * s + 8 * h);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] ^= flip;
+        qf[s] = __builtin_bit_cast(bf16x8, x);
+    }
+    const float scale_log2e = fabsf(scale) * 1.4426950408889634f;
+
+    // staging: thread covers 16 dims (lch) of rows tid / 8 and 32 + tid / 8 of the tile
+    const int64_t block_bytes = (int64_t)kBS * Hkv * kD;
+    const int sr = threadIdx.x >> 3, lch = threadIdx.x & 7;
+    const unsigned lane_off = (unsigned)(sr & 15) * (unsigned)(Hkv * kD) + (unsigned)kvh * kD + 16u * lch;
+    const int sb = wave >> 1;  // block of the first row within its 32 keys
+    unsigned kw[2], vw[2];     // LDS positions of the two 16-byte chunks of the first row; the second: + 32 rows
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+        kw[e] = (unsigned)(sr * kWideRow + 16 * ((2 * lch + e) ^ (sr & 15)));
+        vw[e] = (unsigned)(kWideImage + sr * kWideRow + 16 * ((2 * lch + e) ^ (2 * (sr & 7))));
+    }
+    // ids and scales of 64 blocks (16 tiles) at once, one a lane, as in the decode kernel
+    auto run_ids = [&](int base) -> int {
+        int j = base + lane;
+        if (j >= blk_end) j = blk_end - 1;
+        return table[j];
+    };
+    auto clamp_id = [&](int id) -> int64_t {
+        int64_t x = id;
+        if (x < 0) x = 0;
+        if (x >= num_cache_blocks) x = num_cache_blocks - 1;
+        return x;
+    };
+    auto run_scales = [&](int base, int ids, float &a, float &b) {
+        const int64_t at = clamp_id(ids) * Hkv + kvh;
+        a = k_scales[at];
+        b = v_scales[at];
+        if (base + lane >= blk_end) a = b = 0.0f;
+    };
+    int id = 0, id_n = 0, id_nn = 0;
+    float ks = 0.f, vs = 0.f, ks_n = 0.f, vs_n = 0.f;
+    u32x4 ck[2], cv[2];                          // codes on their way
+    float fk[kBigBlocks], fv[kBigBlocks];        // scales of the tile that is loaded next / last
+    auto load_tile = [&](int t) {
+        const int j = (kBigBlocks * t) & (kRun - 1);
+#pragma unroll
+        for (int b = 0; b < kBigBlocks; ++b) {
+            fk[b] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, ks), j + b)) * scale_log2e;
+            fv[b] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, vs), j + b));
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int64_t at = clamp_id(__builtin_amdgcn_readlane(id, j + 2 * i + sb)) * block_bytes;
+            ck[i] = *reinterpret_cast<const u32x4 *>(k_cache + at + lane_off);
+            cv[i] = *reinterpret_cast<const u32x4 *>(v_cache + at + lane_off);
+        }
+        if (j == kRun - kBigBlocks) {
+            const int base = blk_begin + kBigBlocks * (t + 1);
+            id = id_n;
+            ks = ks_n;
+            vs = vs_n;
+            id_n = id_nn;
+            run_scales(base + kRun, id_n, ks_n, vs_n);
+            id_nn = run_ids(base + 2 * kRun);
+        }
+    };
+    // codes of tile t -> bf16 in LDS.  V rows that no row of the tile sees are zeros; -> whether a NaN is
+    // among the values that only some rows see (those become 0, see mark_nan)
+    auto stage_tile = [&](int t, unsigned char *buf) -> bool {
+        const int key0 = (blk_begin + kBigBlocks * t) * kBS;
+        bool has_nan = false;
+        if (key0 + kBigKeys > keys_all) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int key = key0 + 32 * i + sr;
+                if (key >= keys || key >= blk_end * kBS) cv[i] = u32x4{0u, 0u, 0u, 0u};
+                if constexpr (F == Kv8Format::E4M3)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) has_nan |= nan_bytes(cv[i][e]) != 0;
+            }
+            if constexpr (F == Kv8Format::E4M3)
+                if (has_nan)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) cv[i][e] &= ~nan_bytes(cv[i][e]);
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                *reinterpret_cast<bf16x8 *>(buf + kw[e] + 32 * kWideRow * i) = widen8<F>(ck[i][2 * e], ck[i][2 * e + 1]);
+                *reinterpret_cast<bf16x8 *>(buf + vw[e] + 32 * kWideRow * i) = widen8<F>(cv[i][2 * e], cv[i][2 * e + 1]);
+            }
+        return has_nan;
+    };
+
+    float m_ref = -INFINITY, l_run = 0.0f;
+    f32x16 acc[4];  // O^T: dims 32 dt + 8 (i / 4) + 4 h + i % 4 of this lane's row
+#pragma unroll
+    for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[dt][i] = 0.0f;
+
+    const unsigned krd = (unsigned)((32 * kg + c) * kWideRow);
+    // transposed V read: lane reads 8 bytes of row 4 h + ((lane & 15) >> 2) (+ 8), dims 16 (lane >> 4 & 1) + 4 (lane & 3)
+    const int vr = 4 * h + ((lane & 15) >> 2);
+    const unsigned vch = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+    const unsigned vrd = (unsigned)(kWideImage + (32 * kg + vr) * kWideRow + 8 * (lane & 1));
+    auto v_fragment = [&](const unsigned char *buf, int key16, int dt) -> bf16x8 {
+        typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+        const unsigned at = vrd + (unsigned)(16 * key16 * kWideRow) + 16 * ((4 * dt + vch) ^ (2 * (unsigned)(vr & 7)));
+        const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(buf + at));
+        const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(buf + at + 8 * kWideRow));
+        return __builtin_bit_cast(bf16x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+    };
+
+    auto compute_tile = [&](int t, const unsigned char *buf, const float (&fk_t)[kBigBlocks],
+                            const float (&fv_t)[kBigBlocks]) {
+        const int key0 = (blk_begin + kBigBlocks * t) * kBS + 32 * kg;
+        f32x16 s[NS];
+#pragma unroll
+        for (int n = 0; n < NS; ++n) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[n][i] = 0.0f;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const bf16x8 a = *reinterpret_cast<const bf16x8 *>(buf + krd + 32 * kWideRow * n +
+                                                                  16 * ((2 * k + h) ^ (c & 15)));
+                s[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, qf[k], s[n], 0, 0, 0);
+            }
+        }
+        // element i of score tile n is key 32 n + 8 (i / 4) + 4 h + i % 4: block 2 n + i / 8
+        float f[2 * NS];
+#pragma unroll
+        for (int b = 0; b < 2 * NS; ++b) f[b] = fk_t[2 * kg + b];
+        if (key0 + 32 * NS > keys_all || key0 + 32 * NS > blk_end * kBS) {
+#pragma unroll
+            for (int n = 0; n < NS; ++n)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int key = key0 + 32 * n + 8 * (i / 4) + 4 * h + i % 4;
+                    s[n][i] = key <= last && key < blk_end * kBS ? s[n][i] * f[2 * n + i / 8] : -INFINITY;
+                }
+#pragma unroll
+            for (int b = 0; b < 2 * NS; ++b) f[b] = 1.0f;
+        }
+        float mx = -INFINITY;
+#pragma unroll
+        for (int b = 0; b < 2 * NS; ++b) {
+            float x = s[b / 2][8 * (b % 2)];
+#pragma unroll
+            for (int i = 1; i < 8; ++i) x = fmaxf(x, s[b / 2][8 * (b % 2) + i]);
+            mx = fmaxf(mx, x * f[b]);
+        }
+        mx = half_max(mx);
+        // exponents are taken from a reference that moves only when a row's maximum has passed it by kSlack
+        // (p stays below 2^8, the sums in f32): most tiles then rescale nothing
+        if (__any(mx > m_ref + kSlack || (m_ref == -INFINITY && mx != -INFINITY))) {
+            const float m_new = fmaxf(m_ref, mx);
+            const float alpha = m_new == -INFINITY ? 1.0f : fast_exp2(m_ref - m_new);
+            m_ref = m_new;
+            l_run *= alpha;
+#pragma unroll
+            for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[dt][i] *= alpha;
+        }
+        const float m_safe = m_ref == -INFINITY ? 0.0f : m_ref;
+        float sum = 0.0f;
+        bf16x8 pf[2 * NS];  // P^T as B operand, 16 keys each
+#pragma unroll
+        for (int b = 0; b < 2 * NS; ++b) {
+            float p[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                p[i] = fast_exp2(fmaf(s[b / 2][8 * (b % 2) + i], f[b], -m_safe));
+                sum += p[i];
+                p[i] *= fv_t[2 * kg + b];
+            }
+            pf[b] = __builtin_bit_cast(bf16x8, u32x4{pack_bf16x2(p[0], p[1]), pack_bf16x2(p[2], p[3]),
+                                                     pack_bf16x2(p[4], p[5]), pack_bf16x2(p[6], p[7])});
+        }
+        l_run += sum;
+#pragma unroll
+        for (int b = 0; b < 2 * NS; ++b)
+#pragma unroll
+            for (int dt = 0; dt < 4; ++dt)
+                acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v_fragment(buf, b, dt), pf[b], acc[dt], 0, 0, 0);
+        settle();
+    };
+    // NaN values that only some rows of the tile see (0 * NaN would reach the others): which (dim, row) pairs
+    // see one is a product of zeros and ones.  The whole workgroup; `buf`'s V is overwritten.
+    auto mark_nan = [&](int t, unsigned char *buf) {
+        const int key0 = (blk_begin + kBigBlocks * t) * kBS;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int key = key0 + 32 * i + sr;
+            u32x4 one = {0u, 0u, 0u, 0u};
+            if (key < keys && key < blk_end * kBS) {
+                const int64_t at = clamp_id(table[key / kBS]) * block_bytes;
+                one = *reinterpret_cast<const u32x4 *>(v_cache + at + lane_off);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) one[e] = nan_bytes(one[e]) & 0x38383838u;  // 1.0
+            }
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+                *reinterpret_cast<bf16x8 *>(buf + vw[e] + 32 * kWideRow * i) = widen8<F>(one[2 * e], one[2 * e + 1]);
+        }
+        __syncthreads();
+        if (works) {
+#pragma unroll 1
+            for (int b = 0; b < 2 * NS; ++b) {
+                u32x4 see;
+#pragma unroll
+                for (int e = 0; e < 8; e += 2) {
+                    const int key = key0 + 32 * kg + 16 * b + 8 * (e / 4) + 4 * h + e % 4;
+                    see[e / 2] = (key <= last ? 0x3f80u : 0u) | (key + 1 <= last ? 0x3f800000u : 0u);
+                }
+#pragma unroll
+                for (int dt = 0; dt < 4; ++dt) {
+                    f32x16 z;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) z[i] = 0.0f;
+                    z = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v_fragment(buf, b, dt), __builtin_bit_cast(bf16x8, see),
+                                                                z, 0, 0, 0);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) acc[dt][i] = z[i] > 0.0f ? __builtin_nanf("") : acc[dt][i];
+                }
+            }
+            settle();
+        }
+        __syncthreads();
+    };
+
+    if (ntiles > 0) {
+        id = run_ids(blk_begin);
+        id_n = run_ids(blk_begin + kRun);
+        run_scales(blk_begin, id, ks, vs);
+        run_scales(blk_begin + kRun, id_n, ks_n, vs_n);
+        id_nn = run_ids(blk_begin + 2 * kRun);
+        float fk_t[kBigBlocks], fv_t[kBigBlocks], fk_n[kBigBlocks], fv_n[kBigBlocks];
+        auto keep = [&](float (&a)[kBigBlocks], float (&b)[kBigBlocks]) {
+#pragma unroll
+            for (int i = 0; i < kBigBlocks; ++i) {
+                a[i] = fk[i];
+                b[i] = fv[i];
+            }
+        };
+        load_tile(0);
+        keep(fk_t, fv_t);
+        bool nan_t = stage_tile(0, lds), nan_n = false;
+        if (ntiles > 1) load_tile(1);
+        keep(fk_n, fv_n);
+        if (F == Kv8Format::E4M3 && threadIdx.x == 0) nan_seen = 0;
+        for (int t = 0; t < ntiles; ++t) {
+            unsigned char *buf = lds + (t & 1) * 2 * kWideImage, *next = lds + ((t + 1) & 1) * 2 * kWideImage;
+            __syncthreads();
+            if (t + 1 < ntiles) nan_n = stage_tile(t + 1, next);
+            if (t + 2 < ntiles) load_tile(t + 2);
+            if (works) compute_tile(t, buf, fk_t, fv_t);
+            if constexpr (F == Kv8Format::E4M3)
+                if ((blk_begin + kBigBlocks * (t + 1)) * kBS > keys_all) {  // the same for all waves
+                    if (nan_t) nan_seen = 1;
+                    __syncthreads();
+                    const bool any = nan_seen != 0;
+                    __syncthreads();
+                    if (any) mark_nan(t, buf);
+                    if (threadIdx.x == 0) nan_seen = 0;
+                    __syncthreads();
+                }
+            nan_t = nan_n;
+#pragma unroll
+            for (int i = 0; i < kBigBlocks; ++i) {
+                fk_t[i] = fk_n[i];
+                fv_t[i] = fv_n[i];
+            }
+            keep(fk_n, fv_n);
+        }
+    }
+
+    float l = half_sum(l_run);
+    if constexpr (KG == 2) {  // the second key half's waves hand theirs over: O [64 values a lane], m, l
+        __syncthreads();
+        float *slot = reinterpret_cast<float *>(lds) + (wave & 1) * (66 * 64) + lane;
+        if (kg == 1) {
+#pragma unroll
+            for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) slot[64 * (16 * dt + i)] = acc[dt][i];
+            slot[64 * 64] = m_ref;
+            slot[64 * 65] = l;
+        }
+        __syncthreads();
+        if (kg == 1) return;
+        const float m2 = slot[64 * 64], l2 = slot[64 * 65];
+        const float m = fmaxf(m_ref, m2);
+        const float a1 = m_ref == -INFINITY ? 0.0f : fast_exp2(m_ref - m), a2 = m2 == -INFINITY ? 0.0f : fast_exp2(m2 - m);
+#pragma unroll
+        for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[dt][i] = acc[dt][i] * a1 + slot[64 * (16 * dt + i)] * a2;
+        l = l * a1 + l2 * a2;
+        m_ref = m;
+    }
+    if (!live) return;
+    if (num_splits == 1) {
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // no key seen: zeros
+        __bf16 *op = out + orow * kD + 4 * h;
+#pragma unroll
+        for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4)
+                *reinterpret_cast<u32x2 *>(op + 32 * dt + 2 * i) =
+                    u32x2{pack_bf16x2(acc[dt][i] * inv, acc[dt][i + 1] * inv),
+                          pack_bf16x2(acc[dt][i + 2] * inv, acc[dt][i + 3] * inv)};
+    } else {
+        const int64_t prow = orow * num_splits + split;
+        float *op = ws_o + prow * kD + 4 * h;
+#pragma unroll
+        for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4)
+                *reinterpret_cast<f32x4 *>(op + 32 * dt + 2 * i) = f32x4{acc[dt][i], acc[dt][i + 1], acc[dt][i + 2], acc[dt][i + 3]};
+        if (h == 0) {
+            ws_ml[2 * prow] = m_ref;
+            ws_ml[2 * prow + 1] = l;
+        }
+    }
+}
+
+bool fast_shape(DType dt, const PagedAttnArgs &a) {
+    return dt == DType::BF16 && a.head_dim == kD && a.block_size == kBS;
+}
+
+int64_t query_rows(const PagedAttnArgs &a) { return (int64_t)a.num_new_tokens * (a.num_heads / a.num_kv_heads); }
+
+bool decode_path(DType dt, const PagedAttnArgs &a) { return fast_shape(dt, a) && query_rows(a) <= kMaxDecodeRows; }
+
+// workgroups of 64 rows while that is all there is, else of 128
+int tile_rows(const PagedAttnArgs &a) { return query_rows(a) <= 64 ? 64 : 128; }
+
+// Parts of the key walk: enough for two workgroups on every CU, each part 256 keys at least
+int tile_splits(const PagedAttnArgs &a) {
+    const int64_t rows = tile_rows(a);
+    const int64_t units = (int64_t)a.num_seqs * a.num_kv_heads * ((query_rows(a) + rows - 1) / rows);
+    int64_t splits = 2 * device_cus() / units;
+    const int64_t most = a.max_blocks_per_seq / 16;
+    if (splits > most) splits = most;
+    if (splits > 64) splits = 64;  // the merge kernel holds one split's (m, l) per lane
+    return splits < 1 ? 1 : (int)splits;
+}
+
+int splits_of(DType dt, const PagedAttnArgs &a) {
+    if (!fast_shape(dt, a)) return 1;
+    return decode_path(dt, a) ? paged_attn_num_splits(a.num_seqs, a.num_kv_heads, a.max_blocks_per_seq) : tile_splits(a);
+}
+
+// partials of a launch that is split: O and (m, l); false if the workspace is too small for them
+bool partials(const PagedAttnArgs &a, int splits, float **ws_o, float **ws_ml) {
+    const size_t rows = (size_t)a.num_seqs * a.num_new_tokens * a.num_heads;
+    *ws_o = *ws_ml = nullptr;
+    if (splits == 1) return true;
+    if (!a.workspace || a.workspace_bytes < rows * splits * (kD + 2) * sizeof(float)) return false;
+    *ws_o = static_cast<float *>(a.workspace);
+    *ws_ml = *ws_o + rows * splits * kD;
+    return true;
+}
+
+int blocks_per_split(const PagedAttnArgs &a, int splits, int granule) {
+    const int bps = (a.max_blocks_per_seq + splits - 1) / splits;
+    return (bps + granule - 1) / granule * granule;
+}
+
+template <Kv8Format F, int KG>
+hipError_t launch_tile(const PagedAttnArgs &a, const float *ks, const float *vs, hipStream_t stream) {
+    const int splits = tile_splits(a), rows = 128 / KG;
+    float *ws_o, *ws_ml;
+    if (!partials(a, splits, &ws_o, &ws_ml)) return hipErrorInvalidValue;
+    const int64_t tiles = (query_rows(a) + rows - 1) / rows;
+    if (tiles > 65535) return hipErrorInvalidValue;
+    paged_attn_kv8_tile_kernel<F, KG>
+        <<<dim3((unsigned)(a.num_seqs * a.num_kv_heads), (unsigned)tiles, splits), dim3(256), 0, stream>>>(
+            static_cast<const __bf16 *>(a.q), static_cast<const unsigned char *>(a.k_cache),
+            static_cast<const unsigned char *>(a.v_cache), ks, vs, a.block_tables, a.context_lens,
+            static_cast<__bf16 *>(a.out), ws_o, ws_ml, a.num_new_tokens, a.num_heads, a.num_kv_heads,
+            a.max_blocks_per_seq, a.num_cache_blocks, a.scale, splits, blocks_per_split(a, splits, kBigBlocks));
+    const hipError_t err = hipGetLastError();
+    if (err != hipSuccess || splits == 1) return err;
+    return launch_paged_attn_merge(ws_o, ws_ml, a.out, (int64_t)a.num_seqs * a.num_new_tokens * a.num_heads, splits,
+                                   stream);
 }
 
 template <Kv8Format F, int NQT, int HPB>
@@ -551,20 +1021,16 @@ void launch_decode_as(const PagedAttnArgs &a, const float *ks, const float *vs, 
 template <Kv8Format F>
 hipError_t launch_decode(const PagedAttnArgs &a, const float *ks, const float *vs, hipStream_t stream) {
     const int splits = paged_attn_num_splits(a.num_seqs, a.num_kv_heads, a.max_blocks_per_seq);
-    const size_t rows = (size_t)a.num_seqs * a.num_new_tokens * a.num_heads;
-    if (splits > 1 && (!a.workspace || a.workspace_bytes < rows * splits * (kD + 2) * sizeof(float)))
-        return hipErrorInvalidValue;
-    int bps = (a.max_blocks_per_seq + splits - 1) / splits;
-    bps = (bps + kTileBlocks - 1) / kTileBlocks * kTileBlocks;
-    float *ws_o = static_cast<float *>(a.workspace);
-    float *ws_ml = ws_o ? ws_o + rows * splits * kD : nullptr;
+    float *ws_o, *ws_ml;
+    if (!partials(a, splits, &ws_o, &ws_ml)) return hipErrorInvalidValue;
+    const int bps = blocks_per_split(a, splits, kTileBlocks);
     // loads that do not stay in the caches, unless what the tables reach fits the 256 MiB Infinity Cache
     const int64_t reach = (int64_t)a.num_seqs * a.max_blocks_per_seq * 2 * kBS * a.num_kv_heads * kD;
     const bool nt = reach > ((int64_t)256 << 20);
     // kv heads per workgroup: up to 8 waves share a block's rows; small launches spread over the CUs
     int hpb = a.num_kv_heads >= 8 ? 8 : (a.num_kv_heads >= 4 ? 4 : (a.num_kv_heads >= 2 ? 2 : 1));
     while (hpb > 1 && (int64_t)splits * a.num_seqs * ((a.num_kv_heads + hpb - 1) / hpb) < device_cus()) hpb /= 2;
-    const int nqt = (a.num_new_tokens * (a.num_heads / a.num_kv_heads) + 15) / 16;
+    const int nqt = (int)((query_rows(a) + 15) / 16);
     if (nqt > 1 && hpb > 4) hpb = 4;  // the 512-register budget of a 4-wave workgroup
 #define NVLLM_KV8_CASE(NQT, HPB) \
     case NQT * 16 + HPB: launch_decode_as<F, NQT, HPB>(a, ks, vs, splits, bps, ws_o, ws_ml, nt, stream); break;
@@ -577,18 +1043,19 @@ hipError_t launch_decode(const PagedAttnArgs &a, const float *ks, const float *v
 #undef NVLLM_KV8_CASE
     const hipError_t err = hipGetLastError();
     if (err != hipSuccess || splits == 1) return err;
-    return launch_paged_attn_merge(ws_o, ws_ml, a.out, (int64_t)rows, splits, stream);
+    return launch_paged_attn_merge(ws_o, ws_ml, a.out, (int64_t)a.num_seqs * a.num_new_tokens * a.num_heads, splits,
+                                   stream);
 }
 
 }  // namespace
 
 PagedKv8Path paged_attn_kv8_path(DType dt, const PagedAttnArgs &a) {
-    return decode_path(dt, a) ? PagedKv8Path::Decode : PagedKv8Path::Generic;
+    if (!fast_shape(dt, a)) return PagedKv8Path::Generic;
+    return decode_path(dt, a) ? PagedKv8Path::Decode : PagedKv8Path::Tile;
 }
 
 size_t paged_attn_kv8_workspace_bytes(DType dt, const PagedAttnArgs &a) {
-    if (!decode_path(dt, a)) return 0;
-    const int splits = paged_attn_num_splits(a.num_seqs, a.num_kv_heads, a.max_blocks_per_seq);
+    const int splits = splits_of(dt, a);
     if (splits <= 1) return 0;
     return (size_t)a.num_seqs * a.num_new_tokens * a.num_heads * splits * (kD + 2) * sizeof(float);
 }
@@ -596,9 +1063,17 @@ size_t paged_attn_kv8_workspace_bytes(DType dt, const PagedAttnArgs &a) {
 hipError_t launch_paged_attn_kv8(DType dt, Kv8Format fmt, const PagedAttnArgs &a, const float *k_scales,
                                  const float *v_scales, hipStream_t stream) {
     if (a.num_seqs <= 0) return hipSuccess;
+    const bool int8 = fmt == Kv8Format::Int8;
     if (decode_path(dt, a))
-        return fmt == Kv8Format::Int8 ? launch_decode<Kv8Format::Int8>(a, k_scales, v_scales, stream)
-                                      : launch_decode<Kv8Format::E4M3>(a, k_scales, v_scales, stream);
+        return int8 ? launch_decode<Kv8Format::Int8>(a, k_scales, v_scales, stream)
+                    : launch_decode<Kv8Format::E4M3>(a, k_scales, v_scales, stream);
+    if (fast_shape(dt, a)) {
+        if (tile_rows(a) == 64)
+            return int8 ? launch_tile<Kv8Format::Int8, 2>(a, k_scales, v_scales, stream)
+                        : launch_tile<Kv8Format::E4M3, 2>(a, k_scales, v_scales, stream);
+        return int8 ? launch_tile<Kv8Format::Int8, 1>(a, k_scales, v_scales, stream)
+                    : launch_tile<Kv8Format::E4M3, 1>(a, k_scales, v_scales, stream);
+    }
     if (dt == DType::BF16)
         return fmt == Kv8Format::Int8 ? launch_generic<__bf16, Kv8Format::Int8>(a, k_scales, v_scales, stream)
                                       : launch_generic<__bf16, Kv8Format::E4M3>(a, k_scales, v_scales, stream);

@@ -150,7 +150,7 @@ def gather_cache_blocks_kv8(key_cache, value_cache, key_scales, value_scales, bl
     return keys, values
 
 
-PAGED_KV8_PATHS = {0: "decode", 2: "generic"}
+PAGED_KV8_PATHS = ("decode", "tile", "generic")
 
 
 def paged_attention_kv8_path(num_seqs, num_new_tokens, num_heads, num_kv_heads, head_dim, block_size,

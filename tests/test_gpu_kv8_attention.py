@@ -98,14 +98,14 @@ def test_small_shapes(dev, fmt, dtype, Hq, H, D, bs, T):
 
 @pytest.mark.parametrize("fmt", FMT)
 @pytest.mark.parametrize("Hq,H", [(16, 8), (32, 8), (8, 8), (24, 8), (16, 1), (6, 3), (28, 4), (5, 5)])
-@pytest.mark.parametrize("T", [1, 2, 4, 7, 16, 33])
+@pytest.mark.parametrize("T", [1, 2, 4, 7, 16, 33, 70])
 def test_head_layouts_and_query_counts(dev, fmt, Hq, H, T):
     rng = np.random.default_rng(Hq * 100 + H + T)
     check(rng, fmt, "bf16", [T, T + 15, 16 * 5, 129 + T], T, Hq, H, 128, 16, dev)
 
 
 @pytest.mark.parametrize("fmt", FMT)
-@pytest.mark.parametrize("T", [1, 4, 16, 40])
+@pytest.mark.parametrize("T", [1, 4, 12, 13, 16, 17, 32, 33, 100])
 def test_lengths_around_the_tiles(dev, fmt, T):
     rng = np.random.default_rng(T)
     lens = [n for n in (1, 2, 15, 16, 17, 31, 32, 33, 47, 48, 63, 64, 65, 127, 128, 129, 255, 257, 1023, 1025) if n >= T]
@@ -130,7 +130,7 @@ def test_rows_that_see_no_key_are_zero(dev, fmt, dtype, D, bs, T):
 
 
 @pytest.mark.parametrize("fmt", FMT)
-@pytest.mark.parametrize("T", [1, 4, 40])
+@pytest.mark.parametrize("T", [1, 4, 30, 40, 200])
 def test_long_contexts(dev, fmt, T):
     """one sequence over 8192 keys and a short neighbour"""
     rng = np.random.default_rng(T)

@@ -106,6 +106,9 @@ def test_path_and_sizes():
     assert nv.paged_attention_kv8_path(4, 1, 16, 8, 128, 16, 3, dtype=torch.float32) == "generic"
     for T, Hq in ((1, 8), (1, 32), (4, 32), (12, 32), (48, 8)):
         assert nv.paged_attention_kv8_path(4, T, Hq, 8, 128, 16, 3) == "decode"
+    for T, Hq in ((13, 32), (49, 8), (4, 128), (1024, 16)):
+        assert nv.paged_attention_kv8_path(4, T, Hq, 8, 128, 16, 3) == "tile"
+        assert nv.paged_attention_kv8_path(4, T, Hq, 8, 128, 8, 3) == "generic"
     with pytest.raises(nv.ConfigError):
         nv.paged_attention_kv8_path(4, 1, 17, 8, 128, 16, 3)
     L = C.lib()
