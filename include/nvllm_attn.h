@@ -276,9 +276,9 @@ int nvllm_reshape_and_cache_kv8(const void *key, const void *value, void *k_cach
                                 int64_t num_cache_blocks, int format, int dtype,
                                 nvllm_stream_t stream);
 
-/* nvllm_qk_norm_rope_cache_* with quantisation: the rotated K and V go into the 8-bit cache, rounded
- * once, from f32 (from f64 where the tensors are f32), not by way of k_out.  q_out may be q; k_out
- * (optional) must not overlap k. */
+/* nvllm_qk_norm_rope_cache_* with quantisation: the rotated K and V go into the 8-bit cache, K computed in
+ * f64 and rounded once (not by way of k_out); q_out and k_out in f32.  q_out may be q; k_out (optional)
+ * must not overlap k. */
 int nvllm_qk_norm_rope_cache_kv8(const void *q, const void *k, const void *v, void *q_out,
                                  void *k_out, const void *q_weight, const void *k_weight, float eps,
                                  const void *cos_cache, const void *sin_cache,

@@ -41,6 +41,7 @@ int check_cache(const char *who, std::int64_t num_cache_blocks, int block_size, 
     if (format != 0 && format != 1) return fail(ErrorKind::Unsupported, who, "format must be 0 (int8) or 1 (E4M3)");
     if (dtype != 0 && dtype != 1) return fail(ErrorKind::Unsupported, who, "dtype must be 0 (bf16) or 1 (f32)");
     if (head_dim > 256) return fail(ErrorKind::Unsupported, who, "head_dim > 256");
+    if (num_cache_blocks > 0x7fffffff) return fail(ErrorKind::Unsupported, who, "more than 2^31 - 1 blocks");
     if (block_size > kernels::kKv8MaxBlockSize) return fail(ErrorKind::Unsupported, who, "block_size > 256");
     return NVLLM_OK;
 }

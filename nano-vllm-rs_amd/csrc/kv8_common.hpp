@@ -107,19 +107,21 @@ template <Kv8Format F> __device__ __forceinline__ unsigned char encode1(float y)
     return (unsigned char)encode4<F>(y, 0.0f, 0.0f, 0.0f);
 }
 
-// The same from 64 bits.  y is rounded to the format's grid before it becomes an f32 (which then holds
-// it exactly): a rounding to f32 first would put 1 value in 2^17 on the wrong side of a border.
-template <Kv8Format F> __device__ __forceinline__ unsigned char encode1(double y) {
-    if constexpr (F == Kv8Format::Int8) {
-        y = rint(y);
-    } else {
-        int e;
-        (void)frexp(y, &e);
-        e = e < -5 ? -5 : e;  // below 2^-6 the steps are as wide as there
-        if (fabs(y) <= 448.0) y = ldexp(rint(ldexp(y, 4 - e)), e - 4);
+// y to 24 bits, to odd: truncated, and the last bit set where that lost something.  A later rounding to a
+// code then falls as if from y itself (rounding to nearest here would put 1 value in 2^17 on the wrong
+// side of a code's border).
+__device__ __forceinline__ float narrow_odd(double y) {
+    const float f = (float)y;
+    const double d = (double)f;
+    unsigned u = __builtin_bit_cast(unsigned, f);
+    if (d != y && y == y) {
+        if (fabs(d) > fabs(y)) u -= 1;  // (an infinity, from a y past f32's range, becomes the largest number)
+        u |= 1;
     }
-    return encode1<F>((float)y);
+    return __builtin_bit_cast(float, u);
 }
+__device__ __forceinline__ float narrow_odd(float y) { return y; }
+template <Kv8Format F> __device__ __forceinline__ unsigned char encode1(double y) { return encode1<F>(narrow_odd(y)); }
 
 // the codes of a kept row under a larger scale (ratio = old / new, a power of two <= 1/2).  A code
 // that is no number of the format (int8's -128, which no write makes) is brought back into range.

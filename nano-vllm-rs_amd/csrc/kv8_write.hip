@@ -11,13 +11,13 @@
 // row 0 is written exactly when a block comes fresh from the allocator: no call has to reset scales.
 //
 // The scale couples all tokens that a call puts into one block, and a slot mapping may name them in
-// any order.  So each block gets ONE owner: the token that writes its lowest row in this call.  The
-// owner's wave finds the block's other tokens, takes the maximum, and writes codes and scale; no
-// atomics on the cache, and of tokens that name the same slot the last one wins, as in a sequential
+// any order.  So each block gets ONE owner: the workgroup that looks after the first of its tokens.  It
+// finds the block's other tokens, takes the maximum, and writes codes and scale; no atomics on the cache, and of tokens that name the same slot the last one wins, as in a sequential
 // loop (the reference's, src/attention/paged.rs:231-262).
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "kv8_common.hpp"
 
@@ -54,57 +54,66 @@ __global__ __launch_bounds__(kThreads) void kv8_index_kernel(const int64_t *__re
     }
 }
 
-// The blocks that the chunk's tokens own.  LDS: map[c * bs + o] = the token of this call that writes
-// row o of token c's block (-1: none), owner[0 .. count) = the chunk's owning tokens.
+// The blocks that this chunk of tokens owns: those whose first token (of the tokens whose row is not
+// overwritten by a later one) is in the chunk.  LDS: map[u * bs + o] = the token of the call that writes row
+// o of the chunk's u-th block (-1: none).  Returns how many blocks the chunk owns, owner[i] = u of the i-th.
 struct Chunk {
-    int *map;
-    int *owner;
-    int64_t *block;  // block id of each token of the chunk, -1 where its slot is not valid
+    int *map;      // [kMaxChunk * bs]
+    int *owner;    // [kMaxChunk]
+    int *block;    // [kMaxChunk]: the different blocks of the chunk's slots
 };
 
 __device__ __forceinline__ int find_blocks(const Chunk &ch, const int64_t *__restrict__ slots, int n, int t0,
                                            int chunk, int bs, int64_t num_slots,
                                            const int32_t *__restrict__ index) {
-    __shared__ int count;
+    __shared__ int uniques, count;
     const int tid = threadIdx.x;
-    if (tid < chunk) {
-        int64_t b = -1;
-        if (t0 + tid < n) {
+    if (tid < 64) {
+        int b = -1;
+        if (tid < chunk && t0 + tid < n) {
             const int64_t s = slots[t0 + tid];
-            if (s >= 0 && s < num_slots) b = s / bs;
+            if (s >= 0 && s < num_slots) b = (int)(s / bs);
         }
-        ch.block[tid] = b;
+        bool first = b >= 0;
+        for (int j = 0; j < chunk - 1; ++j) {
+            const int bj = __shfl(b, j);  // by all lanes: an inactive one has nothing to read
+            if (j < tid && bj == b) first = false;
+        }
+        const unsigned long long m = __ballot(first);
+        if (first) ch.block[__popcll(m & ((1ull << tid) - 1))] = b;
+        if (tid == 0) {
+            uniques = __popcll(m);
+            count = 0;
+        }
     }
-    if (tid == 0) count = 0;
+    __syncthreads();
+    const int nu = uniques;
     if (index) {
-        __syncthreads();
-        for (int i = tid; i < chunk * bs; i += kThreads) {
-            const int c = i / bs;
-            const int64_t b = ch.block[c];
-            int e = -1;
-            if (b >= 0) {
-                const int64_t s = b * bs + (i - c * bs);
-                e = index[s];
-                if (e < 0 || e >= n || slots[e] != s) e = -1;
-            }
+        for (int i = tid; i < nu * bs; i += kThreads) {
+            const int64_t s = (int64_t)ch.block[i / bs] * bs + i % bs;
+            int e = index[s];
+            if (e < 0 || e >= n || slots[e] != s) e = -1;
             ch.map[i] = e;
         }
     } else {
-        for (int i = tid; i < chunk * bs; i += kThreads) ch.map[i] = -1;
+        for (int i = tid; i < nu * bs; i += kThreads) ch.map[i] = -1;
         __syncthreads();
         for (int t = tid; t < n; t += kThreads) {
             const int64_t s = slots[t];
             if (s < 0 || s >= num_slots) continue;
-            const int64_t b = s / bs;
-            for (int c = 0; c < chunk; ++c)
-                if (ch.block[c] == b) atomicMax(ch.map + c * bs + (int)(s - b * bs), t);
+            const int b = (int)(s / bs);
+            for (int u = 0; u < nu; ++u)
+                if (ch.block[u] == b) atomicMax(ch.map + u * bs + (int)(s - (int64_t)b * bs), t);
         }
     }
     __syncthreads();
-    if (tid < chunk && ch.block[tid] >= 0) {
-        int o = 0;
-        while (o < bs - 1 && ch.map[tid * bs + o] < 0) ++o;
-        if (ch.map[tid * bs + o] == t0 + tid) ch.owner[atomicAdd(&count, 1)] = tid;
+    if (tid < nu) {
+        int first = n;
+        for (int o = 0; o < bs; ++o) {
+            const int t = ch.map[tid * bs + o];
+            if (t >= 0 && t < first) first = t;
+        }
+        if (first >= t0 && first < t0 + chunk) ch.owner[atomicAdd(&count, 1)] = tid;
     }
     __syncthreads();
     return count;
@@ -145,8 +154,8 @@ __device__ __forceinline__ void write_unit(const int *map, int bs, int D, int Hk
 }
 
 // Norm and rotation of one row by one wave: x / sqrt(mean(x^2) + eps) * weight, then the rotation of
-// the pairs (d, d + D/2).  AT: f32 for bf16 tensors; f64 for f32 ones, where a value that f32 leaves on the other
-// side of a code's border would show as a whole step.
+// the pairs (d, d + D/2).  AT: f64 for what is quantised, as a value that f32 arithmetic moves across a code's
+// border would show as a whole step (and f64 runs at the rate of f32 here); f32 for what is not.
 template <typename ET, typename AT> struct RotatedRow {
     const ET *x, *w, *c, *s;
     int half;
@@ -182,7 +191,7 @@ template <typename ET> struct PlainRow {
 template <typename ET, Kv8Format F, bool PRODUCER>
 __global__ __launch_bounds__(kThreads) void kv8_write_generic_kernel(const Kv8WriteArgs a, int chunk, int row_blocks,
                                                                      bool indexed) {
-    typedef typename std::conditional<sizeof(ET) == 4, double, float>::type AT;
+    typedef typename std::conditional<sizeof(ET) == 4, double, float>::type QT;  // of q_out and k_out
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const int D = a.head_dim, Hkv = a.num_kv_heads, Hq = a.num_heads;
     const ET *key = static_cast<const ET *>(a.key), *value = static_cast<const ET *>(a.value);
@@ -196,7 +205,7 @@ __global__ __launch_bounds__(kThreads) void kv8_write_generic_kernel(const Kv8Wr
             const ET *x = h < Hq ? static_cast<const ET *>(a.q) + (t * Hq + h) * D : key + (t * Hkv + h - Hq) * D;
             ET *y = h < Hq ? static_cast<ET *>(a.q_out) + (t * Hq + h) * D
                            : static_cast<ET *>(a.k_out) + (t * Hkv + h - Hq) * D;
-            const auto row = rotated_row<ET, AT>(x, static_cast<const ET *>(h < Hq ? a.q_weight : a.k_weight),
+            const auto row = rotated_row<ET, QT>(x, static_cast<const ET *>(h < Hq ? a.q_weight : a.k_weight),
                                                  static_cast<const ET *>(a.cos_cache),
                                                  static_cast<const ET *>(a.sin_cache), a.positions[t], a.max_positions,
                                                  D, a.eps);
@@ -210,7 +219,7 @@ __global__ __launch_bounds__(kThreads) void kv8_write_generic_kernel(const Kv8Wr
     }
     extern __shared__ int dyn[];
     __shared__ int owner[kMaxChunk];
-    __shared__ int64_t block[kMaxChunk];
+    __shared__ int block[kMaxChunk];
     const Chunk ch{dyn, owner, block};
     const int bs = a.block_size, n = (int)a.num_tokens, t0 = ((int)blockIdx.x - row_blocks) * chunk;
     const int count = find_blocks(ch, a.slot_mapping, n, t0, chunk, bs, a.num_cache_blocks * bs,
@@ -224,7 +233,7 @@ __global__ __launch_bounds__(kThreads) void kv8_write_generic_kernel(const Kv8Wr
         float *scales = is_v ? a.v_scales : a.k_scales;
         if (PRODUCER && !is_v)
             write_unit<F>(map, bs, D, Hkv, block[c], head, cache, scales, [&](int t) {
-                return rotated_row<ET, AT>(key + ((int64_t)t * Hkv + head) * D, static_cast<const ET *>(a.k_weight),
+                return rotated_row<ET, double>(key + ((int64_t)t * Hkv + head) * D, static_cast<const ET *>(a.k_weight),
                                            static_cast<const ET *>(a.cos_cache), static_cast<const ET *>(a.sin_cache),
                                            a.positions[t], a.max_positions, D, a.eps);
             });
@@ -252,6 +261,213 @@ hipError_t launch_generic(const Kv8WriteArgs &a, bool indexed, hipStream_t strea
                                                                                                      indexed);
     }
     return hipGetLastError();
+}
+
+// ---------------------------------------------------------------------------
+// Fast path: bf16, head_dim 128, block_size 16.
+//
+// Bound by HBM on prompts (K and V read once, half as many bytes written) and by latency on a decode step.
+// A wave takes one (block, kv head) of K or V: 8 lanes a row, two rows a lane (o and o + 8), so the block is
+// read with four 16-byte loads a lane, its maximum found with six shuffles and written with two 16-byte
+// stores, all rows of the block at once.  `parts` workgroups share a chunk's units, so that a decode step's
+// few tokens still spread over the chip.
+// ---------------------------------------------------------------------------
+constexpr int kFastD = 128;
+constexpr int kFastBS = 16;
+
+// 16 values of a row.  Plain rows: dims 16 ch .. + 15.  Rotated rows: 8 ch .. + 7, then 64 + 8 ch .. + 7, so
+// that a lane holds both dims of its pairs.
+template <bool ROT> __device__ __forceinline__ int dim_of(int ch, int half) {
+    return ROT ? 64 * half + 8 * ch : 16 * ch + 8 * half;
+}
+
+__device__ __forceinline__ void unpack8(u32x4 w, float *x) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        x[2 * i] = bf16_lo(w[i]);
+        x[2 * i + 1] = bf16_hi(w[i]);
+    }
+}
+
+// norm and rotation of a row that 8 lanes hold (a[8] dims 8 ch .., b[8] dims 64 + 8 ch ..), in place
+template <typename AT>
+__device__ __forceinline__ void rotate_row(AT *a, AT *b, const __bf16 *w, const __bf16 *cos_row, const __bf16 *sin_row,
+                                           int ch, float eps) {
+    AT ss = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) ss += a[i] * a[i] + b[i] * b[i];
+#pragma unroll
+    for (int m = 1; m < 8; m <<= 1) ss += __shfl_xor(ss, m);
+    const AT inv = (AT)1 / (AT)sqrt((AT)(ss * (AT)(1.0 / kFastD) + (AT)eps));
+    float w1[8], w2[8], c1[8], c2[8], s1[8], s2[8];
+    const auto get = [&](const __bf16 *p, float *lo, float *hi) {
+        unpack8(*reinterpret_cast<const u32x4 *>(p + 8 * ch), lo);
+        unpack8(*reinterpret_cast<const u32x4 *>(p + 64 + 8 * ch), hi);
+    };
+    get(w, w1, w2);
+    get(cos_row, c1, c2);
+    get(sin_row, s1, s2);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const AT n1 = a[i] * inv * (AT)w1[i], n2 = b[i] * inv * (AT)w2[i];
+        a[i] = n1 * (AT)c1[i] - n2 * (AT)s1[i];
+        b[i] = n2 * (AT)c2[i] + n1 * (AT)s2[i];
+    }
+}
+
+template <Kv8Format F, bool ROT>
+__device__ __forceinline__ void write_fast_unit(const Kv8WriteArgs &a, const int *map, int block, int head, bool is_v) {
+    typedef typename std::conditional<ROT, double, float>::type AT;  // rotated values: see RotatedRow
+    const int lane = threadIdx.x & 63, r = lane >> 3, ch = lane & 7;
+    const int Hkv = a.num_kv_heads;
+    const __bf16 *src = static_cast<const __bf16 *>(is_v ? a.value : a.key);
+    float *sp = (is_v ? a.v_scales : a.k_scales) + (int64_t)block * Hkv + head;
+    const bool begins = map[0] >= 0;
+    const float was = begins ? 0.0f : *sp;
+    u32x4 w[2][2];
+    int t[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        t[i] = map[r + 8 * i];
+        w[i][0] = w[i][1] = u32x4{0u, 0u, 0u, 0u};
+        if (t[i] >= 0) {
+            const __bf16 *p = src + ((int64_t)t[i] * Hkv + head) * kFastD;
+            w[i][0] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(p + dim_of<ROT>(ch, 0)));
+            w[i][1] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(p + dim_of<ROT>(ch, 1)));
+        }
+    }
+    AT x[2][16];
+    float amax = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        float f[16];
+        unpack8(w[i][0], f);
+        unpack8(w[i][1], f + 8);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) x[i][j] = f[j];
+        if constexpr (ROT) {
+            int pos = t[i] >= 0 ? a.positions[t[i]] : 0;
+            pos = pos < 0 ? 0 : (pos >= a.max_positions ? a.max_positions - 1 : pos);  // stay inside the tables
+            rotate_row<AT>(x[i], x[i] + 8, static_cast<const __bf16 *>(a.k_weight),
+                           static_cast<const __bf16 *>(a.cos_cache) + (int64_t)pos * kFastD,
+                           static_cast<const __bf16 *>(a.sin_cache) + (int64_t)pos * kFastD, ch, a.eps);
+            if (t[i] < 0)  // a row of zeros with eps 0 is NaN here
+#pragma unroll
+                for (int j = 0; j < 16; ++j) x[i][j] = 0;
+        }
+#pragma unroll
+        for (int j = 0; j < 16; ++j) amax = fmaxf(amax, finite_abs((float)x[i][j]));
+    }
+    const float s = fmaxf(was, scale_of<F>(wave_max(amax)));
+    const float inv = inverse_scale(s);
+    const bool grows = !begins && s > was;
+    unsigned char *base = static_cast<unsigned char *>(is_v ? a.v_cache : a.k_cache) +
+                          ((int64_t)block * kFastBS * Hkv + head) * kFastD;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        u32x4 *out = reinterpret_cast<u32x4 *>(base + (int64_t)(r + 8 * i) * Hkv * kFastD + 16 * ch);
+        unsigned c[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            c[j] = encode4<F>(narrow_odd(x[i][4 * j] * (AT)inv), narrow_odd(x[i][4 * j + 1] * (AT)inv),
+                              narrow_odd(x[i][4 * j + 2] * (AT)inv), narrow_odd(x[i][4 * j + 3] * (AT)inv));
+        if constexpr (ROT) {
+            // even lanes have dims 8 ch and 64 + 8 ch; trade with the neighbour for 16 dims in a row:
+            // even lanes 8 ch .. + 15, odd lanes 64 + 8 (ch - 1) .. + 15
+            const bool odd = ch & 1;
+            const unsigned g0 = __shfl_xor((int)(odd ? c[0] : c[2]), 1), g1 = __shfl_xor((int)(odd ? c[1] : c[3]), 1);
+            const u32x4 y = odd ? u32x4{g0, g1, c[2], c[3]} : u32x4{c[0], c[1], g0, g1};
+            out = reinterpret_cast<u32x4 *>(base + (int64_t)(r + 8 * i) * Hkv * kFastD +
+                                            (odd ? 64 + 8 * (ch - 1) : 8 * ch));
+            if (t[i] >= 0) *out = y;
+        } else {
+            if (t[i] >= 0) *out = u32x4{c[0], c[1], c[2], c[3]};
+        }
+        if (grows && t[i] < 0) {
+            u32x4 y = *out;
+            const float ratio = was * inv;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) y[j] = rescale4<F>(y[j], ratio);
+            *out = y;
+        }
+    }
+    if (lane == 0 && (begins || grows)) *sp = s;
+}
+
+// Workgroups [0, chunk_blocks * parts): part `% parts` of chunk `/ parts`; behind them (producer) rows of Q, and of
+// K to k_out, 8 lanes a row, 32 rows a workgroup.
+template <Kv8Format F, bool PRODUCER>
+__global__ __launch_bounds__(kThreads) void kv8_write_kernel(const Kv8WriteArgs a, int chunk, int parts,
+                                                             int chunk_blocks, bool indexed) {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int Hkv = a.num_kv_heads;
+    if constexpr (PRODUCER) {
+        if (blockIdx.x >= (unsigned)(chunk_blocks * parts)) {
+            const int Hq = a.num_heads, heads = Hq + (a.k_out ? Hkv : 0);
+            const int64_t rows = a.num_tokens * heads;
+            const int64_t r = (int64_t)(blockIdx.x - chunk_blocks * parts) * 32 + (threadIdx.x >> 3);
+            if (r >= rows) return;  // whole groups of 8 lanes leave together
+            const int64_t t = rows <= 0xffffffffLL ? (int64_t)((unsigned)r / (unsigned)heads) : r / heads;
+            const int h = (int)(r - t * heads), ch = threadIdx.x & 7;
+            const bool is_q = h < Hq;
+            const int64_t at = is_q ? (t * Hq + h) * kFastD : (t * Hkv + h - Hq) * kFastD;
+            const __bf16 *p = static_cast<const __bf16 *>(is_q ? a.q : a.key) + at;
+            __bf16 *y = static_cast<__bf16 *>(is_q ? a.q_out : a.k_out) + at;
+            int pos = a.positions[t];
+            pos = pos < 0 ? 0 : (pos >= a.max_positions ? a.max_positions - 1 : pos);
+            float lo[8], hi[8];
+            unpack8(__builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(p + 8 * ch)), lo);
+            unpack8(__builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(p + 64 + 8 * ch)), hi);
+            rotate_row<float>(lo, hi, static_cast<const __bf16 *>(is_q ? a.q_weight : a.k_weight),
+                              static_cast<const __bf16 *>(a.cos_cache) + (int64_t)pos * kFastD,
+                              static_cast<const __bf16 *>(a.sin_cache) + (int64_t)pos * kFastD, ch, a.eps);
+            *reinterpret_cast<u32x4 *>(y + 8 * ch) = u32x4{pack_bf16x2(lo[0], lo[1]), pack_bf16x2(lo[2], lo[3]),
+                                                           pack_bf16x2(lo[4], lo[5]), pack_bf16x2(lo[6], lo[7])};
+            *reinterpret_cast<u32x4 *>(y + 64 + 8 * ch) = u32x4{pack_bf16x2(hi[0], hi[1]), pack_bf16x2(hi[2], hi[3]),
+                                                                pack_bf16x2(hi[4], hi[5]), pack_bf16x2(hi[6], hi[7])};
+            return;
+        }
+    }
+    __shared__ int map[kMaxChunk * kFastBS], owner[kMaxChunk], block[kMaxChunk];
+    const Chunk ch{map, owner, block};
+    const int part = blockIdx.x % parts, t0 = (int)(blockIdx.x / parts) * chunk;
+    const int count = find_blocks(ch, a.slot_mapping, (int)a.num_tokens, t0, chunk, kFastBS,
+                                  a.num_cache_blocks * kFastBS, indexed ? a.workspace : nullptr);
+    for (int u = part * kWaves + wave; u < count * Hkv * 2; u += parts * kWaves) {
+        const int i = u / (2 * Hkv), head = u % Hkv;
+        const bool is_v = (u / Hkv) & 1;
+        const int c = __builtin_amdgcn_readfirstlane(owner[i]);
+        const int b = __builtin_amdgcn_readfirstlane(block[c]);
+        if (PRODUCER && !is_v)
+            write_fast_unit<F, true>(a, map + c * kFastBS, b, head, false);
+        else
+            write_fast_unit<F, false>(a, map + c * kFastBS, b, head, is_v);
+    }
+}
+
+template <Kv8Format F> hipError_t launch_fast(const Kv8WriteArgs &a, bool indexed, hipStream_t stream) {
+    // tokens per workgroup: up to a block's worth, while that leaves work for every CU
+    int chunk = kMaxChunk;
+    while (chunk > 1 && a.num_tokens < (int64_t)chunk * 256) chunk /= 2;
+    const int64_t chunks = (a.num_tokens + chunk - 1) / chunk;
+    // workgroups per chunk: a unit a wave while the launch is small
+    int parts = (2 * a.num_kv_heads + kWaves - 1) / kWaves;
+    while (parts > 1 && chunks * parts > 2048) --parts;
+    const int64_t rows = a.q ? a.num_tokens * (a.num_heads + (a.k_out ? a.num_kv_heads : 0)) : 0;
+    const int64_t blocks = chunks * parts + (rows + 31) / 32;
+    if (blocks > 0x7fffffffLL) return hipErrorInvalidValue;
+    if (a.q)
+        kv8_write_kernel<F, true><<<dim3((unsigned)blocks), dim3(kThreads), 0, stream>>>(a, chunk, parts, (int)chunks, indexed);
+    else
+        kv8_write_kernel<F, false><<<dim3((unsigned)blocks), dim3(kThreads), 0, stream>>>(a, chunk, parts, (int)chunks, indexed);
+    return hipGetLastError();
+}
+
+bool fast_shape(DType dt, const Kv8WriteArgs &a) {
+    const auto at16 = [](const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; };
+    return dt == DType::BF16 && a.head_dim == kFastD && a.block_size == kFastBS && at16(a.key) && at16(a.value) &&
+           at16(a.k_cache) && at16(a.v_cache) && at16(a.q) && at16(a.q_out) && at16(a.k_out) && at16(a.q_weight) &&
+           at16(a.k_weight) && at16(a.cos_cache) && at16(a.sin_cache);
 }
 
 // Read-back of whole blocks: out[i] = codes of block ids[i] times its scales, in bf16 (exact) or f32.
@@ -329,6 +545,9 @@ hipError_t launch_kv8_write(DType dt, Kv8Format fmt, const Kv8WriteArgs &a, hipS
         const hipError_t err = hipGetLastError();
         if (err != hipSuccess) return err;
     }
+    if (fast_shape(dt, a))
+        return fmt == Kv8Format::Int8 ? launch_fast<Kv8Format::Int8>(a, indexed, stream)
+                                      : launch_fast<Kv8Format::E4M3>(a, indexed, stream);
     if (dt == DType::BF16)
         return fmt == Kv8Format::Int8 ? launch_generic<__bf16, Kv8Format::Int8>(a, indexed, stream)
                                       : launch_generic<__bf16, Kv8Format::E4M3>(a, indexed, stream);

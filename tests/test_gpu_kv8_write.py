@@ -1,8 +1,7 @@
 """The quantising write, the producer and the read-back of the 8-bit cache against the 64-bit oracle.
 
 A plain write is exact by construction (power-of-two scales): codes and scales are compared bit for
-bit.  The producer's K is computed in f32 (bf16 tensors) or f64 (f32 tensors) before its one rounding;
-its tolerance is derived at the test."""
+bit.  The producer's K is computed in f64 before its one rounding; its tolerance is derived at the test."""
 import numpy as np
 import pytest
 import torch
@@ -210,9 +209,9 @@ def _producer(rng, fmt, dtype, n, Hq, H, D, bs, dev, slots, nb, k_out=True):
 def test_producer(dev, fmt, dtype, n, Hq, H, D, bs):
     """q_out and k_out: f32 arithmetic of some ten operations (each off by 2^-24 of terms no larger than
     |a| + |b| of the pair), the sum of squares (relative D * 2^-24 at worst), one rounding.  Codes: V is
-    exact.  K's value may sit next to a code's border, so a code may differ by one step where the f64
-    value is within the f32 error of the border; its scale may differ only where amax is that near a
-    border of its own, which none of these inputs is."""
+    exact.  K is computed in f64, its value known to some (D / 2 + 12) 2^-53 of its pair: a code may differ
+    by one step where a border lies that near, its scale only where amax lies within 2^-24 of a border of
+    its own, which none of these inputs does."""
     rng = np.random.default_rng(n * 7 + D)
     nb = n // bs + 6
     slots = (rng.permutation(nb)[np.arange(n) // bs] * bs + np.arange(n) % bs).tolist()
@@ -237,7 +236,7 @@ def test_producer(dev, fmt, dtype, n, Hq, H, D, bs):
     assert np.array_equal(ks.double().cpu().numpy(), ksn)
     got = numbers_of(kc, fmt)
     at = np.argwhere(got != kn)
-    err = err if dtype == "bf16" else (D / 2 + 12) * 2.0 ** -53  # f64 inside for f32 tensors
+    err = (D / 2 + 12) * 2.0 ** -53
     token = {s: t for t, s in enumerate(slots)}
     for b, row, h, d in at:
         t = token[b * bs + row]
