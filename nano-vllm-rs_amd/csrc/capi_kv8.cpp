@@ -231,11 +231,11 @@ int nvllm_paged_attn_kv8(const void *q, const void *k_cache, const void *v_cache
                          int num_kv_heads, int head_dim, int block_size, int max_blocks_per_seq,
                          int64_t num_cache_blocks, float scale, int format, int dtype, nvllm_stream_t stream) {
     static const char *who = "paged_attn_kv8";
-    if (!q || !k_cache || !v_cache || !k_scales || !v_scales || !block_tables || !context_lens || !out)
-        return fail(ErrorKind::Null, who, "null pointer");
     if (const int rc = check_cache(who, num_cache_blocks, block_size, num_kv_heads, head_dim, format, dtype)) return rc;
     if (const int rc = check_attn(who, num_seqs, num_new_tokens, num_heads, num_kv_heads, max_blocks_per_seq)) return rc;
     if (num_seqs == 0) return NVLLM_OK;
+    if (!q || !k_cache || !v_cache || !k_scales || !v_scales || !block_tables || !context_lens || !out)
+        return fail(ErrorKind::Null, who, "null pointer");
     const unsigned elt = dtype == 0 ? 2 : 4;
     if (!aligned(q, elt) || !aligned(out, elt) || !aligned(k_scales, 4) || !aligned(v_scales, 4) ||
         !aligned(block_tables, 4) || !aligned(context_lens, 4))

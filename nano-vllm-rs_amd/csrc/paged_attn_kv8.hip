@@ -155,10 +155,12 @@ hipError_t launch_generic(const PagedAttnArgs &a, const float *ks, const float *
 // ---------------------------------------------------------------------------
 // Decode path: bf16, head_dim 128, block_size 16, up to 48 query rows (T * Hq/Hkv) per kv head.
 //
-// Bound by HBM: a cached token costs 2 * Hkv * 128 bytes, half of the bf16 cache's.  The work is cut as
-// in paged_attn.hip: grid (splits, sequences, kv-head groups), one wave per kv head of a workgroup, all
-// query rows of the head in one wave, no barriers; HPB waves walk the same table entries, so together
-// they read whole blocks.  What one byte a value changes:
+// Bound by HBM: a cached token costs 2 * Hkv * 128 bytes, half of the bf16 cache's.  A workgroup has one kv head
+// of one sequence, its W waves a part of the keys each (all query rows of the head), and they join through LDS at
+// the end: one launch, no workspace.  Only where (sequence, kv head) pairs are few are the keys split over
+// workgroups as well, with partials and a merge launch as in paged_attn.hip.  (Waves for the heads of a sequence
+// instead, which read whole blocks together, as the bf16 kernel has them: 256 x 2048 int8 184 against 166 us,
+// 64 x 4096 with 4 splits 91 against 95; short walks even out better.)  What one byte a value changes:
 //   tile    32 keys (2 blocks), 8 KiB.  NBUF tiles in registers, all but one of them on their way;
 //   K       8 lanes x 16 B read a 128-byte row, 8 rows an instruction; through the wave's LDS image (16-byte
 //           chunk ch of row r at position ch ^ (r & 7): 8 rows x 1 chunk and 1 row x 8 chunks both touch
@@ -183,6 +185,100 @@ constexpr int kRun = 64;                // blocks whose ids and scales a wave ho
 constexpr int kMaxDecodeRows = 48;
 
 __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// lane l's value and lane l ^ 32's.  In asm: given the builtin the same value twice, hipcc takes its two
+// results for equal.  s_nop 1 = the wait states between a vector write and the swap; the swap itself needs
+// none before its results are read.
+__device__ __forceinline__ void swap_halves(float &a, float &b) {
+    asm volatile("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(a), "+v"(b));
+}
+// the same for lanes l and l ^ 16
+__device__ __forceinline__ void swap_rows(float &a, float &b) {
+    asm volatile("s_nop 1\n\tv_permlane16_swap_b32 %0, %1" : "+v"(a), "+v"(b));
+}
+__device__ __forceinline__ float half_max(float x) {
+    float a = x, b = x;
+    swap_halves(a, b);
+    return fmaxf(a, b);
+}
+__device__ __forceinline__ float half_sum(float x) {
+    float a = x, b = x;
+    swap_halves(a, b);
+    return a + b;
+}
+
+// over the four lanes l ^ {0, 16, 32, 48}
+__device__ __forceinline__ float quad_max(float x) {
+    float a = x, b = x;
+    swap_rows(a, b);
+    return half_max(fmaxf(a, b));
+}
+
+// Exponents are taken from a reference that moves only when a row's maximum has passed it by kSlack: p stays
+// below 2^8 (its rounding to bf16 is relative, the sums are f32), and most tiles rescale nothing.
+constexpr float kSlack = 8.0f;
+
+// block id as the kernels use it: inside the pool
+__device__ __forceinline__ int pool_id(int id, int64_t num_cache_blocks) {
+    const int most = (int)num_cache_blocks - 1;  // the C entries refuse larger pools
+    return id < 0 ? 0 : (id > most ? most : id);
+}
+
+// A kv head's rows of a cache block as a buffer: 16 bytes of it at lane_offset + row_offset, zeros without a
+// memory access if `valid` is false.  Tiles past the end are "loaded" that way, so that every step of a loop
+// issues the same loads: behind a load that a branch may skip, hipcc's waits count only what is outstanding on
+// the branch that skipped it, and so wait for the newest tile as well.  (It also keeps addresses scalar.)
+typedef __amdgpu_buffer_rsrc_t Rows;
+__device__ __forceinline__ Rows block_rows(const unsigned char *base, int64_t offset, int bytes, bool valid) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char *>(base + offset), 0, valid ? bytes : 0, 0x00027000);
+}
+template <bool STREAM> __device__ __forceinline__ u32x4 load16(Rows rows, unsigned lane_offset, unsigned row_offset) {
+    return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rows, lane_offset, row_offset, STREAM ? 2 : 0));
+}
+
+// A wave's view of its part of a block table: lane l holds id and scales of block `base + l` of a run of 64, and
+// the next run's are on their way.  What is loaded is looked at (clamped, masked) only when its run begins, so
+// that nothing waits for it before.  Past the part's end: the last id (read, and masked), scale 0.
+struct Run {
+    const int32_t *table;
+    const float *k_scales, *v_scales;  // of the kv head: + Hkv * id
+    int Hkv, end, lane;
+    int64_t num_cache_blocks;
+    int id, id_n, id_nn;               // id_nn: as the table has it
+    float ks, vs, ks_n, vs_n;          // _n: as loaded
+
+    __device__ __forceinline__ int raw_id(int base) const {
+        const int j = base + lane;
+        return table[j < end ? j : end - 1];
+    }
+    __device__ __forceinline__ void ask_scales(int ids, float &a, float &b) const {
+        a = k_scales[(int64_t)ids * Hkv];
+        b = v_scales[(int64_t)ids * Hkv];
+    }
+    __device__ __forceinline__ void begin(int base) {
+        id = pool_id(raw_id(base), num_cache_blocks);
+        id_n = pool_id(raw_id(base + kRun), num_cache_blocks);
+        id_nn = raw_id(base + 2 * kRun);
+        ask_scales(id, ks, vs);
+        if (base + lane >= end) ks = vs = 0.0f;
+        ask_scales(id_n, ks_n, vs_n);
+    }
+    __device__ __forceinline__ void advance(int base) {  // base: the run that begins
+        id = id_n;
+        ks = base + lane < end ? ks_n : 0.0f;
+        vs = base + lane < end ? vs_n : 0.0f;
+        id_n = pool_id(id_nn, num_cache_blocks);
+        ask_scales(id_n, ks_n, vs_n);
+        id_nn = raw_id(base + 2 * kRun);
+    }
+    __device__ __forceinline__ int64_t id_at(int j) const { return __builtin_amdgcn_readlane(id, j); }
+    __device__ __forceinline__ float k_at(int j) const {
+        return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, ks), j));
+    }
+    __device__ __forceinline__ float v_at(int j) const {
+        return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, vs), j));
+    }
+};
 
 // 8 codes -> 8 bf16, exact
 template <Kv8Format F> __device__ __forceinline__ bf16x8 widen8(unsigned w0, unsigned w1) {
@@ -222,29 +318,33 @@ __device__ __forceinline__ unsigned nan_bytes(unsigned w) {
     return ((t & 0x80808080u) >> 7) * 0xffu;
 }
 
-template <Kv8Format F, int NQT, int HPB, int NBUF>
-__global__ __launch_bounds__(64 * HPB, NQT == 1 ? 2 : 1) void paged_attn_kv8_decode_kernel(
+template <Kv8Format F, int NQT, int W, int NBUF, bool STREAM>
+__global__ __launch_bounds__(64 * W, NQT == 1 ? 2 : 1) void paged_attn_kv8_decode_kernel(
     const __bf16 *__restrict__ q, const unsigned char *__restrict__ k_cache, const unsigned char *__restrict__ v_cache,
     const float *__restrict__ k_scales, const float *__restrict__ v_scales, const int32_t *__restrict__ block_tables,
     const int32_t *__restrict__ context_lens, __bf16 *__restrict__ out, float *__restrict__ ws_o,
     float *__restrict__ ws_ml, int T, int Hq, int Hkv, int max_blocks_per_seq, int64_t num_cache_blocks,
-    float scale_log2e, int num_splits, int blocks_per_split, bool stream) {
-    __shared__ __attribute__((aligned(16))) unsigned char lds_all[HPB * 2 * kImage];
+    float scale, int num_splits, int blocks_per_split) {
+    __shared__ __attribute__((aligned(16))) unsigned char lds_all[W * 2 * kImage];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4, c = lane & 15;
     const int split = blockIdx.x, seq = blockIdx.y;
-    const int kvh = blockIdx.z * HPB + wave;
-    if (kvh >= Hkv) return;  // whole wave; no barriers are used anywhere
+    const int kvh = blockIdx.z;
 
     const int G = Hq / Hkv, R = T * G;
     int ctx = context_lens[seq];
     const int64_t cap = (int64_t)max_blocks_per_seq * kBS;
     if (ctx > cap) ctx = (int)cap;  // never read past the table row
     const int nblk_seq = ctx > 0 ? (int)(((int64_t)ctx + kBS - 1) / kBS) : 0;
-    const int blk_begin = split * blocks_per_split;
+    int blk_begin = split * blocks_per_split;
     int blk_end = blk_begin + blocks_per_split;
     if (blk_end > nblk_seq) blk_end = nblk_seq;
+    // this wave's part, in whole tiles
+    const int all = blk_end > blk_begin ? blk_end - blk_begin : 0;
+    const int part = ((all + W - 1) / W + kTileBlocks - 1) / kTileBlocks * kTileBlocks;
+    blk_begin += wave * part;
+    if (blk_end > blk_begin + part) blk_end = blk_begin + part;
     const int ntiles = blk_end > blk_begin ? (blk_end - blk_begin + kTileBlocks - 1) / kTileBlocks : 0;
     unsigned char *lds_k = lds_all + wave * 2 * kImage, *lds_v = lds_k + kImage;
     const int32_t *table = block_tables + (int64_t)seq * max_blocks_per_seq;
@@ -252,6 +352,8 @@ __global__ __launch_bounds__(64 * HPB, NQT == 1 ? 2 : 1) void paged_attn_kv8_dec
     // Q^T fragments (B operand): k-step 2i + h of lane (g, c) holds Q[row c][16 (4i + g) + 8h .. + 7]
     bf16x8 qf[NQT][4];
     int t_of_row[NQT];
+    const unsigned flip = scale < 0.0f ? 0x80008000u : 0u;  // a negative scale moves into Q: factors stay >= 0
+    const float scale_log2e = fabsf(scale) * 1.4426950408889634f;
 #pragma unroll
     for (int qt = 0; qt < NQT; ++qt) {
         const int r = qt * 16 + c;
@@ -262,6 +364,8 @@ __global__ __launch_bounds__(64 * HPB, NQT == 1 ? 2 : 1) void paged_attn_kv8_dec
         for (int s = 0; s < 4; ++s) {
             u32x4 x = {0u, 0u, 0u, 0u};
             if (r < R) x = *reinterpret_cast<const u32x4 *>(qrow + 16 * (4 * (s >> 1) + g) + 8 * (s & 1));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] ^= flip;
             qf[qt][s] = __builtin_bit_cast(bf16x8, x);
         }
     }
@@ -269,7 +373,8 @@ __global__ __launch_bounds__(64 * HPB, NQT == 1 ? 2 : 1) void paged_attn_kv8_dec
     const int64_t block_bytes = (int64_t)kBS * Hkv * kD;
     const unsigned row_stride = (unsigned)Hkv * kD;
     const int lr = lane >> 3, lch = lane & 7;
-    const unsigned lane_off = (unsigned)lr * row_stride + (unsigned)kvh * kD + 16u * lch;
+    const int head_bytes = (kBS - 1) * (int)row_stride + kD;  // from a head's first byte of a block to its last
+    const unsigned lane_off = (unsigned)lr * row_stride + 16u * lch;
     const unsigned wr = (unsigned)(lr * kD + 16 * (lch ^ lr));                    // + 2048 b + 1024 i
     const unsigned krd0 = (unsigned)(c * kD + 16 * (g ^ (c & 7)));                // + 2048 b, chunk g
     const unsigned krd1 = (unsigned)(c * kD + 16 * ((4 + g) ^ (c & 7)));          // chunk 4 + g
@@ -278,59 +383,22 @@ __global__ __launch_bounds__(64 * HPB, NQT == 1 ? 2 : 1) void paged_attn_kv8_dec
     const unsigned tr_base = (unsigned)(tr_row * kD + 8 * (c & 1));
     const unsigned tr_sw = (unsigned)(tr_row & 7);
 
-    // ids and scales of the runs of 64 blocks.  Past the split's end: the last id (read, and masked), scale 0
-    auto run_ids = [&](int base) -> int {
-        int j = base + lane;
-        if (j >= blk_end) j = blk_end - 1;
-        return table[j];
-    };
-    auto clamp_id = [&](int id) -> int64_t {
-        int64_t x = id;
-        if (x < 0) x = 0;
-        if (x >= num_cache_blocks) x = num_cache_blocks - 1;
-        return x;
-    };
-    int id = 0, id_n = 0, id_nn = 0;
-    float ks = 0.f, vs = 0.f, ks_n = 0.f, vs_n = 0.f;
-    auto run_scales = [&](int base, int ids, float &a, float &b) {
-        const int64_t at = clamp_id(ids) * Hkv + kvh;
-        a = k_scales[at];
-        b = v_scales[at];
-        if (base + lane >= blk_end) a = b = 0.0f;
-    };
+    Run run{table, k_scales + kvh, v_scales + kvh, Hkv, blk_end, lane, num_cache_blocks};
     auto load_tile = [&](Tile &tl, int t) {
         const int j = (kTileBlocks * t) & (kRun - 1);
 #pragma unroll
         for (int b = 0; b < kTileBlocks; ++b) {
-            tl.ks[b] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, ks), j + b));
-            tl.vs[b] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, vs), j + b));
-        }
-        int64_t at[kTileBlocks];
-#pragma unroll
-        for (int b = 0; b < kTileBlocks; ++b) at[b] = clamp_id(__builtin_amdgcn_readlane(id, j + b)) * block_bytes;
-#pragma unroll
-        for (int b = 0; b < kTileBlocks; ++b)
+            tl.ks[b] = run.k_at(j + b);
+            tl.vs[b] = run.v_at(j + b);
+            const int64_t at = run.id_at(j + b) * block_bytes + kvh * kD;
+            const Rows k = block_rows(k_cache, at, head_bytes, t < ntiles), v = block_rows(v_cache, at, head_bytes, t < ntiles);
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const u32x4 *p = reinterpret_cast<const u32x4 *>(k_cache + at[b] + lane_off + (size_t)(8 * i) * row_stride);
-                tl.k[b][i] = stream ? __builtin_nontemporal_load(p) : *p;
+                tl.k[b][i] = load16<STREAM>(k, lane_off, 8 * i * row_stride);
+                tl.v[b][i] = load16<STREAM>(v, lane_off, 8 * i * row_stride);
             }
-#pragma unroll
-        for (int b = 0; b < kTileBlocks; ++b)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const u32x4 *p = reinterpret_cast<const u32x4 *>(v_cache + at[b] + lane_off + (size_t)(8 * i) * row_stride);
-                tl.v[b][i] = stream ? __builtin_nontemporal_load(p) : *p;
-            }
-        if (j == kRun - kTileBlocks) {  // the run's last tile: on to the next
-            const int base = blk_begin + kTileBlocks * (t + 1);
-            id = id_n;
-            ks = ks_n;
-            vs = vs_n;
-            id_n = id_nn;
-            run_scales(base + kRun, id_n, ks_n, vs_n);
-            id_nn = run_ids(base + 2 * kRun);
         }
+        if (j == kRun - kTileBlocks) run.advance(blk_begin + kTileBlocks * (t + 1));
     };
 
     float m_run[NQT], l_run[NQT];
@@ -437,41 +505,49 @@ __global__ __launch_bounds__(64 * HPB, NQT == 1 ? 2 : 1) void paged_attn_kv8_dec
 #pragma unroll
             for (int i = 0; i < 2; ++i) *reinterpret_cast<u32x4 *>(lds_v + wr + 2048 * b + 1024 * i) = tl.v[b][i];
         // online softmax in the exp2 domain; a query row's state lives in the lanes c = row
+        float f[kTileBlocks];
+#pragma unroll
+        for (int b = 0; b < kTileBlocks; ++b) f[b] = tl.ks[b] * scale_log2e;
+        if (tail) {
+#pragma unroll
+            for (int qt = 0; qt < NQT; ++qt)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const bool see = key0 + (j >> 2) * kBS + 4 * g + (j & 3) <= ctx - T + t_of_row[qt] &&
+                                     blk0 + (j >> 2) < blk_end;
+                    s[qt][j >> 2][j & 3] = see ? s[qt][j >> 2][j & 3] * f[j >> 2] : -INFINITY;
+                }
+#pragma unroll
+            for (int b = 0; b < kTileBlocks; ++b) f[b] = 1.0f;
+        }
         bf16x8 pf[NQT];
 #pragma unroll
         for (int qt = 0; qt < NQT; ++qt) {
-            float sv[8];
+            float mx = -INFINITY;
+#pragma unroll
+            for (int b = 0; b < kTileBlocks; ++b)  // factors are >= 0
+                mx = fmaxf(mx, f[b] * fmaxf(fmaxf(s[qt][b][0], s[qt][b][1]), fmaxf(s[qt][b][2], s[qt][b][3])));
+            mx = quad_max(mx);
+            if (__any(mx > m_run[qt] + kSlack)) {
+                const float m_new = fmaxf(m_run[qt], mx);
+                const float alpha = m_new == -INFINITY ? 1.0f : fast_exp2(m_run[qt] - m_new);
+                m_run[qt] = m_new;
+                l_run[qt] *= alpha;
+#pragma unroll
+                for (int dt = 0; dt < 8; ++dt) acc[qt][dt] *= alpha;
+            }
+            const float m_safe = m_run[qt] == -INFINITY ? 0.0f : m_run[qt];
+            float p[8], sum = 0.0f;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                sv[j] = s[qt][j >> 2][j & 3] * (tl.ks[j >> 2] * scale_log2e);
-                if (tail) {
-                    const bool see = key0 + (j >> 2) * kBS + 4 * g + (j & 3) <= ctx - T + t_of_row[qt] &&
-                                     blk0 + (j >> 2) < blk_end;
-                    sv[j] = see ? sv[j] : -INFINITY;
-                }
+                p[j] = fast_exp2(fmaf(s[qt][j >> 2][j & 3], f[j >> 2], -m_safe));
+                sum += p[j];
+                p[j] *= tl.vs[j >> 2];
             }
-            float mx = sv[0];
-#pragma unroll
-            for (int j = 1; j < 8; ++j) mx = fmaxf(mx, sv[j]);
-            mx = fmaxf(mx, __shfl_xor(mx, 16));
-            mx = fmaxf(mx, __shfl_xor(mx, 32));
-            const float m_new = fmaxf(m_run[qt], mx);
-            const float m_safe = m_new == -INFINITY ? 0.0f : m_new;
-            const float alpha = fast_exp2(m_run[qt] - m_safe);
-            float sum = 0.0f;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                sv[j] = fast_exp2(sv[j] - m_safe);
-                sum += sv[j];
-                sv[j] *= tl.vs[j >> 2];
-            }
-            l_run[qt] = l_run[qt] * alpha + sum;
-            m_run[qt] = m_new;
-#pragma unroll
-            for (int dt = 0; dt < 8; ++dt) acc[qt][dt] *= alpha;
+            l_run[qt] += sum;
             // the matrix unit takes p in bf16: each weight off by 2^-8 at most, as the output's own rounding
-            pf[qt] = __builtin_bit_cast(bf16x8, u32x4{pack_bf16x2(sv[0], sv[1]), pack_bf16x2(sv[2], sv[3]),
-                                                      pack_bf16x2(sv[4], sv[5]), pack_bf16x2(sv[6], sv[7])});
+            pf[qt] = __builtin_bit_cast(bf16x8, u32x4{pack_bf16x2(p[0], p[1]), pack_bf16x2(p[2], p[3]),
+                                                      pack_bf16x2(p[4], p[5]), pack_bf16x2(p[6], p[7])});
         }
         // O^T += V^T P^T
 #pragma unroll
@@ -485,48 +561,67 @@ __global__ __launch_bounds__(64 * HPB, NQT == 1 ? 2 : 1) void paged_attn_kv8_dec
     };
 
     if (ntiles > 0) {
-        id = run_ids(blk_begin);
-        id_n = run_ids(blk_begin + kRun);
-        run_scales(blk_begin, id, ks, vs);
-        run_scales(blk_begin + kRun, id_n, ks_n, vs_n);
-        id_nn = run_ids(blk_begin + 2 * kRun);
+        run.begin(blk_begin);
         Tile tl[NBUF];
 #pragma unroll
-        for (int u = 0; u < NBUF - 1; ++u)
-            if (u < ntiles) load_tile(tl[u], u);
+        for (int u = 0; u < NBUF - 1; ++u) load_tile(tl[u], u);
         for (int t = 0; t < ntiles; t += NBUF)
 #pragma unroll
-            for (int u = 0; u < NBUF; ++u)
-                if (t + u < ntiles) {
-                    if (t + u + NBUF - 1 < ntiles) load_tile(tl[(u + NBUF - 1) % NBUF], t + u + NBUF - 1);
-                    compute_tile(tl[u], t + u);
-                }
+            for (int u = 0; u < NBUF; ++u) {
+                load_tile(tl[(u + NBUF - 1) % NBUF], t + u + NBUF - 1);
+                if (t + u < ntiles) compute_tile(tl[u], t + u);
+            }
     }
 
+    // join the waves' parts, one query tile after the other: (m, l) of each row, then O relative to the common
+    // maximum, chunk 4 dt + g of row c at chunk position (4 dt + g) ^ c of its 512 bytes
+    __shared__ float ml[W][16][2];
+    float *mine = reinterpret_cast<float *>(lds_all + wave * 2 * kImage);
 #pragma unroll
     for (int qt = 0; qt < NQT; ++qt) {
         float l = l_run[qt];
         l += __shfl_xor(l, 16);
         l += __shfl_xor(l, 32);
-        const int r = qt * 16 + c;
-        if (r >= R) continue;
-        const int64_t orow = ((int64_t)seq * T + t_of_row[qt]) * Hq + kvh * G + (r - t_of_row[qt] * G);
-        if (num_splits == 1) {
-            const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // no key seen: zeros
-            __bf16 *op = out + orow * kD + 4 * g;
+        if (qt > 0) __syncthreads();  // the previous tile's sums have been read
+        if (g == 0) {
+            ml[wave][c][0] = m_run[qt];
+            ml[wave][c][1] = l;
+        }
+        __syncthreads();
+        float m = ml[0][c][0];
 #pragma unroll
-            for (int dt = 0; dt < 8; ++dt)
-                *reinterpret_cast<u32x2 *>(op + 16 * dt) =
-                    u32x2{pack_bf16x2(acc[qt][dt][0] * inv, acc[qt][dt][1] * inv),
-                          pack_bf16x2(acc[qt][dt][2] * inv, acc[qt][dt][3] * inv)};
-        } else {
-            const int64_t prow = orow * num_splits + split;
-            float *op = ws_o + prow * kD + 4 * g;
+        for (int w = 1; w < W; ++w) m = fmaxf(m, ml[w][c][0]);
+        const float f = m_run[qt] == -INFINITY ? 0.0f : fast_exp2(m_run[qt] - m);
 #pragma unroll
-            for (int dt = 0; dt < 8; ++dt) *reinterpret_cast<f32x4 *>(op + 16 * dt) = acc[qt][dt];
-            if (g == 0) {
-                ws_ml[2 * prow] = m_run[qt];
-                ws_ml[2 * prow + 1] = l;
+        for (int dt = 0; dt < 8; ++dt)
+            *reinterpret_cast<f32x4 *>(mine + 128 * c + 4 * ((4 * dt + g) ^ c)) = acc[qt][dt] * f;
+        __syncthreads();
+#pragma unroll
+        for (int i = threadIdx.x; i < 512; i += 64 * W) {
+            const int rr = i >> 5, chunk = i & 31, r = qt * 16 + rr;
+            if (r >= R) continue;
+            float mr = ml[0][rr][0], L = 0.0f;
+#pragma unroll
+            for (int w = 1; w < W; ++w) mr = fmaxf(mr, ml[w][rr][0]);
+            f32x4 y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int w = 0; w < W; ++w) {
+                L += ml[w][rr][0] == -INFINITY ? 0.0f : ml[w][rr][1] * fast_exp2(ml[w][rr][0] - mr);
+                y += *reinterpret_cast<const f32x4 *>(lds_all + w * 2 * kImage + 512 * rr + 16 * (chunk ^ rr));
+            }
+            const int t = r / G;
+            const int64_t orow = ((int64_t)seq * T + t) * Hq + kvh * G + (r - t * G);
+            if (num_splits == 1) {
+                const float inv = L == 0.0f ? 0.0f : 1.0f / L;  // no key seen: zeros
+                *reinterpret_cast<u32x2 *>(out + orow * kD + 4 * chunk) =
+                    u32x2{pack_bf16x2(y[0] * inv, y[1] * inv), pack_bf16x2(y[2] * inv, y[3] * inv)};
+            } else {
+                const int64_t prow = orow * num_splits + split;
+                *reinterpret_cast<f32x4 *>(ws_o + prow * kD + 4 * chunk) = y;
+                if (chunk == 0) {
+                    ws_ml[2 * prow] = mr;
+                    ws_ml[2 * prow + 1] = L;
+                }
             }
         }
     }
@@ -553,24 +648,6 @@ constexpr int kWideRow = 2 * kD;              // bytes of a widened row
 constexpr int kBigKeys = 64;                  // keys of a tile
 constexpr int kBigBlocks = kBigKeys / kBS;
 constexpr int kWideImage = kBigKeys * kWideRow;  // 16 KiB
-constexpr float kSlack = 8.0f;  // exponents may pass the reference by this before everything is rescaled
-
-// lane l's value and lane l ^ 32's.  In asm: given the builtin the same value twice, hipcc takes its two
-// results for equal.  s_nop 1 = the wait states between a vector write and the swap; the swap itself needs
-// none before its results are read.
-__device__ __forceinline__ void swap_halves(float &a, float &b) {
-    asm volatile("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(a), "+v"(b));
-}
-__device__ __forceinline__ float half_max(float x) {
-    float a = x, b = x;
-    swap_halves(a, b);
-    return fmaxf(a, b);
-}
-__device__ __forceinline__ float half_sum(float x) {
-    float a = x, b = x;
-    swap_halves(a, b);
-    return a + b;
-}
 
 template <Kv8Format F, int KG>
 __global__ __launch_bounds__(256, 2) void paged_attn_kv8_tile_kernel(
@@ -626,7 +703,8 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kv8_tile_kernel(
     // staging: thread covers 16 dims (lch) of rows tid / 8 and 32 + tid / 8 of the tile
     const int64_t block_bytes = (int64_t)kBS * Hkv * kD;
     const int sr = threadIdx.x >> 3, lch = threadIdx.x & 7;
-    const unsigned lane_off = (unsigned)(sr & 15) * (unsigned)(Hkv * kD) + (unsigned)kvh * kD + 16u * lch;
+    const int head_bytes = (kBS - 1) * Hkv * kD + kD;
+    const unsigned lane_off = (unsigned)(sr & 15) * (unsigned)(Hkv * kD) + 16u * lch;
     const int sb = wave >> 1;  // block of the first row within its 32 keys
     unsigned kw[2], vw[2];     // LDS positions of the two 16-byte chunks of the first row; the second: + 32 rows
 #pragma unroll
@@ -634,50 +712,23 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kv8_tile_kernel(
         kw[e] = (unsigned)(sr * kWideRow + 16 * ((2 * lch + e) ^ (sr & 15)));
         vw[e] = (unsigned)(kWideImage + sr * kWideRow + 16 * ((2 * lch + e) ^ (2 * (sr & 7))));
     }
-    // ids and scales of 64 blocks (16 tiles) at once, one a lane, as in the decode kernel
-    auto run_ids = [&](int base) -> int {
-        int j = base + lane;
-        if (j >= blk_end) j = blk_end - 1;
-        return table[j];
-    };
-    auto clamp_id = [&](int id) -> int64_t {
-        int64_t x = id;
-        if (x < 0) x = 0;
-        if (x >= num_cache_blocks) x = num_cache_blocks - 1;
-        return x;
-    };
-    auto run_scales = [&](int base, int ids, float &a, float &b) {
-        const int64_t at = clamp_id(ids) * Hkv + kvh;
-        a = k_scales[at];
-        b = v_scales[at];
-        if (base + lane >= blk_end) a = b = 0.0f;
-    };
-    int id = 0, id_n = 0, id_nn = 0;
-    float ks = 0.f, vs = 0.f, ks_n = 0.f, vs_n = 0.f;
+    Run run{table, k_scales + kvh, v_scales + kvh, Hkv, blk_end, lane, num_cache_blocks};
     u32x4 ck[2], cv[2];                          // codes on their way
     float fk[kBigBlocks], fv[kBigBlocks];        // scales of the tile that is loaded next / last
     auto load_tile = [&](int t) {
         const int j = (kBigBlocks * t) & (kRun - 1);
 #pragma unroll
         for (int b = 0; b < kBigBlocks; ++b) {
-            fk[b] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, ks), j + b)) * scale_log2e;
-            fv[b] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, vs), j + b));
+            fk[b] = run.k_at(j + b) * scale_log2e;
+            fv[b] = run.v_at(j + b);
         }
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const int64_t at = clamp_id(__builtin_amdgcn_readlane(id, j + 2 * i + sb)) * block_bytes;
-            ck[i] = *reinterpret_cast<const u32x4 *>(k_cache + at + lane_off);
-            cv[i] = *reinterpret_cast<const u32x4 *>(v_cache + at + lane_off);
+            const int64_t at = run.id_at(j + 2 * i + sb) * block_bytes + kvh * kD;
+            ck[i] = load16<false>(block_rows(k_cache, at, head_bytes, t < ntiles), lane_off, 0);
+            cv[i] = load16<false>(block_rows(v_cache, at, head_bytes, t < ntiles), lane_off, 0);
         }
-        if (j == kRun - kBigBlocks) {
-            const int base = blk_begin + kBigBlocks * (t + 1);
-            id = id_n;
-            ks = ks_n;
-            vs = vs_n;
-            id_n = id_nn;
-            run_scales(base + kRun, id_n, ks_n, vs_n);
-            id_nn = run_ids(base + 2 * kRun);
-        }
+        if (j == kRun - kBigBlocks) run.advance(blk_begin + kBigBlocks * (t + 1));
     };
     // codes of tile t -> bf16 in LDS.  V rows that no row of the tile sees are zeros; -> whether a NaN is
     // among the values that only some rows see (those become 0, see mark_nan)
@@ -769,9 +820,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kv8_tile_kernel(
             mx = fmaxf(mx, x * f[b]);
         }
         mx = half_max(mx);
-        // exponents are taken from a reference that moves only when a row's maximum has passed it by kSlack
-        // (p stays below 2^8, the sums in f32): most tiles then rescale nothing
-        if (__any(mx > m_ref + kSlack || (m_ref == -INFINITY && mx != -INFINITY))) {
+        if (__any(mx > m_ref + kSlack)) {
             const float m_new = fmaxf(m_ref, mx);
             const float alpha = m_new == -INFINITY ? 1.0f : fast_exp2(m_ref - m_new);
             m_ref = m_new;
@@ -814,8 +863,8 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kv8_tile_kernel(
             const int key = key0 + 32 * i + sr;
             u32x4 one = {0u, 0u, 0u, 0u};
             if (key < keys && key < blk_end * kBS) {
-                const int64_t at = clamp_id(table[key / kBS]) * block_bytes;
-                one = *reinterpret_cast<const u32x4 *>(v_cache + at + lane_off);
+                const int64_t at = pool_id(table[key / kBS], num_cache_blocks) * block_bytes;
+                one = *reinterpret_cast<const u32x4 *>(v_cache + at + kvh * kD + lane_off);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) one[e] = nan_bytes(one[e]) & 0x38383838u;  // 1.0
             }
@@ -850,11 +899,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kv8_tile_kernel(
     };
 
     if (ntiles > 0) {
-        id = run_ids(blk_begin);
-        id_n = run_ids(blk_begin + kRun);
-        run_scales(blk_begin, id, ks, vs);
-        run_scales(blk_begin + kRun, id_n, ks_n, vs_n);
-        id_nn = run_ids(blk_begin + 2 * kRun);
+        run.begin(blk_begin);
         float fk_t[kBigBlocks], fv_t[kBigBlocks], fk_n[kBigBlocks], fv_n[kBigBlocks];
         auto keep = [&](float (&a)[kBigBlocks], float (&b)[kBigBlocks]) {
 #pragma unroll
@@ -866,14 +911,14 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kv8_tile_kernel(
         load_tile(0);
         keep(fk_t, fv_t);
         bool nan_t = stage_tile(0, lds), nan_n = false;
-        if (ntiles > 1) load_tile(1);
+        load_tile(1);
         keep(fk_n, fv_n);
         if (F == Kv8Format::E4M3 && threadIdx.x == 0) nan_seen = 0;
         for (int t = 0; t < ntiles; ++t) {
             unsigned char *buf = lds + (t & 1) * 2 * kWideImage, *next = lds + ((t + 1) & 1) * 2 * kWideImage;
             __syncthreads();
             if (t + 1 < ntiles) nan_n = stage_tile(t + 1, next);
-            if (t + 2 < ntiles) load_tile(t + 2);
+            load_tile(t + 2);
             if (works) compute_tile(t, buf, fk_t, fv_t);
             if constexpr (F == Kv8Format::E4M3)
                 if ((blk_begin + kBigBlocks * (t + 1)) * kBS > keys_all) {  // the same for all waves
@@ -967,11 +1012,6 @@ int tile_splits(const PagedAttnArgs &a) {
     return splits < 1 ? 1 : (int)splits;
 }
 
-int splits_of(DType dt, const PagedAttnArgs &a) {
-    if (!fast_shape(dt, a)) return 1;
-    return decode_path(dt, a) ? paged_attn_num_splits(a.num_seqs, a.num_kv_heads, a.max_blocks_per_seq) : tile_splits(a);
-}
-
 // partials of a launch that is split: O and (m, l); false if the workspace is too small for them
 bool partials(const PagedAttnArgs &a, int splits, float **ws_o, float **ws_ml) {
     const size_t rows = (size_t)a.num_seqs * a.num_new_tokens * a.num_heads;
@@ -1007,37 +1047,48 @@ hipError_t launch_tile(const PagedAttnArgs &a, const float *ks, const float *vs,
                                    stream);
 }
 
-template <Kv8Format F, int NQT, int HPB>
-void launch_decode_as(const PagedAttnArgs &a, const float *ks, const float *vs, int splits, int bps, float *ws_o,
-                      float *ws_ml, bool stream_loads, hipStream_t stream) {
-    paged_attn_kv8_decode_kernel<F, NQT, HPB, NQT == 1 ? 3 : 4>
-        <<<dim3(splits, a.num_seqs, (a.num_kv_heads + HPB - 1) / HPB), dim3(64 * HPB), 0, stream>>>(
+int decode_waves(const PagedAttnArgs &a) { return query_rows(a) <= 16 ? 4 : 2; }
+
+// Parts of the keys over workgroups: up to 1024 waves in all (4 a CU), each with 64 keys at least.  Two parts do not
+// pay for the merge launch (16 x 2048: 20.8 against 20.7 us, 16 x 512: 9.3 against 8.3), unless half the CUs would
+// stay without the one workgroup of two or more query tiles that they hold.
+int decode_splits(const PagedAttnArgs &a) {
+    const int w = decode_waves(a), forced = launch_policy().paged_splits;
+    int64_t splits = 4 * (int64_t)device_cus() / ((int64_t)a.num_seqs * a.num_kv_heads * w);
+    const int64_t cap = a.max_blocks_per_seq / (4 * w);
+    if (forced > 0) splits = forced;
+    if (splits > cap) splits = cap;
+    if (splits > 64) splits = 64;  // the merge kernel holds one split's (m, l) per lane
+    if (splits < (w == 4 && forced <= 0 ? 3 : 2)) splits = 1;
+    return (int)splits;
+}
+
+template <Kv8Format F, int NQT, int W, bool STREAM>
+void launch_decode_as(const PagedAttnArgs &a, const float *ks, const float *vs, int splits, float *ws_o, float *ws_ml,
+                      hipStream_t stream) {
+    paged_attn_kv8_decode_kernel<F, NQT, W, NQT == 1 ? 3 : 4, STREAM>
+        <<<dim3(splits, a.num_seqs, a.num_kv_heads), dim3(64 * W), 0, stream>>>(
             static_cast<const __bf16 *>(a.q), static_cast<const unsigned char *>(a.k_cache),
             static_cast<const unsigned char *>(a.v_cache), ks, vs, a.block_tables, a.context_lens,
             static_cast<__bf16 *>(a.out), ws_o, ws_ml, a.num_new_tokens, a.num_heads, a.num_kv_heads,
-            a.max_blocks_per_seq, a.num_cache_blocks, a.scale * 1.4426950408889634f, splits, bps, stream_loads);
+            a.max_blocks_per_seq, a.num_cache_blocks, a.scale, splits, blocks_per_split(a, splits, kTileBlocks));
 }
 
 template <Kv8Format F>
 hipError_t launch_decode(const PagedAttnArgs &a, const float *ks, const float *vs, hipStream_t stream) {
-    const int splits = paged_attn_num_splits(a.num_seqs, a.num_kv_heads, a.max_blocks_per_seq);
+    const int splits = decode_splits(a);
     float *ws_o, *ws_ml;
     if (!partials(a, splits, &ws_o, &ws_ml)) return hipErrorInvalidValue;
-    const int bps = blocks_per_split(a, splits, kTileBlocks);
     // loads that do not stay in the caches, unless what the tables reach fits the 256 MiB Infinity Cache
     const int64_t reach = (int64_t)a.num_seqs * a.max_blocks_per_seq * 2 * kBS * a.num_kv_heads * kD;
     const bool nt = reach > ((int64_t)256 << 20);
-    // kv heads per workgroup: up to 8 waves share a block's rows; small launches spread over the CUs
-    int hpb = a.num_kv_heads >= 8 ? 8 : (a.num_kv_heads >= 4 ? 4 : (a.num_kv_heads >= 2 ? 2 : 1));
-    while (hpb > 1 && (int64_t)splits * a.num_seqs * ((a.num_kv_heads + hpb - 1) / hpb) < device_cus()) hpb /= 2;
-    const int nqt = (int)((query_rows(a) + 15) / 16);
-    if (nqt > 1 && hpb > 4) hpb = 4;  // the 512-register budget of a 4-wave workgroup
-#define NVLLM_KV8_CASE(NQT, HPB) \
-    case NQT * 16 + HPB: launch_decode_as<F, NQT, HPB>(a, ks, vs, splits, bps, ws_o, ws_ml, nt, stream); break;
-    switch (nqt * 16 + hpb) {
-        NVLLM_KV8_CASE(1, 8) NVLLM_KV8_CASE(1, 4) NVLLM_KV8_CASE(1, 2) NVLLM_KV8_CASE(1, 1)
-        NVLLM_KV8_CASE(2, 4) NVLLM_KV8_CASE(2, 2) NVLLM_KV8_CASE(2, 1)
-        NVLLM_KV8_CASE(3, 4) NVLLM_KV8_CASE(3, 2) NVLLM_KV8_CASE(3, 1)
+#define NVLLM_KV8_CASE(NQT, W)                                                                  \
+    case NQT:                                                                                   \
+        if (nt) launch_decode_as<F, NQT, W, true>(a, ks, vs, splits, ws_o, ws_ml, stream);      \
+        else launch_decode_as<F, NQT, W, false>(a, ks, vs, splits, ws_o, ws_ml, stream);        \
+        break;
+    switch ((int)((query_rows(a) + 15) / 16)) {
+        NVLLM_KV8_CASE(1, 4) NVLLM_KV8_CASE(2, 2) NVLLM_KV8_CASE(3, 2)
         default: return hipErrorInvalidValue;
     }
 #undef NVLLM_KV8_CASE
@@ -1045,6 +1096,11 @@ hipError_t launch_decode(const PagedAttnArgs &a, const float *ks, const float *v
     if (err != hipSuccess || splits == 1) return err;
     return launch_paged_attn_merge(ws_o, ws_ml, a.out, (int64_t)a.num_seqs * a.num_new_tokens * a.num_heads, splits,
                                    stream);
+}
+
+int splits_of(DType dt, const PagedAttnArgs &a) {
+    if (!fast_shape(dt, a)) return 1;
+    return decode_path(dt, a) ? decode_splits(a) : tile_splits(a);
 }
 
 }  // namespace

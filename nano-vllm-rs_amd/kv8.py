@@ -6,56 +6,76 @@ for a `KVCacheConfig` of one of these dtypes.  include/nvllm_attn.h says what a 
 Activations are bfloat16 or float32.  As in `attention`, tensors are contiguous and on a HIP device, all
 of a call on one; a call runs on that device's current stream.
 """
-import contextlib
-
 import torch
 
 from . import capi
-from .core import KV8_FORMATS, ConfigError, check
+from .core import ConfigError, check
 
 _DT = {torch.bfloat16: 0, torch.float32: 1}
+_FORMATS = {torch.int8: 0, torch.float8_e4m3fn: 1}
 
 
 def _refuse(message, code=capi.NVLLM_ERR_CONFIG):
     raise ConfigError(code, message)
 
 
-def _launch(device, *tensors):
-    """Checks what every tensor of a call has to be; returns the stream to launch on and the guard to
-    launch under."""
+# the current stream's handle (the public way makes a Stream object each time, 2 us of a call's 10)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _launch(tensors):
+    """Checks what every tensor of a call has to be; -> the device index."""
+    at = tensors[0].get_device()
     for t in tensors:
         if t is None:
             continue
-        if not t.is_cuda:
-            raise RuntimeError("nano_vllm_rs_amd operators need HIP device tensors (no CPU fallback exists)")
-        if t.device != device:
-            _refuse("tensors are on different devices: %s and %s" % (device, t.device))
+        if t.get_device() != at or at < 0:
+            if not t.is_cuda or at < 0:
+                raise RuntimeError("nano_vllm_rs_amd operators need HIP device tensors (no CPU fallback exists)")
+            _refuse("tensors are on different devices: %d and %d" % (at, t.get_device()))
         if not t.is_contiguous():
             _refuse("tensor must be contiguous")
-    guard = (contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device))
-    return torch.cuda.current_stream(device).cuda_stream, guard
+    return at
+
+
+def _on_device(function):
+    """Launches happen with the tensors' device current: `function(index, ...)` is called under a guard if it
+    is not."""
+
+    def call(index, *args):
+        if index == torch.cuda.current_device():
+            return function(index, *args)
+        with torch.cuda.device(index):
+            return function(index, *args)
+
+    return call
 
 
 def _cache(key_cache, value_cache, key_scales, value_scales):
     """-> (num_blocks, block_size, Hkv, D, format)"""
-    if key_cache.dtype not in KV8_FORMATS:
+    fmt = _FORMATS.get(key_cache.dtype)
+    if fmt is None:
         _refuse("cache dtype must be int8 or float8_e4m3fn, not %s" % key_cache.dtype, capi.NVLLM_ERR_UNSUPPORTED)
-    if key_cache.dim() != 4 or value_cache.shape != key_cache.shape or value_cache.dtype != key_cache.dtype:
+    shape = key_cache.shape
+    if len(shape) != 4 or value_cache.shape != shape or value_cache.dtype != key_cache.dtype:
         _refuse("key and value cache must be [num_blocks, block_size, Hkv, D] of one dtype")
-    nb, bs, hkv, d = key_cache.shape
+    nb, bs, hkv, d = shape
     for s in (key_scales, value_scales):
         if s.dtype != torch.float32 or s.shape != (nb, hkv):
             _refuse("scales must be float32 [num_blocks, Hkv]")
-    return nb, bs, hkv, d, KV8_FORMATS[key_cache.dtype]
+    return nb, bs, hkv, d, fmt
 
 
 def _dtype(t, *same):
-    if t.dtype not in _DT:
+    dtype = t.dtype
+    code = _DT.get(dtype)
+    if code is None:
         _refuse("dtype must be bfloat16 or float32", capi.NVLLM_ERR_UNSUPPORTED)
     for x in same:
-        if x is not None and x.dtype != t.dtype:
-            _refuse("dtypes differ: %s and %s" % (t.dtype, x.dtype))
-    return _DT[t.dtype]
+        if x is not None and x.dtype != dtype:
+            _refuse("dtypes differ: %s and %s" % (dtype, x.dtype))
+    return code
 
 
 def _write_workspace(workspace, n, bs, nb, device):
@@ -63,15 +83,11 @@ def _write_workspace(workspace, n, bs, nb, device):
         need = capi.lib().nvllm_kv8_write_workspace_bytes(n, bs, nb)
         if need:
             workspace = torch.empty(need, dtype=torch.uint8, device=device)
-    return workspace
+    return (workspace.data_ptr(), workspace.numel() * workspace.element_size()) if workspace is not None else (None, 0)
 
 
 def _p(t):
     return t.data_ptr() if t is not None else None
-
-
-def _size(t):
-    return t.numel() * t.element_size() if t is not None else 0
 
 
 def reshape_and_cache_kv8(key, value, key_cache, value_cache, key_scales, value_scales, slot_mapping,
@@ -86,13 +102,18 @@ def reshape_and_cache_kv8(key, value, key_cache, value_cache, key_scales, value_
     if slot_mapping.dtype != torch.int64 or slot_mapping.shape != (n,):
         _refuse("slot_mapping must be int64 [num_tokens]")
     dt = _dtype(key, value)
-    dev = key.device
-    stream, guard = _launch(dev, key, value, key_cache, value_cache, key_scales, value_scales, slot_mapping, workspace)
-    with guard:
-        ws = _write_workspace(workspace, n, bs, nb, dev)
-        check(capi.lib().nvllm_reshape_and_cache_kv8(
-            key.data_ptr(), value.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), key_scales.data_ptr(),
-            value_scales.data_ptr(), slot_mapping.data_ptr(), _p(ws), _size(ws), n, hkv, d, bs, nb, fmt, dt, stream))
+    index = _launch((key, value, key_cache, value_cache, key_scales, value_scales, slot_mapping, workspace))
+    _reshape_and_cache(index, key, value, key_cache, value_cache, key_scales, value_scales, slot_mapping, workspace,
+                       n, hkv, d, bs, nb, fmt, dt)
+
+
+@_on_device
+def _reshape_and_cache(index, key, value, key_cache, value_cache, key_scales, value_scales, slot_mapping, workspace,
+                       n, hkv, d, bs, nb, fmt, dt):
+    ws, size = _write_workspace(workspace, n, bs, nb, key.device)
+    check(capi.lib().nvllm_reshape_and_cache_kv8(
+        key.data_ptr(), value.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), key_scales.data_ptr(),
+        value_scales.data_ptr(), slot_mapping.data_ptr(), ws, size, n, hkv, d, bs, nb, fmt, dt, _raw_stream(index)))
 
 
 def qk_norm_rope_cache_kv8(query, key, value, q_weight, k_weight, eps, rotary, positions, key_cache, value_cache,
@@ -117,17 +138,22 @@ def qk_norm_rope_cache_kv8(query, key, value, q_weight, k_weight, eps, rotary, p
     if q_out.shape != query.shape or (k_out is not None and k_out.shape != key.shape):
         _refuse("q_out / k_out must have the shape of query / key")
     dt = _dtype(query, key, value, q_weight, k_weight, cos, sin, q_out, k_out)
-    dev = query.device
-    stream, guard = _launch(dev, query, key, value, q_weight, k_weight, cos, sin, positions, key_cache, value_cache,
-                            key_scales, value_scales, slot_mapping, k_out, q_out, workspace)
-    with guard:
-        ws = _write_workspace(workspace, n, bs, nb, dev)
-        check(capi.lib().nvllm_qk_norm_rope_cache_kv8(
-            query.data_ptr(), key.data_ptr(), value.data_ptr(), q_out.data_ptr(), _p(k_out), q_weight.data_ptr(),
-            k_weight.data_ptr(), float(eps), cos.data_ptr(), sin.data_ptr(), cos.shape[0], positions.data_ptr(),
-            key_cache.data_ptr(), value_cache.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(),
-            slot_mapping.data_ptr(), _p(ws), _size(ws), n, hq, hkv, d, bs, nb, fmt, dt, stream))
+    index = _launch((query, key, value, q_weight, k_weight, cos, sin, positions, key_cache, value_cache, key_scales,
+                     value_scales, slot_mapping, k_out, q_out, workspace))
+    _qk_norm_rope_cache(index, query, key, value, q_weight, k_weight, eps, cos, sin, positions, key_cache, value_cache,
+                        key_scales, value_scales, slot_mapping, k_out, q_out, workspace, n, hq, hkv, d, bs, nb, fmt, dt)
     return q_out
+
+
+@_on_device
+def _qk_norm_rope_cache(index, query, key, value, q_weight, k_weight, eps, cos, sin, positions, key_cache, value_cache,
+                        key_scales, value_scales, slot_mapping, k_out, q_out, workspace, n, hq, hkv, d, bs, nb, fmt, dt):
+    ws, size = _write_workspace(workspace, n, bs, nb, query.device)
+    check(capi.lib().nvllm_qk_norm_rope_cache_kv8(
+        query.data_ptr(), key.data_ptr(), value.data_ptr(), q_out.data_ptr(), _p(k_out), q_weight.data_ptr(),
+        k_weight.data_ptr(), float(eps), cos.data_ptr(), sin.data_ptr(), cos.shape[0], positions.data_ptr(),
+        key_cache.data_ptr(), value_cache.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(),
+        slot_mapping.data_ptr(), ws, size, n, hq, hkv, d, bs, nb, fmt, dt, _raw_stream(index)))
 
 
 def gather_cache_blocks_kv8(key_cache, value_cache, key_scales, value_scales, block_ids, dtype=torch.bfloat16):
@@ -138,15 +164,20 @@ def gather_cache_blocks_kv8(key_cache, value_cache, key_scales, value_scales, bl
         _refuse("block_ids must be int32 [n]")
     if dtype not in _DT:
         _refuse("dtype must be bfloat16 or float32", capi.NVLLM_ERR_UNSUPPORTED)
-    dev = key_cache.device
-    stream, guard = _launch(dev, key_cache, value_cache, key_scales, value_scales, block_ids)
-    n = block_ids.shape[0]
-    with guard:
-        out = torch.empty((2, n, bs, hkv, d), dtype=dtype, device=dev)
-        keys, values = out.unbind(0)
-        check(capi.lib().nvllm_gather_cache_blocks_kv8(
-            key_cache.data_ptr(), value_cache.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(),
-            block_ids.data_ptr(), n, keys.data_ptr(), values.data_ptr(), nb, bs, hkv, d, fmt, _DT[dtype], stream))
+    index = _launch((key_cache, value_cache, key_scales, value_scales, block_ids))
+    return _gather_cache_blocks(index, key_cache, value_cache, key_scales, value_scales, block_ids, dtype,
+                                block_ids.shape[0], nb, bs, hkv, d, fmt)
+
+
+@_on_device
+def _gather_cache_blocks(index, key_cache, value_cache, key_scales, value_scales, block_ids, dtype, n, nb, bs, hkv, d,
+                         fmt):
+    keys = torch.empty((n, bs, hkv, d), dtype=dtype, device=key_cache.device)
+    values = torch.empty_like(keys)
+    check(capi.lib().nvllm_gather_cache_blocks_kv8(
+        key_cache.data_ptr(), value_cache.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(),
+        block_ids.data_ptr(), n, keys.data_ptr(), values.data_ptr(), nb, bs, hkv, d, fmt, _DT[dtype],
+        _raw_stream(index)))
     return keys, values
 
 
@@ -176,19 +207,23 @@ def paged_attention_kv8(query, key_cache, value_cache, key_scales, value_scales,
     if block_tables.dim() != 2 or block_tables.shape[0] != n or context_lens.shape != (n,):
         _refuse("block_tables must be [num_seqs, max_blocks], context_lens [num_seqs]")
     dt = _dtype(query)
-    dev = query.device
-    stream, guard = _launch(dev, query, key_cache, value_cache, key_scales, value_scales, block_tables, context_lens,
-                            workspace)
-    width = block_tables.shape[1]
+    index = _launch((query, key_cache, value_cache, key_scales, value_scales, block_tables, context_lens, workspace))
+    return _paged_attention(index, query, key_cache, value_cache, key_scales, value_scales, block_tables, context_lens,
+                            float(scale), workspace, n, t, hq, hkv, d, bs, block_tables.shape[1], nb, fmt, dt)
+
+
+@_on_device
+def _paged_attention(index, query, key_cache, value_cache, key_scales, value_scales, block_tables, context_lens, scale,
+                     workspace, n, t, hq, hkv, d, bs, width, nb, fmt, dt):
     L = capi.lib()
-    with guard:
-        out = torch.empty((n, t, hq * d), dtype=query.dtype, device=dev)
-        if workspace is None:
-            need = L.nvllm_paged_attn_kv8_workspace_bytes(n, t, hq, hkv, d, bs, width, dt)
-            if need:
-                workspace = torch.empty(need, dtype=torch.uint8, device=dev)
-        check(L.nvllm_paged_attn_kv8(
-            query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), key_scales.data_ptr(),
-            value_scales.data_ptr(), block_tables.data_ptr(), context_lens.data_ptr(), out.data_ptr(), _p(workspace),
-            _size(workspace), n, t, hq, hkv, d, bs, width, nb, float(scale), fmt, dt, stream))
+    out = torch.empty((n, t, hq * d), dtype=query.dtype, device=query.device)
+    if workspace is None:
+        need = L.nvllm_paged_attn_kv8_workspace_bytes(n, t, hq, hkv, d, bs, width, dt)
+        if need:
+            workspace = torch.empty(need, dtype=torch.uint8, device=query.device)
+    size = workspace.numel() * workspace.element_size() if workspace is not None else 0
+    check(L.nvllm_paged_attn_kv8(
+        query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), key_scales.data_ptr(),
+        value_scales.data_ptr(), block_tables.data_ptr(), context_lens.data_ptr(), out.data_ptr(), _p(workspace),
+        size, n, t, hq, hkv, d, bs, width, nb, scale, fmt, dt, _raw_stream(index)))
     return out
