@@ -411,6 +411,7 @@ __global__ __launch_bounds__(64 * W, NQT == 1 ? 2 : 1) void paged_attn_kv8_decod
         for (int dt = 0; dt < 8; ++dt) acc[qt][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
     const int first_masked = ctx - (T - 1);  // first key that some query row cannot see
+    unsigned nan_seen = 0;                   // among the values of the tiles from there on
 
     // A operand of P.V: 8 keys (4g .. 4g+3 of both blocks) of dim 16 dt + c
     auto v_fragment = [&](int dt) -> bf16x8 {
@@ -419,65 +420,24 @@ __global__ __launch_bounds__(64 * W, NQT == 1 ? 2 : 1) void paged_attn_kv8_decod
             __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i32x2 *)(lds_v + tr_base + 16u * ((unsigned)dt ^ tr_sw)));
         return widen8<F>((unsigned)w[0], (unsigned)w[1]);
     };
-    // A NaN among the values of keys that some rows must not see: 0 * NaN would reach those rows.  Which
-    // (dim, row) pairs do see one is a product of zeros and ones; they become NaN here, and the code 0.
-    auto mark_nan = [&](Tile &tl, int t) {
-        const int blk0 = blk_begin + kTileBlocks * t, key0 = blk0 * kBS;
-#pragma unroll
-        for (int b = 0; b < kTileBlocks; ++b)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                u32x4 one;
-#pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    const unsigned n = nan_bytes(tl.v[b][i][w]);
-                    one[w] = n & 0x38383838u;  // 1.0
-                    tl.v[b][i][w] &= ~n;
-                }
-                *reinterpret_cast<u32x4 *>(lds_v + wr + 2048 * b + 1024 * i) = one;
-            }
-        u32x4 see[NQT];
-#pragma unroll
-        for (int qt = 0; qt < NQT; ++qt)
-#pragma unroll
-            for (int e = 0; e < 8; e += 2) {
-                const int key = key0 + (e >> 2) * kBS + 4 * g + (e & 3), last = ctx - T + t_of_row[qt];
-                see[qt][e >> 1] = (key <= last ? 0x3f80u : 0u) | (key + 1 <= last ? 0x3f800000u : 0u);
-            }
-#pragma unroll
-        for (int dt = 0; dt < 8; ++dt) {
-            const bf16x8 one = v_fragment(dt);
-#pragma unroll
-            for (int qt = 0; qt < NQT; ++qt) {
-                const f32x4 hit = __builtin_amdgcn_mfma_f32_16x16x32_bf16(one, __builtin_bit_cast(bf16x8, see[qt]),
-                                                                          f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) acc[qt][dt][e] = hit[e] > 0.0f ? __builtin_nanf("") : acc[qt][dt][e];
-            }
-        }
-    };
-
     auto compute_tile = [&](Tile &tl, int t) {
         const int blk0 = blk_begin + kTileBlocks * t, key0 = blk0 * kBS;
         const bool tail = key0 + kTileKeys > first_masked || blk0 + kTileBlocks > blk_end;
-        bool has_nan = false;
         if (tail) {  // V rows past the context hold anything: zeros, so that 0 * them is 0
 #pragma unroll
             for (int b = 0; b < kTileBlocks; ++b)
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     if (key0 + b * kBS + 8 * i + lr >= ctx || blk0 + b >= blk_end) tl.v[b][i] = u32x4{0u, 0u, 0u, 0u};
-                    if constexpr (F == Kv8Format::E4M3) {
-                        unsigned any = 0;
+                    if constexpr (F == Kv8Format::E4M3)  // and so for a NaN that only some rows see (below)
 #pragma unroll
-                        for (int w = 0; w < 4; ++w) any |= nan_bytes(tl.v[b][i][w]);
-                        has_nan |= any != 0;
-                    }
+                        for (int w = 0; w < 4; ++w) {
+                            const unsigned n = nan_bytes(tl.v[b][i][w]);
+                            nan_seen |= n;
+                            tl.v[b][i][w] &= ~n;
+                        }
                 }
-            has_nan = __any(has_nan);
         }
-        if constexpr (F == Kv8Format::E4M3)
-            if (has_nan) mark_nan(tl, t);
 #pragma unroll
         for (int b = 0; b < kTileBlocks; ++b)
 #pragma unroll
@@ -573,6 +533,47 @@ __global__ __launch_bounds__(64 * W, NQT == 1 ? 2 : 1) void paged_attn_kv8_decod
             }
     }
 
+    if constexpr (F == Kv8Format::E4M3)
+        if (__any(nan_seen != 0)) {
+            // A NaN among values that some rows must not see (0 * NaN would have reached them, so the loop took it for
+            // 0): which (dim, row) pairs do see one is a product of zeros and ones.
+            for (int t = 0; t < ntiles; ++t) {
+                const int blk0 = blk_begin + kTileBlocks * t, key0 = blk0 * kBS;
+                if (key0 + kTileKeys <= first_masked && blk0 + kTileBlocks <= blk_end) continue;
+#pragma unroll
+                for (int b = 0; b < kTileBlocks; ++b)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        u32x4 one = {0u, 0u, 0u, 0u};
+                        if (key0 + b * kBS + 8 * i + lr < ctx && blk0 + b < blk_end) {
+                            const int64_t at = pool_id(table[blk0 + b], num_cache_blocks) * block_bytes + kvh * kD;
+                            one = *reinterpret_cast<const u32x4 *>(v_cache + at + 8 * i * row_stride + lane_off);
+#pragma unroll
+                            for (int w = 0; w < 4; ++w) one[w] = nan_bytes(one[w]) & 0x38383838u;  // 1.0
+                        }
+                        *reinterpret_cast<u32x4 *>(lds_v + wr + 2048 * b + 1024 * i) = one;
+                    }
+#pragma unroll
+                for (int dt = 0; dt < 8; ++dt) {
+                    const bf16x8 one = v_fragment(dt);
+#pragma unroll
+                    for (int qt = 0; qt < NQT; ++qt) {
+                        u32x4 see;
+#pragma unroll
+                        for (int e = 0; e < 8; e += 2) {
+                            const int key = key0 + (e >> 2) * kBS + 4 * g + (e & 3), last = ctx - T + t_of_row[qt];
+                            see[e >> 1] = (key <= last ? 0x3f80u : 0u) | (key + 1 <= last ? 0x3f800000u : 0u);
+                        }
+                        const f32x4 hit = __builtin_amdgcn_mfma_f32_16x16x32_bf16(one, __builtin_bit_cast(bf16x8, see),
+                                                                                  f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) acc[qt][dt][e] = hit[e] > 0.0f ? __builtin_nanf("") : acc[qt][dt][e];
+                    }
+                }
+                settle();
+            }
+        }
+
     // join the waves' parts, one query tile after the other: (m, l) of each row, then O relative to the common
     // maximum, chunk 4 dt + g of row c at chunk position (4 dt + g) ^ c of its 512 bytes
     __shared__ float ml[W][16][2];
@@ -649,6 +650,10 @@ constexpr int kBigKeys = 64;                  // keys of a tile
 constexpr int kBigBlocks = kBigKeys / kBS;
 constexpr int kWideImage = kBigKeys * kWideRow;  // 16 KiB
 
+struct Scales {  // of a tile's blocks, wave-uniform
+    float k[kBigBlocks], v[kBigBlocks];
+};
+
 template <Kv8Format F, int KG>
 __global__ __launch_bounds__(256, 2) void paged_attn_kv8_tile_kernel(
     const __bf16 *__restrict__ q, const unsigned char *__restrict__ k_cache, const unsigned char *__restrict__ v_cache,
@@ -657,6 +662,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kv8_tile_kernel(
     float *__restrict__ ws_ml, int T, int Hq, int Hkv, int max_blocks_per_seq, int64_t num_cache_blocks, float scale,
     int num_splits, int blocks_per_split) {
     constexpr int kRows = 128 / KG, NS = 2 / KG;  // rows of the workgroup; 32-key score tiles of a wave
+    constexpr int AHEAD = KG;                      // tiles of codes in registers
     __shared__ __attribute__((aligned(16))) unsigned char lds[4 * kWideImage];  // [buffer][K, V]
     __shared__ int nan_seen;
     const int lane = threadIdx.x & 63;
@@ -713,14 +719,12 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kv8_tile_kernel(
         vw[e] = (unsigned)(kWideImage + sr * kWideRow + 16 * ((2 * lch + e) ^ (2 * (sr & 7))));
     }
     Run run{table, k_scales + kvh, v_scales + kvh, Hkv, blk_end, lane, num_cache_blocks};
-    u32x4 ck[2], cv[2];                          // codes on their way
-    float fk[kBigBlocks], fv[kBigBlocks];        // scales of the tile that is loaded next / last
-    auto load_tile = [&](int t) {
+    auto load_tile = [&](int t, u32x4 (&ck)[2], u32x4 (&cv)[2], Scales &sc) {
         const int j = (kBigBlocks * t) & (kRun - 1);
 #pragma unroll
         for (int b = 0; b < kBigBlocks; ++b) {
-            fk[b] = run.k_at(j + b) * scale_log2e;
-            fv[b] = run.v_at(j + b);
+            sc.k[b] = run.k_at(j + b);
+            sc.v[b] = run.v_at(j + b);
         }
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -730,11 +734,11 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kv8_tile_kernel(
         }
         if (j == kRun - kBigBlocks) run.advance(blk_begin + kBigBlocks * (t + 1));
     };
-    // codes of tile t -> bf16 in LDS.  V rows that no row of the tile sees are zeros; -> whether a NaN is
-    // among the values that only some rows see (those become 0, see mark_nan)
-    auto stage_tile = [&](int t, unsigned char *buf) -> bool {
+    // codes of tile t -> bf16 in LDS.  V rows that no row of the tile sees are zeros, and so is a NaN that only some
+    // rows see (below)
+    unsigned nan_here = 0;
+    auto stage_tile = [&](int t, unsigned char *buf, u32x4 (&ck)[2], u32x4 (&cv)[2]) {
         const int key0 = (blk_begin + kBigBlocks * t) * kBS;
-        bool has_nan = false;
         if (key0 + kBigKeys > keys_all) {
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
@@ -742,14 +746,12 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kv8_tile_kernel(
                 if (key >= keys || key >= blk_end * kBS) cv[i] = u32x4{0u, 0u, 0u, 0u};
                 if constexpr (F == Kv8Format::E4M3)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) has_nan |= nan_bytes(cv[i][e]) != 0;
+                    for (int e = 0; e < 4; ++e) {
+                        const unsigned n = nan_bytes(cv[i][e]);
+                        nan_here |= n;
+                        cv[i][e] &= ~n;
+                    }
             }
-            if constexpr (F == Kv8Format::E4M3)
-                if (has_nan)
-#pragma unroll
-                    for (int i = 0; i < 2; ++i)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) cv[i][e] &= ~nan_bytes(cv[i][e]);
         }
 #pragma unroll
         for (int i = 0; i < 2; ++i)
@@ -758,7 +760,6 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kv8_tile_kernel(
                 *reinterpret_cast<bf16x8 *>(buf + kw[e] + 32 * kWideRow * i) = widen8<F>(ck[i][2 * e], ck[i][2 * e + 1]);
                 *reinterpret_cast<bf16x8 *>(buf + vw[e] + 32 * kWideRow * i) = widen8<F>(cv[i][2 * e], cv[i][2 * e + 1]);
             }
-        return has_nan;
     };
 
     float m_ref = -INFINITY, l_run = 0.0f;
@@ -781,8 +782,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kv8_tile_kernel(
         return __builtin_bit_cast(bf16x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
     };
 
-    auto compute_tile = [&](int t, const unsigned char *buf, const float (&fk_t)[kBigBlocks],
-                            const float (&fv_t)[kBigBlocks]) {
+    auto compute_tile = [&](int t, const unsigned char *buf, const Scales &sc) {
         const int key0 = (blk_begin + kBigBlocks * t) * kBS + 32 * kg;
         f32x16 s[NS];
 #pragma unroll
@@ -799,7 +799,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kv8_tile_kernel(
         // element i of score tile n is key 32 n + 8 (i / 4) + 4 h + i % 4: block 2 n + i / 8
         float f[2 * NS];
 #pragma unroll
-        for (int b = 0; b < 2 * NS; ++b) f[b] = fk_t[2 * kg + b];
+        for (int b = 0; b < 2 * NS; ++b) f[b] = (kg == 0 ? sc.k[b] : sc.k[kBigBlocks - 2 * NS + b]) * scale_log2e;
         if (key0 + 32 * NS > keys_all || key0 + 32 * NS > blk_end * kBS) {
 #pragma unroll
             for (int n = 0; n < NS; ++n)
@@ -835,12 +835,13 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kv8_tile_kernel(
         bf16x8 pf[2 * NS];  // P^T as B operand, 16 keys each
 #pragma unroll
         for (int b = 0; b < 2 * NS; ++b) {
+            const float v_scale = kg == 0 ? sc.v[b] : sc.v[kBigBlocks - 2 * NS + b];
             float p[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 p[i] = fast_exp2(fmaf(s[b / 2][8 * (b % 2) + i], f[b], -m_safe));
                 sum += p[i];
-                p[i] *= fv_t[2 * kg + b];
+                p[i] *= v_scale;
             }
             pf[b] = __builtin_bit_cast(bf16x8, u32x4{pack_bf16x2(p[0], p[1]), pack_bf16x2(p[2], p[3]),
                                                      pack_bf16x2(p[4], p[5]), pack_bf16x2(p[6], p[7])});
@@ -853,90 +854,77 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kv8_tile_kernel(
                 acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v_fragment(buf, b, dt), pf[b], acc[dt], 0, 0, 0);
         settle();
     };
-    // NaN values that only some rows of the tile see (0 * NaN would reach the others): which (dim, row) pairs
-    // see one is a product of zeros and ones.  The whole workgroup; `buf`'s V is overwritten.
-    auto mark_nan = [&](int t, unsigned char *buf) {
-        const int key0 = (blk_begin + kBigBlocks * t) * kBS;
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int key = key0 + 32 * i + sr;
-            u32x4 one = {0u, 0u, 0u, 0u};
-            if (key < keys && key < blk_end * kBS) {
-                const int64_t at = pool_id(table[key / kBS], num_cache_blocks) * block_bytes;
-                one = *reinterpret_cast<const u32x4 *>(v_cache + at + kvh * kD + lane_off);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) one[e] = nan_bytes(one[e]) & 0x38383838u;  // 1.0
-            }
-#pragma unroll
-            for (int e = 0; e < 2; ++e)
-                *reinterpret_cast<bf16x8 *>(buf + vw[e] + 32 * kWideRow * i) = widen8<F>(one[2 * e], one[2 * e + 1]);
-        }
-        __syncthreads();
-        if (works) {
-#pragma unroll 1
-            for (int b = 0; b < 2 * NS; ++b) {
-                u32x4 see;
-#pragma unroll
-                for (int e = 0; e < 8; e += 2) {
-                    const int key = key0 + 32 * kg + 16 * b + 8 * (e / 4) + 4 * h + e % 4;
-                    see[e / 2] = (key <= last ? 0x3f80u : 0u) | (key + 1 <= last ? 0x3f800000u : 0u);
-                }
-#pragma unroll
-                for (int dt = 0; dt < 4; ++dt) {
-                    f32x16 z;
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) z[i] = 0.0f;
-                    z = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v_fragment(buf, b, dt), __builtin_bit_cast(bf16x8, see),
-                                                                z, 0, 0, 0);
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) acc[dt][i] = z[i] > 0.0f ? __builtin_nanf("") : acc[dt][i];
-                }
-            }
-            settle();
-        }
-        __syncthreads();
-    };
-
+    if (F == Kv8Format::E4M3 && threadIdx.x == 0) nan_seen = 0;
     if (ntiles > 0) {
         run.begin(blk_begin);
-        float fk_t[kBigBlocks], fv_t[kBigBlocks], fk_n[kBigBlocks], fv_n[kBigBlocks];
-        auto keep = [&](float (&a)[kBigBlocks], float (&b)[kBigBlocks]) {
+        // in flight: tiles t + 2 .. t + 1 + AHEAD while tile t is multiplied and t + 1 goes into LDS
+        u32x4 ck[AHEAD][2], cv[AHEAD][2];
+        Scales sc[AHEAD + 1];
+        load_tile(0, ck[0], cv[0], sc[0]);
+        stage_tile(0, lds, ck[0], cv[0]);
 #pragma unroll
-            for (int i = 0; i < kBigBlocks; ++i) {
-                a[i] = fk[i];
-                b[i] = fv[i];
+        for (int u = 1; u <= AHEAD; ++u) load_tile(u, ck[u - 1], cv[u - 1], sc[u]);
+        for (int t0 = 0; t0 < ntiles; t0 += 2)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int t = t0 + u;
+                __syncthreads();
+                stage_tile(t + 1, lds + (1 - u) * 2 * kWideImage, ck[u % AHEAD], cv[u % AHEAD]);
+                Scales next;
+                load_tile(t + 1 + AHEAD, ck[u % AHEAD], cv[u % AHEAD], next);
+                if (works && t < ntiles) compute_tile(t, lds + u * 2 * kWideImage, sc[0]);
+#pragma unroll
+                for (int a = 0; a < AHEAD; ++a) sc[a] = sc[a + 1];
+                sc[AHEAD] = next;
             }
-        };
-        load_tile(0);
-        keep(fk_t, fv_t);
-        bool nan_t = stage_tile(0, lds), nan_n = false;
-        load_tile(1);
-        keep(fk_n, fv_n);
-        if (F == Kv8Format::E4M3 && threadIdx.x == 0) nan_seen = 0;
-        for (int t = 0; t < ntiles; ++t) {
-            unsigned char *buf = lds + (t & 1) * 2 * kWideImage, *next = lds + ((t + 1) & 1) * 2 * kWideImage;
-            __syncthreads();
-            if (t + 1 < ntiles) nan_n = stage_tile(t + 1, next);
-            load_tile(t + 2);
-            if (works) compute_tile(t, buf, fk_t, fv_t);
-            if constexpr (F == Kv8Format::E4M3)
-                if ((blk_begin + kBigBlocks * (t + 1)) * kBS > keys_all) {  // the same for all waves
-                    if (nan_t) nan_seen = 1;
-                    __syncthreads();
-                    const bool any = nan_seen != 0;
-                    __syncthreads();
-                    if (any) mark_nan(t, buf);
-                    if (threadIdx.x == 0) nan_seen = 0;
-                    __syncthreads();
+    }
+    if constexpr (F == Kv8Format::E4M3) {
+        __syncthreads();
+        if (nan_here) nan_seen = 1;
+        __syncthreads();
+        if (nan_seen) {
+            // A NaN among values that only some rows of the tile see (0 * NaN would have reached the others, so it was
+            // taken for 0): which (dim, row) pairs see one is a product of zeros and ones.
+            for (int t = 0; t < ntiles; ++t) {
+                const int key0 = (blk_begin + kBigBlocks * t) * kBS;
+                if (key0 + kBigKeys <= keys_all) continue;
+                __syncthreads();
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int key = key0 + 32 * i + sr;
+                    u32x4 one = {0u, 0u, 0u, 0u};
+                    if (key < keys && key < blk_end * kBS) {
+                        const int64_t at = pool_id(table[key / kBS], num_cache_blocks) * block_bytes + kvh * kD;
+                        one = *reinterpret_cast<const u32x4 *>(v_cache + at + lane_off);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) one[e] = nan_bytes(one[e]) & 0x38383838u;  // 1.0
+                    }
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+                        *reinterpret_cast<bf16x8 *>(lds + vw[e] + 32 * kWideRow * i) = widen8<F>(one[2 * e], one[2 * e + 1]);
                 }
-            nan_t = nan_n;
+                __syncthreads();
+#pragma unroll 1
+                for (int b = 0; b < 2 * NS; ++b) {
+                    u32x4 see;
 #pragma unroll
-            for (int i = 0; i < kBigBlocks; ++i) {
-                fk_t[i] = fk_n[i];
-                fv_t[i] = fv_n[i];
+                    for (int e = 0; e < 8; e += 2) {
+                        const int key = key0 + 32 * kg + 16 * b + 8 * (e / 4) + 4 * h + e % 4;
+                        see[e / 2] = (key <= last ? 0x3f80u : 0u) | (key + 1 <= last ? 0x3f800000u : 0u);
+                    }
+#pragma unroll
+                    for (int dt = 0; dt < 4; ++dt) {
+                        f32x16 z;
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) z[i] = 0.0f;
+                        z = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v_fragment(lds, b, dt),
+                                                                    __builtin_bit_cast(bf16x8, see), z, 0, 0, 0);
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) acc[dt][i] = z[i] > 0.0f ? __builtin_nanf("") : acc[dt][i];
+                    }
+                    settle();
+                }
             }
-            keep(fk_n, fv_n);
         }
     }
 
