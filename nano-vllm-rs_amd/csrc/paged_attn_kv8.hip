@@ -637,10 +637,15 @@ __global__ __launch_bounds__(64 * W, NQT == 1 ? 2 : 1) void paged_attn_kv8_decod
 //   KG = 2: 64 rows; waves 0, 1 take the first 32 keys of each tile and waves 2, 3 the others, so that the
 //           four SIMDs share the work of few rows; the two halves join through LDS at the end.
 // Codes come in as in the decode kernel, but are widened to bf16 ONCE for all rows on their way into LDS
-// (two buffers of K and V, one barrier a tile); two tiles are on their way in registers and LDS while one is
-// multiplied.  S^T = K Q^T and O^T = V^T P^T with mfma_f32_32x32x16_bf16: a query row lives in the lanes
+// (two buffers of K and V, one barrier a tile); two tiles are on their way, one in registers and one in LDS,
+// while one is multiplied.  S^T = K Q^T and O^T = V^T P^T with mfma_f32_32x32x16_bf16: a query row lives in the lanes
 // c and c + 32, P needs no lane movement.  LDS: row r, 16-byte chunk ch of K at position ch ^ (r & 15), of V
 // at ch ^ 2 (r & 7) (transposed reads of 4 rows x 16 dims).
+//
+// Bounds: with many rows the products and, between them, the exponentials (chunk of 4 x 1024 rows behind 7168 keys,
+// 2.6e11 operations: 282 us, 910 TFLOP/s); with few the way of the bytes into LDS (64 x 4096 T = 13, 537 MB: 123 us,
+// 4.4 TB/s; the same without the products 106, without the widening 125).  Two tiles in registers instead of one, 8-byte
+// staging with half the LDS conflicts and products interleaved with the exponentials by hand were each within 3 % or slower.
 // ---------------------------------------------------------------------------
 typedef __attribute__((ext_vector_type(16))) float f32x16;
 typedef __attribute__((ext_vector_type(4))) short s16x4;
@@ -654,7 +659,7 @@ struct Scales {  // of a tile's blocks, wave-uniform
     float k[kBigBlocks], v[kBigBlocks];
 };
 
-template <Kv8Format F, int KG>
+template <Kv8Format F, int KG, bool STREAM>
 __global__ __launch_bounds__(256, 2) void paged_attn_kv8_tile_kernel(
     const __bf16 *__restrict__ q, const unsigned char *__restrict__ k_cache, const unsigned char *__restrict__ v_cache,
     const float *__restrict__ k_scales, const float *__restrict__ v_scales, const int32_t *__restrict__ block_tables,
@@ -662,7 +667,6 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kv8_tile_kernel(
     float *__restrict__ ws_ml, int T, int Hq, int Hkv, int max_blocks_per_seq, int64_t num_cache_blocks, float scale,
     int num_splits, int blocks_per_split) {
     constexpr int kRows = 128 / KG, NS = 2 / KG;  // rows of the workgroup; 32-key score tiles of a wave
-    constexpr int AHEAD = KG;                      // tiles of codes in registers
     __shared__ __attribute__((aligned(16))) unsigned char lds[4 * kWideImage];  // [buffer][K, V]
     __shared__ int nan_seen;
     const int lane = threadIdx.x & 63;
@@ -729,8 +733,8 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kv8_tile_kernel(
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const int64_t at = run.id_at(j + 2 * i + sb) * block_bytes + kvh * kD;
-            ck[i] = load16<false>(block_rows(k_cache, at, head_bytes, t < ntiles), lane_off, 0);
-            cv[i] = load16<false>(block_rows(v_cache, at, head_bytes, t < ntiles), lane_off, 0);
+            ck[i] = load16<STREAM>(block_rows(k_cache, at, head_bytes, t < ntiles), lane_off, 0);
+            cv[i] = load16<STREAM>(block_rows(v_cache, at, head_bytes, t < ntiles), lane_off, 0);
         }
         if (j == kRun - kBigBlocks) run.advance(blk_begin + kBigBlocks * (t + 1));
     };
@@ -857,25 +861,23 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kv8_tile_kernel(
     if (F == Kv8Format::E4M3 && threadIdx.x == 0) nan_seen = 0;
     if (ntiles > 0) {
         run.begin(blk_begin);
-        // in flight: tiles t + 2 .. t + 1 + AHEAD while tile t is multiplied and t + 1 goes into LDS
-        u32x4 ck[AHEAD][2], cv[AHEAD][2];
-        Scales sc[AHEAD + 1];
-        load_tile(0, ck[0], cv[0], sc[0]);
-        stage_tile(0, lds, ck[0], cv[0]);
-#pragma unroll
-        for (int u = 1; u <= AHEAD; ++u) load_tile(u, ck[u - 1], cv[u - 1], sc[u]);
+        // codes of tile t + 2 are on their way while tile t is multiplied and t + 1 goes into LDS
+        u32x4 ck[2], cv[2];
+        Scales sc[2];
+        load_tile(0, ck, cv, sc[0]);
+        stage_tile(0, lds, ck, cv);
+        load_tile(1, ck, cv, sc[1]);
         for (int t0 = 0; t0 < ntiles; t0 += 2)
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 const int t = t0 + u;
                 __syncthreads();
-                stage_tile(t + 1, lds + (1 - u) * 2 * kWideImage, ck[u % AHEAD], cv[u % AHEAD]);
+                stage_tile(t + 1, lds + (1 - u) * 2 * kWideImage, ck, cv);
                 Scales next;
-                load_tile(t + 1 + AHEAD, ck[u % AHEAD], cv[u % AHEAD], next);
+                load_tile(t + 2, ck, cv, next);
                 if (works && t < ntiles) compute_tile(t, lds + u * 2 * kWideImage, sc[0]);
-#pragma unroll
-                for (int a = 0; a < AHEAD; ++a) sc[a] = sc[a + 1];
-                sc[AHEAD] = next;
+                sc[0] = sc[1];
+                sc[1] = next;
             }
     }
     if constexpr (F == Kv8Format::E4M3) {
@@ -989,11 +991,16 @@ bool decode_path(DType dt, const PagedAttnArgs &a) { return fast_shape(dt, a) &&
 // workgroups of 64 rows while that is all there is, else of 128
 int tile_rows(const PagedAttnArgs &a) { return query_rows(a) <= 64 ? 64 : 128; }
 
-// Parts of the key walk: enough for two workgroups on every CU, each part 256 keys at least
+// Parts of the key walk: two workgroups on every CU, each part 256 keys at least.  One workgroup on every CU is more than
+// half as fast as two, so with as many as that a second part pays for the merge only where the walk is long (256
+// workgroups: 2048 keys 53 us whole, 81 us in two parts; 8192 keys 183 and 185; 16384 keys 270 and 247); fewer always do
+// (128 workgroups of 4096 keys: 69 us whole, 49 in two parts, 43 in four).
 int tile_splits(const PagedAttnArgs &a) {
     const int64_t rows = tile_rows(a);
     const int64_t units = (int64_t)a.num_seqs * a.num_kv_heads * ((query_rows(a) + rows - 1) / rows);
-    int64_t splits = 2 * device_cus() / units;
+    const int forced = launch_policy().paged_splits;
+    int64_t splits = forced > 0 ? forced : 2 * device_cus() / units;
+    if (forced <= 0 && splits == 2 && a.max_blocks_per_seq < 8192 / kBS) splits = 1;
     const int64_t most = a.max_blocks_per_seq / 16;
     if (splits > most) splits = most;
     if (splits > 64) splits = 64;  // the merge kernel holds one split's (m, l) per lane
@@ -1016,14 +1023,21 @@ int blocks_per_split(const PagedAttnArgs &a, int splits, int granule) {
     return (bps + granule - 1) / granule * granule;
 }
 
-template <Kv8Format F, int KG>
+// Loads that do not stay in the caches, unless what the tables reach fits the 256 MiB Infinity Cache, or other
+// workgroups read the keys too (more than one tile of rows).  64 x 4096 T = 13 (1 GiB) 134 us without, 123 with; a chunk
+// of 4 x 1024 rows behind 7168 keys 276 without, 281 with.
+bool streams(const PagedAttnArgs &a) {
+    return (int64_t)a.num_seqs * a.max_blocks_per_seq * 2 * kBS * a.num_kv_heads * kD > ((int64_t)256 << 20);
+}
+
+template <Kv8Format F, int KG, bool STREAM>
 hipError_t launch_tile(const PagedAttnArgs &a, const float *ks, const float *vs, hipStream_t stream) {
     const int splits = tile_splits(a), rows = 128 / KG;
     float *ws_o, *ws_ml;
     if (!partials(a, splits, &ws_o, &ws_ml)) return hipErrorInvalidValue;
     const int64_t tiles = (query_rows(a) + rows - 1) / rows;
     if (tiles > 65535) return hipErrorInvalidValue;
-    paged_attn_kv8_tile_kernel<F, KG>
+    paged_attn_kv8_tile_kernel<F, KG, STREAM>
         <<<dim3((unsigned)(a.num_seqs * a.num_kv_heads), (unsigned)tiles, splits), dim3(256), 0, stream>>>(
             static_cast<const __bf16 *>(a.q), static_cast<const unsigned char *>(a.k_cache),
             static_cast<const unsigned char *>(a.v_cache), ks, vs, a.block_tables, a.context_lens,
@@ -1033,6 +1047,12 @@ hipError_t launch_tile(const PagedAttnArgs &a, const float *ks, const float *vs,
     if (err != hipSuccess || splits == 1) return err;
     return launch_paged_attn_merge(ws_o, ws_ml, a.out, (int64_t)a.num_seqs * a.num_new_tokens * a.num_heads, splits,
                                    stream);
+}
+
+template <Kv8Format F>
+hipError_t launch_tile_of(const PagedAttnArgs &a, const float *ks, const float *vs, hipStream_t stream) {
+    if (tile_rows(a) != 64) return launch_tile<F, 1, false>(a, ks, vs, stream);
+    return streams(a) ? launch_tile<F, 2, true>(a, ks, vs, stream) : launch_tile<F, 2, false>(a, ks, vs, stream);
 }
 
 int decode_waves(const PagedAttnArgs &a) { return query_rows(a) <= 16 ? 4 : 2; }
@@ -1067,9 +1087,7 @@ hipError_t launch_decode(const PagedAttnArgs &a, const float *ks, const float *v
     const int splits = decode_splits(a);
     float *ws_o, *ws_ml;
     if (!partials(a, splits, &ws_o, &ws_ml)) return hipErrorInvalidValue;
-    // loads that do not stay in the caches, unless what the tables reach fits the 256 MiB Infinity Cache
-    const int64_t reach = (int64_t)a.num_seqs * a.max_blocks_per_seq * 2 * kBS * a.num_kv_heads * kD;
-    const bool nt = reach > ((int64_t)256 << 20);
+    const bool nt = streams(a);
 #define NVLLM_KV8_CASE(NQT, W)                                                                  \
     case NQT:                                                                                   \
         if (nt) launch_decode_as<F, NQT, W, true>(a, ks, vs, splits, ws_o, ws_ml, stream);      \
@@ -1112,11 +1130,8 @@ hipError_t launch_paged_attn_kv8(DType dt, Kv8Format fmt, const PagedAttnArgs &a
         return int8 ? launch_decode<Kv8Format::Int8>(a, k_scales, v_scales, stream)
                     : launch_decode<Kv8Format::E4M3>(a, k_scales, v_scales, stream);
     if (fast_shape(dt, a)) {
-        if (tile_rows(a) == 64)
-            return int8 ? launch_tile<Kv8Format::Int8, 2>(a, k_scales, v_scales, stream)
-                        : launch_tile<Kv8Format::E4M3, 2>(a, k_scales, v_scales, stream);
-        return int8 ? launch_tile<Kv8Format::Int8, 1>(a, k_scales, v_scales, stream)
-                    : launch_tile<Kv8Format::E4M3, 1>(a, k_scales, v_scales, stream);
+        return int8 ? launch_tile_of<Kv8Format::Int8>(a, k_scales, v_scales, stream)
+                    : launch_tile_of<Kv8Format::E4M3>(a, k_scales, v_scales, stream);
     }
     if (dt == DType::BF16)
         return fmt == Kv8Format::Int8 ? launch_generic<__bf16, Kv8Format::Int8>(a, k_scales, v_scales, stream)

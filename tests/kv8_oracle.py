@@ -101,5 +101,5 @@ def attend(q, k, v, ks, vs, tables, lens, scale):
                 p /= p.sum()
                 out[i, t, h] = p @ vv[:see, h // G]
                 mean[i, t, h] = p @ np.abs(vv[:see, h // G])
-                reach[i, t, h] = (np.abs(kk[:see, h // G]) @ np.abs(q[i, t, h]) * scale).max()
+                reach[i, t, h] = (np.abs(kk[:see, h // G]) @ np.abs(q[i, t, h]) * abs(scale)).max()
     return out, mean, reach

@@ -222,6 +222,35 @@ def test_blocks_past_32_bits_of_bytes(dev, fmt):
     call(dict(far, lens=torch.zeros_like(on["lens"])), 0.1)
 
 
+@pytest.mark.parametrize("fmt", FMT)
+@pytest.mark.parametrize("splits", [1, 2, 3, 7, 64])
+@pytest.mark.parametrize("T", [1, 5, 13, 40])
+def test_any_number_of_parts(dev, policy, fmt, splits, T):
+    """the key walk in a forced number of parts: lengths that end in every part, parts without keys"""
+    policy.setenv("NVLLM_PAGED_SPLITS", splits)
+    rng = np.random.default_rng(splits)
+    check(rng, fmt, "bf16", [n for n in (0, 1, T, 700, 1023, 1024, 1025, 2500) if n == 0 or n >= T], T, 8, 2, 128, 16,
+          dev)
+
+
+@pytest.mark.parametrize("fmt", FMT)
+@pytest.mark.parametrize("T", [1, 4, 13, 30])
+def test_tables_that_reach_past_the_caches(dev, fmt, T):
+    """rows of the table wide enough that the launch streams its loads (more than 256 MiB in reach)"""
+    rng = np.random.default_rng(15)
+    check(rng, fmt, "bf16", [T, 300, 1111], T, 16, 8, 128, 16, dev, slack=3000)
+
+
+@pytest.mark.parametrize("fmt", FMT)
+@pytest.mark.parametrize("dtype,D,bs", [("bf16", 128, 16), ("f32", 64, 8)])
+@pytest.mark.parametrize("T", [1, 6, 20, 70])
+@pytest.mark.parametrize("scale", [-0.2, 0.0])
+def test_softmax_scales_without_a_plus(dev, fmt, dtype, D, bs, T, scale):
+    rng = np.random.default_rng(16)
+    on, host = make(rng, fmt, dtype, [T, 90, 500], T, 8, 4, D, bs, dev)
+    compare(call(on, scale), host, scale, dtype)
+
+
 @pytest.mark.parametrize("T,lens", [(1, [70, 300]), (1, [5000]), (5, [800, 9]), (40, [500, 77])])
 def test_same_bits_again_on_another_stream_and_in_a_graph(dev, T, lens):
     """no result depends on the order of anything: repeated, side by side on two streams, replayed from a
