@@ -289,35 +289,36 @@ __device__ __forceinline__ void unpack8(u32x4 w, float *x) {
     }
 }
 
-// norm and rotation of a row that 8 lanes hold (a[8] dims 8 ch .., b[8] dims 64 + 8 ch ..), in place
+// Norm and rotation of a row that 8 lanes hold (lo: dims 8 ch .. + 7, hi: 64 + 8 ch ..; y[0 .. 7], y[8 .. 15]), in AT;
+// in f32, f64 results are rounded to odd.
 template <typename AT>
-__device__ __forceinline__ void rotate_row(AT *a, AT *b, const __bf16 *w, const __bf16 *cos_row, const __bf16 *sin_row,
-                                           int ch, float eps) {
+__device__ __forceinline__ void rotate_row(u32x4 lo, u32x4 hi, const __bf16 *w, const __bf16 *cos_row,
+                                           const __bf16 *sin_row, int ch, float eps, float *y) {
+    const auto get = [&](const __bf16 *p, u32x4 &l, u32x4 &h) {
+        l = *reinterpret_cast<const u32x4 *>(p + 8 * ch);
+        h = *reinterpret_cast<const u32x4 *>(p + 64 + 8 * ch);
+    };
+    u32x4 w1, w2, c1, c2, s1, s2;
+    get(cos_row, c1, c2);
+    get(sin_row, s1, s2);
+    get(w, w1, w2);
+    const auto at = [](u32x4 p, int i) -> AT { return (AT)(i & 1 ? bf16_hi(p[i / 2]) : bf16_lo(p[i / 2])); };
     AT ss = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) ss += a[i] * a[i] + b[i] * b[i];
+    for (int i = 0; i < 8; ++i) ss += at(lo, i) * at(lo, i) + at(hi, i) * at(hi, i);
 #pragma unroll
     for (int m = 1; m < 8; m <<= 1) ss += __shfl_xor(ss, m);
     const AT inv = (AT)1 / (AT)sqrt((AT)(ss * (AT)(1.0 / kFastD) + (AT)eps));
-    float w1[8], w2[8], c1[8], c2[8], s1[8], s2[8];
-    const auto get = [&](const __bf16 *p, float *lo, float *hi) {
-        unpack8(*reinterpret_cast<const u32x4 *>(p + 8 * ch), lo);
-        unpack8(*reinterpret_cast<const u32x4 *>(p + 64 + 8 * ch), hi);
-    };
-    get(w, w1, w2);
-    get(cos_row, c1, c2);
-    get(sin_row, s1, s2);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const AT n1 = a[i] * inv * (AT)w1[i], n2 = b[i] * inv * (AT)w2[i];
-        a[i] = n1 * (AT)c1[i] - n2 * (AT)s1[i];
-        b[i] = n2 * (AT)c2[i] + n1 * (AT)s2[i];
+        const AT n1 = at(lo, i) * inv * at(w1, i), n2 = at(hi, i) * inv * at(w2, i);
+        y[i] = narrow_odd(n1 * at(c1, i) - n2 * at(s1, i));
+        y[8 + i] = narrow_odd(n2 * at(c2, i) + n1 * at(s2, i));
     }
 }
 
 template <Kv8Format F, bool ROT>
 __device__ __forceinline__ void write_fast_unit(const Kv8WriteArgs &a, const int *map, int block, int head, bool is_v) {
-    typedef typename std::conditional<ROT, double, float>::type AT;  // rotated values: see RotatedRow
     const int lane = threadIdx.x & 63, r = lane >> 3, ch = lane & 7;
     const int Hkv = a.num_kv_heads;
     const __bf16 *src = static_cast<const __bf16 *>(is_v ? a.value : a.key);
@@ -325,38 +326,38 @@ __device__ __forceinline__ void write_fast_unit(const Kv8WriteArgs &a, const int
     const bool begins = map[0] >= 0;
     const float was = begins ? 0.0f : *sp;
     u32x4 w[2][2];
-    int t[2];
+    int t[2], pos[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         t[i] = map[r + 8 * i];
+        pos[i] = 0;
         w[i][0] = w[i][1] = u32x4{0u, 0u, 0u, 0u};
         if (t[i] >= 0) {
+            if constexpr (ROT) pos[i] = a.positions[t[i]];
             const __bf16 *p = src + ((int64_t)t[i] * Hkv + head) * kFastD;
             w[i][0] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(p + dim_of<ROT>(ch, 0)));
             w[i][1] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(p + dim_of<ROT>(ch, 1)));
         }
     }
-    AT x[2][16];
+    float x[2][16];
     float amax = 0.0f;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-        float f[16];
-        unpack8(w[i][0], f);
-        unpack8(w[i][1], f + 8);
-#pragma unroll
-        for (int j = 0; j < 16; ++j) x[i][j] = f[j];
         if constexpr (ROT) {
-            int pos = t[i] >= 0 ? a.positions[t[i]] : 0;
-            pos = pos < 0 ? 0 : (pos >= a.max_positions ? a.max_positions - 1 : pos);  // stay inside the tables
-            rotate_row<AT>(x[i], x[i] + 8, static_cast<const __bf16 *>(a.k_weight),
-                           static_cast<const __bf16 *>(a.cos_cache) + (int64_t)pos * kFastD,
-                           static_cast<const __bf16 *>(a.sin_cache) + (int64_t)pos * kFastD, ch, a.eps);
+            const int at = pos[i] < 0 ? 0 : (pos[i] >= a.max_positions ? a.max_positions - 1 : pos[i]);  // inside the tables
+            rotate_row<double>(w[i][0], w[i][1], static_cast<const __bf16 *>(a.k_weight),
+                               static_cast<const __bf16 *>(a.cos_cache) + (int64_t)at * kFastD,
+                               static_cast<const __bf16 *>(a.sin_cache) + (int64_t)at * kFastD, ch, a.eps, x[i]);
             if (t[i] < 0)  // a row of zeros with eps 0 is NaN here
 #pragma unroll
-                for (int j = 0; j < 16; ++j) x[i][j] = 0;
+                for (int j = 0; j < 16; ++j) x[i][j] = 0.0f;
+            __builtin_amdgcn_sched_barrier(0);  // one row after the other: both at once take 170 registers
+        } else {
+            unpack8(w[i][0], x[i]);
+            unpack8(w[i][1], x[i] + 8);
         }
 #pragma unroll
-        for (int j = 0; j < 16; ++j) amax = fmaxf(amax, finite_abs((float)x[i][j]));
+        for (int j = 0; j < 16; ++j) amax = fmaxf(amax, finite_abs(x[i][j]));
     }
     const float s = fmaxf(was, scale_of<F>(wave_max(amax)));
     const float inv = inverse_scale(s);
@@ -369,8 +370,7 @@ __device__ __forceinline__ void write_fast_unit(const Kv8WriteArgs &a, const int
         unsigned c[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-            c[j] = encode4<F>(narrow_odd(x[i][4 * j] * (AT)inv), narrow_odd(x[i][4 * j + 1] * (AT)inv),
-                              narrow_odd(x[i][4 * j + 2] * (AT)inv), narrow_odd(x[i][4 * j + 3] * (AT)inv));
+            c[j] = encode4<F>(x[i][4 * j] * inv, x[i][4 * j + 1] * inv, x[i][4 * j + 2] * inv, x[i][4 * j + 3] * inv);
         if constexpr (ROT) {
             // even lanes have dims 8 ch and 64 + 8 ch; trade with the neighbour for 16 dims in a row:
             // even lanes 8 ch .. + 15, odd lanes 64 + 8 (ch - 1) .. + 15
@@ -397,7 +397,7 @@ __device__ __forceinline__ void write_fast_unit(const Kv8WriteArgs &a, const int
 // Workgroups [0, chunk_blocks * parts): part `% parts` of chunk `/ parts`; behind them (producer) rows of Q, and of
 // K to k_out, 8 lanes a row, 32 rows a workgroup.
 template <Kv8Format F, bool PRODUCER>
-__global__ __launch_bounds__(kThreads) void kv8_write_kernel(const Kv8WriteArgs a, int chunk, int parts,
+__global__ __launch_bounds__(kThreads, PRODUCER ? 4 : 1) void kv8_write_kernel(const Kv8WriteArgs a, int chunk, int parts,
                                                              int chunk_blocks, bool indexed) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int Hkv = a.num_kv_heads;
@@ -415,16 +415,17 @@ __global__ __launch_bounds__(kThreads) void kv8_write_kernel(const Kv8WriteArgs 
             __bf16 *y = static_cast<__bf16 *>(is_q ? a.q_out : a.k_out) + at;
             int pos = a.positions[t];
             pos = pos < 0 ? 0 : (pos >= a.max_positions ? a.max_positions - 1 : pos);
-            float lo[8], hi[8];
-            unpack8(__builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(p + 8 * ch)), lo);
-            unpack8(__builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(p + 64 + 8 * ch)), hi);
-            rotate_row<float>(lo, hi, static_cast<const __bf16 *>(is_q ? a.q_weight : a.k_weight),
+            float x[16];
+            rotate_row<float>(__builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(p + 8 * ch)),
+                              __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(p + 64 + 8 * ch)),
+                              static_cast<const __bf16 *>(is_q ? a.q_weight : a.k_weight),
                               static_cast<const __bf16 *>(a.cos_cache) + (int64_t)pos * kFastD,
-                              static_cast<const __bf16 *>(a.sin_cache) + (int64_t)pos * kFastD, ch, a.eps);
-            *reinterpret_cast<u32x4 *>(y + 8 * ch) = u32x4{pack_bf16x2(lo[0], lo[1]), pack_bf16x2(lo[2], lo[3]),
-                                                           pack_bf16x2(lo[4], lo[5]), pack_bf16x2(lo[6], lo[7])};
-            *reinterpret_cast<u32x4 *>(y + 64 + 8 * ch) = u32x4{pack_bf16x2(hi[0], hi[1]), pack_bf16x2(hi[2], hi[3]),
-                                                                pack_bf16x2(hi[4], hi[5]), pack_bf16x2(hi[6], hi[7])};
+                              static_cast<const __bf16 *>(a.sin_cache) + (int64_t)pos * kFastD, ch, a.eps, x);
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                *reinterpret_cast<u32x4 *>(y + 64 * i + 8 * ch) =
+                    u32x4{pack_bf16x2(x[8 * i], x[8 * i + 1]), pack_bf16x2(x[8 * i + 2], x[8 * i + 3]),
+                          pack_bf16x2(x[8 * i + 4], x[8 * i + 5]), pack_bf16x2(x[8 * i + 6], x[8 * i + 7])};
             return;
         }
     }
