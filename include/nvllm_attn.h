@@ -263,7 +263,7 @@ int nvllm_qk_norm_rope_cache_f32(const void *q, const void *k, const void *v, vo
  * written; a negative slot, or one past the pool, skips its token.  Two calls that run at the same
  * time must not write the same block. */
 
-/* Workspace of the two writers below: 0 up to 4096 tokens, else 4 bytes per slot of the pool.  Its
+/* Workspace of the two writers below: 0 up to 1024 tokens, else 4 bytes per slot of the pool.  Its
  * contents need no preparation and mean nothing between calls; calls that overlap in time need one
  * each.  A smaller one (or one not 16-byte aligned) is NVLLM_ERR_CONFIG. */
 size_t nvllm_kv8_write_workspace_bytes(int64_t num_tokens, int block_size, int64_t num_cache_blocks);

@@ -33,8 +33,9 @@ constexpr int kWaves = kThreads / 64;
 constexpr int kMaxChunk = 16;  // tokens a workgroup looks after
 
 // Up to this many tokens every workgroup reads the whole slot mapping to find its blocks' tokens;
-// above, a launch in front leaves slot -> token in the workspace.
-constexpr int64_t kScanTokens = 4096;
+// above, a launch in front leaves slot -> token in the workspace.  (Scanned against indexed, us: prompts of 256 7.1 and
+// 8.4, 1024 9.0 and 9.7, 2048 11.2 and 11.2, 4096 14.0 and 12.0; decode steps of 1024 8.6 and 8.5, of 2048 12.0 and 9.2.)
+constexpr int64_t kScanTokens = 1024;
 
 // slot -> token for every slot the call writes.  Nothing is cleared first: an entry counts only if
 // the token it names writes that very slot, so whatever else the workspace holds is seen through.
@@ -61,6 +62,8 @@ struct Chunk {
     int *map;      // [kMaxChunk * bs]
     int *owner;    // [kMaxChunk]
     int *block;    // [kMaxChunk]: the different blocks of the chunk's slots
+    int *rows;     // [kMaxChunk + 1] or none: rows of the u-th block, if the call writes one (o | 0xff00) or two
+                   // (o | o' << 8) of them, else -1; and how many of the chunk's own blocks those are
 };
 
 __device__ __forceinline__ int find_blocks(const Chunk &ch, const int64_t *__restrict__ slots, int n, int t0,
@@ -81,10 +84,7 @@ __device__ __forceinline__ int find_blocks(const Chunk &ch, const int64_t *__res
         }
         const unsigned long long m = __ballot(first);
         if (first) ch.block[__popcll(m & ((1ull << tid) - 1))] = b;
-        if (tid == 0) {
-            uniques = __popcll(m);
-            count = 0;
-        }
+        if (tid == 0) uniques = __popcll(m);
     }
     __syncthreads();
     const int nu = uniques;
@@ -107,13 +107,23 @@ __device__ __forceinline__ int find_blocks(const Chunk &ch, const int64_t *__res
         }
     }
     __syncthreads();
-    if (tid < nu) {
-        int first = n;
-        for (int o = 0; o < bs; ++o) {
+    if (tid < 64) {
+        int first = n, some = 0xffff, many = 0;
+        for (int o = 0; tid < nu && o < bs; ++o) {
             const int t = ch.map[tid * bs + o];
-            if (t >= 0 && t < first) first = t;
+            if (t < 0) continue;
+            if (t < first) first = t;
+            if (++many <= 2) some = many == 1 ? 0xff00 | o : (some & 255) | o << 8;
         }
-        if (first >= t0 && first < t0 + chunk) ch.owner[atomicAdd(&count, 1)] = tid;
+        if (ch.rows && tid < nu) ch.rows[tid] = many <= 2 ? some : -1;
+        const bool mine = tid < nu && first >= t0 && first < t0 + chunk;
+        const unsigned long long m = __ballot(mine);  // the same order in every workgroup that looks after the chunk
+        if (mine) ch.owner[__popcll(m & ((1ull << tid) - 1))] = tid;
+        const unsigned long long f = __ballot(mine && many <= 2);
+        if (tid == 0) {
+            count = __popcll(m);
+            if (ch.rows) ch.rows[kMaxChunk] = __popcll(f);
+        }
     }
     __syncthreads();
     return count;
@@ -220,7 +230,7 @@ __global__ __launch_bounds__(kThreads) void kv8_write_generic_kernel(const Kv8Wr
     extern __shared__ int dyn[];
     __shared__ int owner[kMaxChunk];
     __shared__ int block[kMaxChunk];
-    const Chunk ch{dyn, owner, block};
+    const Chunk ch{dyn, owner, block, nullptr};
     const int bs = a.block_size, n = (int)a.num_tokens, t0 = ((int)blockIdx.x - row_blocks) * chunk;
     const int count = find_blocks(ch, a.slot_mapping, n, t0, chunk, bs, a.num_cache_blocks * bs,
                                   indexed ? a.workspace : nullptr);
@@ -269,8 +279,9 @@ hipError_t launch_generic(const Kv8WriteArgs &a, bool indexed, hipStream_t strea
 // Bound by HBM on prompts (K and V read once, half as many bytes written) and by latency on a decode step.
 // A wave takes one (block, kv head) of K or V: 8 lanes a row, two rows a lane (o and o + 8), so the block is
 // read with four 16-byte loads a lane, its maximum found with six shuffles and written with two 16-byte
-// stores, all rows of the block at once.  `parts` workgroups share a chunk's units, so that a decode step's
-// few tokens still spread over the chip.
+// stores, all rows of the block at once.  Of a block that gets one or two rows (a decode step) a wave takes
+// eight heads instead, 8 lanes those of one head: the producer's decode step of 256 (32 and 8 heads) 9.4 -> 6.3
+// us, of 1024 30 -> 11.4.  `parts` workgroups share a chunk's units, so that few tokens still spread over the chip.
 // ---------------------------------------------------------------------------
 constexpr int kFastD = 128;
 constexpr int kFastBS = 16;
@@ -317,19 +328,24 @@ __device__ __forceinline__ void rotate_row(u32x4 lo, u32x4 hi, const __bf16 *w, 
     }
 }
 
-template <Kv8Format F, bool ROT>
-__device__ __forceinline__ void write_fast_unit(const Kv8WriteArgs &a, const int *map, int block, int head, bool is_v) {
+// FEW: a block of which the call writes one or two rows (`rows`: which).  8 lanes then take those of one head, and the
+// wave eight heads from `head0` on.
+template <Kv8Format F, bool ROT, bool FEW>
+__device__ __forceinline__ void write_fast_unit(const Kv8WriteArgs &a, const int *map, int rows, int block, int head0,
+                                                bool is_v) {
     const int lane = threadIdx.x & 63, r = lane >> 3, ch = lane & 7;
-    const int Hkv = a.num_kv_heads;
+    const int Hkv = a.num_kv_heads, head = FEW ? head0 + r : head0;
+    const bool valid = !FEW || head < Hkv;
     const __bf16 *src = static_cast<const __bf16 *>(is_v ? a.value : a.key);
     float *sp = (is_v ? a.v_scales : a.k_scales) + (int64_t)block * Hkv + head;
     const bool begins = map[0] >= 0;
-    const float was = begins ? 0.0f : *sp;
+    const float was = begins || !valid ? 0.0f : *sp;
     u32x4 w[2][2];
-    int t[2], pos[2];
+    int o[2], t[2], pos[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-        t[i] = map[r + 8 * i];
+        o[i] = FEW ? rows >> (8 * i) & 255 : r + 8 * i;
+        t[i] = valid && o[i] < kFastBS ? map[o[i]] : -1;
         pos[i] = 0;
         w[i][0] = w[i][1] = u32x4{0u, 0u, 0u, 0u};
         if (t[i] >= 0) {
@@ -344,13 +360,17 @@ __device__ __forceinline__ void write_fast_unit(const Kv8WriteArgs &a, const int
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         if constexpr (ROT) {
-            const int at = pos[i] < 0 ? 0 : (pos[i] >= a.max_positions ? a.max_positions - 1 : pos[i]);  // inside the tables
-            rotate_row<double>(w[i][0], w[i][1], static_cast<const __bf16 *>(a.k_weight),
-                               static_cast<const __bf16 *>(a.cos_cache) + (int64_t)at * kFastD,
-                               static_cast<const __bf16 *>(a.sin_cache) + (int64_t)at * kFastD, ch, a.eps, x[i]);
-            if (t[i] < 0)  // a row of zeros with eps 0 is NaN here
 #pragma unroll
-                for (int j = 0; j < 16; ++j) x[i][j] = 0.0f;
+            for (int j = 0; j < 16; ++j) x[i][j] = 0.0f;
+            if (__any(t[i] >= 0)) {  // a decode step writes one row of a block
+                const int at = pos[i] < 0 ? 0 : (pos[i] >= a.max_positions ? a.max_positions - 1 : pos[i]);  // inside the tables
+                rotate_row<double>(w[i][0], w[i][1], static_cast<const __bf16 *>(a.k_weight),
+                                   static_cast<const __bf16 *>(a.cos_cache) + (int64_t)at * kFastD,
+                                   static_cast<const __bf16 *>(a.sin_cache) + (int64_t)at * kFastD, ch, a.eps, x[i]);
+                if (t[i] < 0)  // a row of zeros with eps 0 is NaN here
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) x[i][j] = 0.0f;
+            }
             __builtin_amdgcn_sched_barrier(0);  // one row after the other: both at once take 170 registers
         } else {
             unpack8(w[i][0], x[i]);
@@ -359,14 +379,27 @@ __device__ __forceinline__ void write_fast_unit(const Kv8WriteArgs &a, const int
 #pragma unroll
         for (int j = 0; j < 16; ++j) amax = fmaxf(amax, finite_abs(x[i][j]));
     }
-    const float s = fmaxf(was, scale_of<F>(wave_max(amax)));
-    const float inv = inverse_scale(s);
+    if constexpr (FEW) {
+#pragma unroll
+        for (int m = 1; m < 8; m <<= 1) amax = fmaxf(amax, __shfl_xor(amax, m));
+    } else {
+        amax = wave_max(amax);
+    }
+    const float s = fmaxf(was, scale_of<F>(amax));
+    const float inv = inverse_scale(s), ratio = was * inv;
     const bool grows = !begins && s > was;
     unsigned char *base = static_cast<unsigned char *>(is_v ? a.v_cache : a.k_cache) +
                           ((int64_t)block * kFastBS * Hkv + head) * kFastD;
+    const auto rescale = [&](int row) {
+        u32x4 *out = reinterpret_cast<u32x4 *>(base + (int64_t)row * Hkv * kFastD + 16 * ch);
+        u32x4 y = *out;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[j] = rescale4<F>(y[j], ratio);
+        *out = y;
+    };
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-        u32x4 *out = reinterpret_cast<u32x4 *>(base + (int64_t)(r + 8 * i) * Hkv * kFastD + 16 * ch);
+        unsigned char *out = base + (int64_t)o[i] * Hkv * kFastD;
         unsigned c[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j)
@@ -377,28 +410,26 @@ __device__ __forceinline__ void write_fast_unit(const Kv8WriteArgs &a, const int
             const bool odd = ch & 1;
             const unsigned g0 = __shfl_xor((int)(odd ? c[0] : c[2]), 1), g1 = __shfl_xor((int)(odd ? c[1] : c[3]), 1);
             const u32x4 y = odd ? u32x4{g0, g1, c[2], c[3]} : u32x4{c[0], c[1], g0, g1};
-            out = reinterpret_cast<u32x4 *>(base + (int64_t)(r + 8 * i) * Hkv * kFastD +
-                                            (odd ? 64 + 8 * (ch - 1) : 8 * ch));
-            if (t[i] >= 0) *out = y;
+            if (t[i] >= 0) *reinterpret_cast<u32x4 *>(out + (odd ? 64 + 8 * (ch - 1) : 8 * ch)) = y;
         } else {
-            if (t[i] >= 0) *out = u32x4{c[0], c[1], c[2], c[3]};
+            if (t[i] >= 0) *reinterpret_cast<u32x4 *>(out + 16 * ch) = u32x4{c[0], c[1], c[2], c[3]};
         }
-        if (grows && t[i] < 0) {
-            u32x4 y = *out;
-            const float ratio = was * inv;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) y[j] = rescale4<F>(y[j], ratio);
-            *out = y;
-        }
+        if constexpr (!FEW)
+            if (grows && t[i] < 0) rescale(o[i]);
     }
-    if (lane == 0 && (begins || grows)) *sp = s;
+    if constexpr (FEW)
+        if (grows)
+            for (int row = 0; row < kFastBS; ++row)
+                if (row != o[0] && row != o[1]) rescale(row);
+    if ((FEW ? ch == 0 && valid : lane == 0) && (begins || grows)) *sp = s;
 }
 
 // Workgroups [0, chunk_blocks * parts): part `% parts` of chunk `/ parts`; behind them (producer) rows of Q, and of
-// K to k_out, 8 lanes a row, 32 rows a workgroup.
+// K to k_out, 8 lanes a row, 32 rows a workgroup.  Waves a SIMD: 8 for the plain write (8 x 4096 tokens 42.6 us, with 7
+// 44.8), 4 for the producer with its f64 rows (3: 4 x 2048 tokens 33.5 us against 31; 5 spill).
 template <Kv8Format F, bool PRODUCER>
-__global__ __launch_bounds__(kThreads, PRODUCER ? 4 : 1) void kv8_write_kernel(const Kv8WriteArgs a, int chunk, int parts,
-                                                             int chunk_blocks, bool indexed) {
+__global__ __launch_bounds__(kThreads, PRODUCER ? 4 : 8) void kv8_write_kernel(const Kv8WriteArgs a, int chunk,
+                                                                              int parts, int chunk_blocks, bool indexed) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int Hkv = a.num_kv_heads;
     if constexpr (PRODUCER) {
@@ -429,21 +460,35 @@ __global__ __launch_bounds__(kThreads, PRODUCER ? 4 : 1) void kv8_write_kernel(c
             return;
         }
     }
-    __shared__ int map[kMaxChunk * kFastBS], owner[kMaxChunk], block[kMaxChunk];
-    const Chunk ch{map, owner, block};
+    __shared__ int map[kMaxChunk * kFastBS], owner[kMaxChunk], block[kMaxChunk], rows[kMaxChunk + 1];
+    const Chunk ch{map, owner, block, rows};
     const int part = blockIdx.x % parts, t0 = (int)(blockIdx.x / parts) * chunk;
     const int count = find_blocks(ch, a.slot_mapping, (int)a.num_tokens, t0, chunk, kFastBS,
                                   a.num_cache_blocks * kFastBS, indexed ? a.workspace : nullptr);
-    for (int u = part * kWaves + wave; u < count * Hkv * 2; u += parts * kWaves) {
-        const int i = u / (2 * Hkv), head = u % Hkv;
-        const bool is_v = (u / Hkv) & 1;
-        const int c = __builtin_amdgcn_readfirstlane(owner[i]);
-        const int b = __builtin_amdgcn_readfirstlane(block[c]);
-        if (PRODUCER && !is_v)
-            write_fast_unit<F, true>(a, map + c * kFastBS, b, head, false);
-        else
-            write_fast_unit<F, false>(a, map + c * kFastBS, b, head, is_v);
-    }
+    const int first = part * kWaves + wave, stride = parts * kWaves, eights = (Hkv + 7) / 8;
+    const int fews = __builtin_amdgcn_readfirstlane(rows[kMaxChunk]);
+    if (fews > 0)
+        for (int u = first; u < count * eights * 2; u += stride) {
+            const int i = u / (2 * eights), c = __builtin_amdgcn_readfirstlane(owner[i]);
+            const int b = __builtin_amdgcn_readfirstlane(block[c]), few = __builtin_amdgcn_readfirstlane(rows[c]);
+            const bool is_v = (u / eights) & 1;
+            if (few < 0) continue;
+            if (PRODUCER && !is_v)
+                write_fast_unit<F, true, true>(a, map + c * kFastBS, few, b, 8 * (u % eights), false);
+            else
+                write_fast_unit<F, false, true>(a, map + c * kFastBS, few, b, 8 * (u % eights), is_v);
+        }
+    if (fews < count)
+        for (int u = first; u < count * Hkv * 2; u += stride) {
+            const int i = u / (2 * Hkv), c = __builtin_amdgcn_readfirstlane(owner[i]);
+            const int b = __builtin_amdgcn_readfirstlane(block[c]), few = __builtin_amdgcn_readfirstlane(rows[c]);
+            const bool is_v = (u / Hkv) & 1;
+            if (few >= 0) continue;
+            if (PRODUCER && !is_v)
+                write_fast_unit<F, true, false>(a, map + c * kFastBS, 0, b, u % Hkv, false);
+            else
+                write_fast_unit<F, false, false>(a, map + c * kFastBS, 0, b, u % Hkv, is_v);
+        }
 }
 
 template <Kv8Format F> hipError_t launch_fast(const Kv8WriteArgs &a, bool indexed, hipStream_t stream) {
@@ -451,9 +496,10 @@ template <Kv8Format F> hipError_t launch_fast(const Kv8WriteArgs &a, bool indexe
     int chunk = kMaxChunk;
     while (chunk > 1 && a.num_tokens < (int64_t)chunk * 256) chunk /= 2;
     const int64_t chunks = (a.num_tokens + chunk - 1) / chunk;
-    // workgroups per chunk: a unit a wave while the launch is small
+    // workgroups per chunk: a unit a wave while the launch is small; the producer's leave some of the chip's 1024 places
+    // to the rows of Q (4 x 2048 tokens: 31 us, 38 with up to 2048 of them)
     int parts = (2 * a.num_kv_heads + kWaves - 1) / kWaves;
-    while (parts > 1 && chunks * parts > 2048) --parts;
+    while (parts > 1 && chunks * parts > (a.q ? 768 : 2048)) --parts;
     const int64_t rows = a.q ? a.num_tokens * (a.num_heads + (a.k_out ? a.num_kv_heads : 0)) : 0;
     const int64_t blocks = chunks * parts + (rows + 31) / 32;
     if (blocks > 0x7fffffffLL) return hipErrorInvalidValue;

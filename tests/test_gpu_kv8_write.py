@@ -80,18 +80,33 @@ def test_decode_steps_grow_the_scale(dev, fmt, bs, D):
 
 
 @pytest.mark.parametrize("fmt", FMT)
-@pytest.mark.parametrize("n", [1, 2, 15, 16, 17, 300, 4096, 4097, 6001])
+@pytest.mark.parametrize("n", [1, 2, 15, 16, 17, 300, 1024, 1025, 4097, 6001])
 def test_any_order_skips_and_repeats(dev, fmt, n):
     """random slots: negative ones and ones past the pool are skipped, of repeats the last wins; both
-    ways of finding a block's tokens (4096 is the last that scans), the workspace full of rubbish"""
+    ways of finding a block's tokens (1024 is the last that scans), the workspace full of rubbish"""
     rng = np.random.default_rng(n)
     bs, H, D = 16, 2, 128
     nb = max(3, n // 12)
     slots = rng.integers(-20, nb * bs + 20, n).tolist()
     need = nv.capi.lib().nvllm_kv8_write_workspace_bytes(n, bs, nb)
-    assert (need > 0) == (n > 4096)
+    assert (need > 0) == (n > 1024)
     ws = torch.from_numpy(rng.integers(-5, n + 5, max(need // 4, 4)).astype(np.int32)).to(dev).view(torch.uint8)
     _write_both(rng, fmt, "bf16", nb, bs, H, D, slots, dev, workspace=ws)
+
+
+@pytest.mark.parametrize("fmt", FMT)
+@pytest.mark.parametrize("H", [1, 3, 8, 9, 20])
+@pytest.mark.parametrize("blocks", [3, 40, 700])
+def test_few_rows_of_a_block(dev, fmt, H, blocks):
+    """one, two, three or all rows of blocks that hold others, mixed in one call; some begin, some grow"""
+    rng = np.random.default_rng(H + blocks)
+    bs, D = 16, 128
+    slots = []
+    for b in rng.permutation(blocks + 2)[:blocks].tolist():
+        rows = rng.permutation(bs)[:rng.choice([1, 1, 2, 2, 3, 16])]
+        slots += [b * bs + int(r) for r in rows]
+    rng.shuffle(slots)
+    _write_both(rng, fmt, "bf16", blocks + 2, bs, H, D, slots, dev, sigma=4.0)
 
 
 @pytest.mark.parametrize("fmt", FMT)
@@ -206,15 +221,17 @@ def _producer(rng, fmt, dtype, n, Hq, H, D, bs, dev, slots, nb, k_out=True):
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 @pytest.mark.parametrize("n,Hq,H,D,bs", [(1, 16, 8, 128, 16), (37, 16, 8, 128, 16), (19, 4, 2, 64, 8), (9, 6, 3, 10, 4),
                                          (5, 2, 1, 256, 16), (4100, 2, 1, 128, 16)])
-def test_producer(dev, fmt, dtype, n, Hq, H, D, bs):
+@pytest.mark.parametrize("step", [1, 17])
+def test_producer(dev, fmt, dtype, n, Hq, H, D, bs, step):
     """q_out and k_out: f32 arithmetic of some ten operations (each off by 2^-24 of terms no larger than
     |a| + |b| of the pair), the sum of squares (relative D * 2^-24 at worst), one rounding.  Codes: V is
     exact.  K is computed in f64, its value known to some (D / 2 + 12) 2^-53 of its pair: a code may differ
     by one step where a border lies that near, its scale only where amax lies within 2^-24 of a border of
     its own, which none of these inputs does."""
     rng = np.random.default_rng(n * 7 + D)
-    nb = n // bs + 6
-    slots = (rng.permutation(nb)[np.arange(n) // bs] * bs + np.arange(n) % bs).tolist()
+    nb = n * step // bs + 6
+    at = np.arange(n) * step  # 1: in order; 17: a row of every block
+    slots = (rng.permutation(nb)[at // bs] * bs + at % bs).tolist()
     if n > 4:
         slots[2] = -1
     r = _producer(rng, fmt, dtype, n, Hq, H, D, bs, dev, slots, nb)

@@ -63,7 +63,7 @@ def test_write():
 
 def test_write_workspace():
     need = C.lib().nvllm_kv8_write_workspace_bytes
-    assert need(4096, 16, 100) == 0 and need(4097, 16, 100) == 6400 and need(0, 16, 100) == 0 and need(9999, 0, 5) == 0
+    assert need(1024, 16, 100) == 0 and need(1025, 16, 100) == 6400 and need(0, 16, 100) == 0 and need(9999, 0, 5) == 0
     assert need(4097, 16, 1 << 28) == 1 << 34
     assert write(n=4097, nb=100) == C.NVLLM_ERR_CONFIG and "needs 6400" in C.last_error()
     assert write(n=4097, nb=100, ws=FAKE, wsb=6399) == C.NVLLM_ERR_CONFIG
