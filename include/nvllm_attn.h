@@ -277,8 +277,8 @@ int nvllm_reshape_and_cache_kv8(const void *key, const void *value, void *k_cach
                                 nvllm_stream_t stream);
 
 /* nvllm_qk_norm_rope_cache_* with quantisation: the rotated K and V go into the 8-bit cache, K computed in
- * f64 and rounded once (not by way of k_out); q_out and k_out in f32.  q_out may be q; k_out (optional)
- * must not overlap k. */
+ * f64 and rounded once (not by way of k_out); q_out and k_out in f32.  q_out may be q; neither it
+ * nor k_out (optional) may overlap k or v. */
 int nvllm_qk_norm_rope_cache_kv8(const void *q, const void *k, const void *v, void *q_out,
                                  void *k_out, const void *q_weight, const void *k_weight, float eps,
                                  const void *cos_cache, const void *sin_cache,

@@ -28,9 +28,9 @@ hipStream_t as_stream(nvllm_stream_t s) { return reinterpret_cast<hipStream_t>(s
 
 bool aligned(const void *p, unsigned n) { return (reinterpret_cast<std::uintptr_t>(p) & (n - 1)) == 0; }
 
-bool overlap(const void *a, const void *b, std::int64_t bytes) {
+bool overlap(const void *a, std::int64_t a_bytes, const void *b, std::int64_t b_bytes) {
     const auto x = reinterpret_cast<std::uintptr_t>(a), y = reinterpret_cast<std::uintptr_t>(b);
-    return x < y + (std::uintptr_t)bytes && y < x + (std::uintptr_t)bytes;
+    return x < y + (std::uintptr_t)b_bytes && y < x + (std::uintptr_t)a_bytes;
 }
 
 // what every entry on the cache checks: its geometry, the formats, the scales' alignment
@@ -43,6 +43,8 @@ int check_cache(const char *who, std::int64_t num_cache_blocks, int block_size, 
     if (head_dim > 256) return fail(ErrorKind::Unsupported, who, "head_dim > 256");
     if (num_cache_blocks > 0x7fffffff) return fail(ErrorKind::Unsupported, who, "more than 2^31 - 1 blocks");
     if (block_size > kernels::kKv8MaxBlockSize) return fail(ErrorKind::Unsupported, who, "block_size > 256");
+    if ((int64_t)block_size * num_kv_heads * head_dim > 0x7fffffffLL)
+        return fail(ErrorKind::Unsupported, who, "block of more than 2^31 - 1 values");
     return NVLLM_OK;
 }
 
@@ -50,7 +52,6 @@ int write_common(const char *who, const kernels::Kv8WriteArgs &a, size_t workspa
                  nvllm_stream_t stream) {
     if (!a.key || !a.value || !a.k_cache || !a.v_cache || !a.k_scales || !a.v_scales || !a.slot_mapping)
         return fail(ErrorKind::Null, who, "null pointer");
-    if (a.num_tokens > 0x7fffffff) return fail(ErrorKind::Unsupported, who, "more than 2^31 - 1 tokens");
     const unsigned elt = dtype == 0 ? 2 : 4;
     if (!aligned(a.key, elt) || !aligned(a.value, elt) || !aligned(a.k_scales, 4) || !aligned(a.v_scales, 4) ||
         !aligned(a.slot_mapping, 8))
@@ -87,6 +88,7 @@ int nvllm_reshape_and_cache_kv8(const void *key, const void *value, void *k_cach
     static const char *who = "reshape_and_cache_kv8";
     if (num_tokens < 0) return fail(ErrorKind::Config, who, "negative or zero dimension");
     if (const int rc = check_cache(who, num_cache_blocks, block_size, num_kv_heads, head_dim, format, dtype)) return rc;
+    if (num_tokens > (1 << 30)) return fail(ErrorKind::Unsupported, who, "more than 2^30 tokens");
     if (num_tokens == 0) return NVLLM_OK;
     kernels::Kv8WriteArgs a{};
     a.key = key;
@@ -118,6 +120,7 @@ int nvllm_qk_norm_rope_cache_kv8(const void *q, const void *k, const void *v, vo
     if (const int rc = check_cache(who, num_cache_blocks, block_size, num_kv_heads, head_dim, format, dtype)) return rc;
     if (head_dim % 2 != 0)  // rope.rs:49 assert!(dim.is_multiple_of(2))
         return fail(ErrorKind::Config, who, "RoPE dimension must be even");
+    if (num_tokens > (1 << 30)) return fail(ErrorKind::Unsupported, who, "more than 2^30 tokens");
     if (num_tokens == 0) return NVLLM_OK;
     if (!q || !q_out || !q_weight || !k_weight || !cos_cache || !sin_cache || !positions)
         return fail(ErrorKind::Null, who, "null pointer");
@@ -125,8 +128,14 @@ int nvllm_qk_norm_rope_cache_kv8(const void *q, const void *k, const void *v, vo
     for (const void *p : {q, (const void *)q_out, (const void *)k_out, q_weight, k_weight, cos_cache, sin_cache})
         if (!aligned(p, elt)) return fail(ErrorKind::Config, who, "pointer not aligned to its element type");
     if (!aligned(positions, 4)) return fail(ErrorKind::Config, who, "pointer not aligned to its element type");
-    if (k && k_out && overlap(k, k_out, num_tokens * num_kv_heads * head_dim * elt))
-        return fail(ErrorKind::Config, who, "k_out must not overlap k: a block's rows are read by other waves");
+    // other waves read the rows of k and v while these are written
+    const int64_t kv_bytes = num_tokens * num_kv_heads * head_dim * elt, q_bytes = num_tokens * num_heads * head_dim * elt;
+    for (const void *p : {k, v}) {
+        if (p && k_out && overlap(k_out, kv_bytes, p, kv_bytes))
+            return fail(ErrorKind::Config, who, "k_out must not overlap k or v");
+        if (p && overlap(q_out, q_bytes, p, kv_bytes))
+            return fail(ErrorKind::Config, who, "q_out must not overlap k or v");
+    }
     kernels::Kv8WriteArgs a{};
     a.key = k;
     a.value = v;
@@ -169,8 +178,6 @@ int nvllm_gather_cache_blocks_kv8(const void *k_cache, const void *v_cache, cons
     if (!aligned(k_out, elt) || !aligned(v_out, elt) || !aligned(k_scales, 4) || !aligned(v_scales, 4) ||
         !aligned(block_ids, 4))
         return fail(ErrorKind::Config, who, "pointer not aligned to its element type");
-    if ((int64_t)block_size * num_kv_heads * head_dim > 0x7fffffffLL)
-        return fail(ErrorKind::Unsupported, who, "block of more than 2^31 - 1 values");
     return hip_status(kernels::launch_kv8_gather(static_cast<kernels::DType>(dtype),
                                                  static_cast<kernels::Kv8Format>(format), k_cache, v_cache, k_scales,
                                                  v_scales, block_ids, num_ids, k_out, v_out, num_cache_blocks,
@@ -192,7 +199,7 @@ static kernels::PagedAttnArgs attn_shape(int num_seqs, int num_new_tokens, int n
 }
 
 static int check_attn(const char *who, int num_seqs, int num_new_tokens, int num_heads, int num_kv_heads,
-                      int max_blocks_per_seq) {
+                      int block_size, int max_blocks_per_seq) {
     if (num_seqs < 0 || num_new_tokens <= 0 || num_heads <= 0)
         return fail(ErrorKind::Config, who, "negative or zero dimension");
     if (max_blocks_per_seq <= 0)  // paged.rs:133-137
@@ -200,6 +207,9 @@ static int check_attn(const char *who, int num_seqs, int num_new_tokens, int num
     if (num_heads % num_kv_heads != 0)
         return fail(ErrorKind::Config, who, "num_heads must be a multiple of num_kv_heads");
     if (num_seqs > 65535) return fail(ErrorKind::Unsupported, who, "num_seqs > 65535 per launch");
+    if (num_kv_heads > 65535) return fail(ErrorKind::Unsupported, who, "num_kv_heads > 65535");
+    if ((int64_t)max_blocks_per_seq * block_size > (1 << 30))
+        return fail(ErrorKind::Unsupported, who, "block tables of more than 2^30 tokens");
     if ((int64_t)num_heads * num_new_tokens > 0x7fffffffLL)
         return fail(ErrorKind::Unsupported, who, "more than 2^31 - 1 query rows per sequence");
     return NVLLM_OK;
@@ -219,7 +229,9 @@ int nvllm_paged_attn_kv8_path(int num_seqs, int num_new_tokens, int num_heads, i
                               int block_size, int max_blocks_per_seq, int dtype) {
     static const char *who = "paged_attn_kv8_path";
     if (const int rc = check_cache(who, 1, block_size, num_kv_heads, head_dim, 0, dtype)) return rc;
-    if (const int rc = check_attn(who, num_seqs, num_new_tokens, num_heads, num_kv_heads, max_blocks_per_seq)) return rc;
+    if (const int rc = check_attn(who, num_seqs, num_new_tokens, num_heads, num_kv_heads, block_size,
+                                  max_blocks_per_seq))
+        return rc;
     return (int)kernels::paged_attn_kv8_path(
         static_cast<kernels::DType>(dtype),
         attn_shape(num_seqs, num_new_tokens, num_heads, num_kv_heads, head_dim, block_size, max_blocks_per_seq));
@@ -232,7 +244,9 @@ int nvllm_paged_attn_kv8(const void *q, const void *k_cache, const void *v_cache
                          int64_t num_cache_blocks, float scale, int format, int dtype, nvllm_stream_t stream) {
     static const char *who = "paged_attn_kv8";
     if (const int rc = check_cache(who, num_cache_blocks, block_size, num_kv_heads, head_dim, format, dtype)) return rc;
-    if (const int rc = check_attn(who, num_seqs, num_new_tokens, num_heads, num_kv_heads, max_blocks_per_seq)) return rc;
+    if (const int rc = check_attn(who, num_seqs, num_new_tokens, num_heads, num_kv_heads, block_size,
+                                  max_blocks_per_seq))
+        return rc;
     if (num_seqs == 0) return NVLLM_OK;
     if (!q || !k_cache || !v_cache || !k_scales || !v_scales || !block_tables || !context_lens || !out)
         return fail(ErrorKind::Null, who, "null pointer");

@@ -23,85 +23,124 @@ using namespace kv8;
 
 // ---------------------------------------------------------------------------
 // Generic path: any head_dim <= 256, any block size, bf16 or f32.  One workgroup per (sequence, new
-// token, query head); its four waves take every fourth tile of 64 keys and join at the end.  f32 FMA.
-// A lane is a key for q.k and four dims for p.v.
+// token, query head); its W waves take every W-th tile of 64 keys and join at the end.  f32 FMA.
+// A lane is a key for q.k and four dims for p.v.  `vec`: bytes of K a load takes (16, 4, 1; V at most 4).
+// Bound by latency, and by the arithmetic where there is work for the whole chip (K and V are read and converted
+// once per query head): the table's entry is read a tile ahead and eight rows of V are on their way during q.k
+// (64 x 1024, head_dim 128, f32: 98 -> 61 us).
 // ---------------------------------------------------------------------------
-template <typename ET, Kv8Format F>
-__global__ __launch_bounds__(256) void paged_attn_kv8_generic_kernel(
+// block id as the kernels use it: inside the pool
+__device__ __forceinline__ int pool_id(int id, int64_t num_cache_blocks) {
+    const int most = (int)num_cache_blocks - 1;  // the C entries refuse larger pools
+    return id < 0 ? 0 : (id > most ? most : id);
+}
+
+constexpr int kAtOnce = 8;  // rows of V that a group of lanes has on their way
+
+// what lanes of the wave wrote to LDS before, lanes of it may read after
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+template <typename ET, Kv8Format F, int W>
+__global__ __launch_bounds__(64 * W) void paged_attn_kv8_generic_kernel(
     const ET *__restrict__ q, const unsigned char *__restrict__ k_cache, const unsigned char *__restrict__ v_cache,
     const float *__restrict__ k_scales, const float *__restrict__ v_scales, const int32_t *__restrict__ block_tables,
     const int32_t *__restrict__ context_lens, ET *__restrict__ out, int T, int Hq, int Hkv, int D, int block_size,
-    int max_blocks_per_seq, int64_t num_cache_blocks, float scale, bool wide) {
+    int max_blocks_per_seq, int64_t num_cache_blocks, float scale, int vec) {
     __shared__ float q_s[256];
-    __shared__ float p_s[4][64];
-    __shared__ int64_t row_s[4][64];  // element offset of each key's row
-    __shared__ float o_s[4][256];
-    __shared__ float m_s[4], l_s[4];
+    __shared__ float p_s[W][64];
+    __shared__ int64_t row_s[W][64];  // element offset of each key's row
+    __shared__ float o_s[W][256];
+    __shared__ float m_s[W], l_s[W];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int h = (int)(blockIdx.x % (unsigned)Hq), t = (int)(blockIdx.x / (unsigned)Hq), seq = blockIdx.y;
     const int kvh = h / (Hq / Hkv);
-    int64_t ctx = context_lens[seq];
+    int ctx = context_lens[seq];
     const int64_t cap = (int64_t)max_blocks_per_seq * block_size;
-    if (ctx > cap) ctx = cap;  // never read past the table row
-    const int64_t keys = ctx - T + t + 1;  // keys this query sees: 0 .. keys - 1 (none if <= 0)
+    if (ctx > cap) ctx = (int)cap;  // never read past the table row
+    if (ctx < 0) ctx = 0;
+    const int keys = ctx - T + t + 1;  // keys this query sees: 0 .. keys - 1 (none if <= 0)
     const int64_t orow = (((int64_t)seq * T + t) * Hq + h) * D;
-    for (int d = threadIdx.x; d < 256; d += 256) {
-        q_s[d] = d < D ? to_f32(q[orow + d]) : 0.0f;
-        for (int w = 0; w < 4; ++w) o_s[w][d] = 0.0f;
-    }
+    const bool wide = vec >= 4;
+    if (threadIdx.x < 256) q_s[threadIdx.x] = (int)threadIdx.x < D ? to_f32(q[orow + threadIdx.x]) : 0.0f;
+    for (int d = lane; d < 256; d += 64) o_s[wave][d] = 0.0f;
     __syncthreads();
     const int32_t *table = block_tables + (int64_t)seq * max_blocks_per_seq;
     const int lanes = wide ? D / 4 : 64, together = wide ? 64 / lanes : 1;  // lanes per V row, rows at once
     const int vr = wide ? lane / lanes : 0, vc = wide ? lane % lanes : lane;
     float m = -INFINITY, l = 0.0f, o[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int64_t base = 64 * wave; base < keys; base += 256) {
-        const int64_t key = base + lane;
-        float s = -INFINITY, vs = 0.0f;
-        if (key < keys) {
-            const int64_t lb = key / block_size;
-            int64_t pb = table[lb];
-            pb = pb < 0 ? 0 : (pb >= num_cache_blocks ? num_cache_blocks - 1 : pb);
-            const int64_t row = ((pb * block_size + (key - lb * block_size)) * Hkv + kvh) * D;
-            row_s[wave][lane] = row;
-            float acc = 0.0f;
-            if (wide) {
-                for (int d = 0; d < D; d += 4) {
-                    float x[4];
-                    decode4<F>(*reinterpret_cast<const unsigned *>(k_cache + row + d), x);
+    int base = 64 * wave;
+    int64_t pb = base + lane < keys ? pool_id(table[(base + lane) / block_size], num_cache_blocks) : 0;
+    for (; base < keys; base += 64 * W) {
+        const int key = base + lane, n = keys - base < 64 ? keys - base : 64;
+        // a lane without a key takes the tile's first (its weight is 0)
+        const int64_t at = ((pb * block_size + key % block_size) * Hkv + kvh) * D;
+        const int64_t first = __shfl(at, 0), row = key < keys ? at : first;
+        row_s[wave][lane] = row;
+        const float ks = key < keys ? k_scales[pb * Hkv + kvh] : 0.0f, vs = key < keys ? v_scales[pb * Hkv + kvh] : 0.0f;
+        const int next = key + 64 * W;
+        pb = next < keys ? pool_id(table[next / block_size], num_cache_blocks) : 0;
+        wave_sync();
+        unsigned v[kAtOnce];  // on their way during q.k and the softmax
+        const auto load_v = [&](int j0) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) acc += q_s[d + i] * x[i];
-                }
-            } else {
-                for (int d = 0; d < D; ++d) acc += q_s[d] * decode1<F>(k_cache[row + d]);
+            for (int j = 0; j < kAtOnce; ++j) {
+                const int r = j0 + j * together + vr;
+                v[j] = *reinterpret_cast<const unsigned *>(v_cache + row_s[wave][r < 64 ? r : 0] + 4 * vc);
             }
-            s = acc * (scale * k_scales[pb * Hkv + kvh]);
-            vs = v_scales[pb * Hkv + kvh];
+        };
+        if (wide) load_v(0);
+        float acc = 0.0f;
+        if (vec == 16) {
+#pragma unroll 4
+            for (int d = 0; d < D; d += 16) {
+                const u32x4 w = *reinterpret_cast<const u32x4 *>(k_cache + row + d);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float x[4];
+                    decode4<F>(w[e], x);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) acc += q_s[d + 4 * e + i] * x[i];
+                }
+            }
+        } else if (wide) {
+            for (int d = 0; d < D; d += 4) {
+                float x[4];
+                decode4<F>(*reinterpret_cast<const unsigned *>(k_cache + row + d), x);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc += q_s[d + i] * x[i];
+            }
+        } else {
+            for (int d = 0; d < D; ++d) acc += q_s[d] * decode1<F>(k_cache[row + d]);
         }
+        const float s = key < keys ? acc * (scale * ks) : -INFINITY;
         const float m_new = fmaxf(m, wave_max(s));
         const float m_safe = m_new == -INFINITY ? 0.0f : m_new;  // keys that all score -inf weigh nothing
         const float alpha = expf(m - m_safe);
         const float p = key < keys ? expf(s - m_safe) : 0.0f;
-        float ps = p;
-#pragma unroll
-        for (int x = 32; x > 0; x >>= 1) ps += __shfl_xor(ps, x);
-        l = l * alpha + ps;
+        l = l * alpha + p;  // the lane's own keys; joined at the end
         m = m_new;
         p_s[wave][lane] = p * vs;
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        wave_sync();
 #pragma unroll
         for (int i = 0; i < 4; ++i) o[i] *= alpha;
-        const int n = (int)(keys - base < 64 ? keys - base : 64);
         if (wide) {
-            if (vr < together)
-                for (int j = vr; j < n; j += together) {
+            for (int j0 = 0; j0 < n; j0 += kAtOnce * together) {
+                if (j0 > 0) load_v(j0);
+#pragma unroll
+                for (int j = 0; j < kAtOnce; ++j) {
+                    const int r = j0 + j * together + vr;
+                    if (vr >= together || r >= n) continue;
                     float x[4];
-                    decode4<F>(*reinterpret_cast<const unsigned *>(v_cache + row_s[wave][j] + 4 * vc), x);
-                    const float pw = p_s[wave][j];
+                    decode4<F>(v[j], x);
+                    const float pw = p_s[wave][r];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) o[i] += pw * x[i];
                 }
+            }
         } else {
             for (int j = 0; j < n; ++j) {
                 const float pw = p_s[wave][j];
@@ -110,8 +149,10 @@ __global__ __launch_bounds__(256) void paged_attn_kv8_generic_kernel(
                     if (vc + 64 * i < D) o[i] += pw * decode1<F>(v_cache[row_s[wave][j] + vc + 64 * i]);
             }
         }
-        __builtin_amdgcn_wave_barrier();
+        wave_sync();
     }
+#pragma unroll
+    for (int x = 32; x > 0; x >>= 1) l += __shfl_xor(l, x);
     // join: the lanes of a wave that hold the same dims, then the waves
     if (lane == 0) {
         m_s[wave] = m;
@@ -124,31 +165,48 @@ __global__ __launch_bounds__(256) void paged_attn_kv8_generic_kernel(
                 const int d = wide ? 4 * vc + i : vc + 64 * i;
                 if (d < D) o_s[wave][d] += o[i];
             }
-        __syncthreads();
+        wave_sync();
     }
-    const float mx = fmaxf(fmaxf(m_s[0], m_s[1]), fmaxf(m_s[2], m_s[3]));
-    float L = 0.0f, y = 0.0f;
+    __syncthreads();
     const int d = threadIdx.x;
+    if (d >= D) return;
+    float mx = m_s[0], L = 0.0f, y = 0.0f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
+    for (int w = 1; w < W; ++w) mx = fmaxf(mx, m_s[w]);
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
         const float f = m_s[w] == -INFINITY ? 0.0f : expf(m_s[w] - mx);
         L += f * l_s[w];
         y += f * o_s[w][d];
     }
-    if (d < D) out[orow + d] = static_cast<ET>(L == 0.0f ? 0.0f : y / L);  // no key seen: zeros
+    out[orow + d] = static_cast<ET>(L == 0.0f ? 0.0f : y / L);  // no key seen: zeros
+}
+
+// Sixteen waves where a workgroup has a CU to itself and long tables (int8, f32, head_dim 64, 8 heads, us with 4 and 16
+// waves: 9 x 777 T = 3 14.9 and 10.1, 1 x 4000 47 and 22, 1 x 500 9.7 and 8.5, 1 x 250 6.9 and 7.7; 64 x 1024 with 16
+// heads 49 and 59).
+int generic_waves(const PagedAttnArgs &a) {
+    const int64_t groups = (int64_t)a.num_seqs * a.num_new_tokens * a.num_heads;
+    return groups <= device_cus() && (int64_t)a.max_blocks_per_seq * a.block_size > 512 ? 16 : 4;
 }
 
 template <typename ET, Kv8Format F>
 hipError_t launch_generic(const PagedAttnArgs &a, const float *ks, const float *vs, hipStream_t stream) {
     const int64_t rows = (int64_t)a.num_heads * a.num_new_tokens;
     if (rows > 0x7fffffffLL) return hipErrorInvalidValue;
-    const auto at4 = [](const void *p) { return (reinterpret_cast<uintptr_t>(p) & 3) == 0; };
-    const bool wide = a.head_dim % 4 == 0 && at4(a.k_cache) && at4(a.v_cache);
-    paged_attn_kv8_generic_kernel<ET, F><<<dim3((unsigned)rows, a.num_seqs), dim3(256), 0, stream>>>(
-        static_cast<const ET *>(a.q), static_cast<const unsigned char *>(a.k_cache),
-        static_cast<const unsigned char *>(a.v_cache), ks, vs, a.block_tables, a.context_lens,
-        static_cast<ET *>(a.out), a.num_new_tokens, a.num_heads, a.num_kv_heads, a.head_dim, a.block_size,
-        a.max_blocks_per_seq, a.num_cache_blocks, a.scale, wide);
+    const auto aligned = [&](unsigned n) {
+        return a.head_dim % n == 0 && ((reinterpret_cast<uintptr_t>(a.k_cache) | reinterpret_cast<uintptr_t>(a.v_cache)) & (n - 1)) == 0;
+    };
+    const int vec = aligned(16) ? 16 : aligned(4) ? 4 : 1;
+#define NVLLM_KV8_GENERIC(W)                                                                                        \
+    paged_attn_kv8_generic_kernel<ET, F, W><<<dim3((unsigned)rows, a.num_seqs), dim3(64 * W), 0, stream>>>(         \
+        static_cast<const ET *>(a.q), static_cast<const unsigned char *>(a.k_cache),                                \
+        static_cast<const unsigned char *>(a.v_cache), ks, vs, a.block_tables, a.context_lens,                      \
+        static_cast<ET *>(a.out), a.num_new_tokens, a.num_heads, a.num_kv_heads, a.head_dim, a.block_size,          \
+        a.max_blocks_per_seq, a.num_cache_blocks, a.scale, vec)
+    if (generic_waves(a) == 16) NVLLM_KV8_GENERIC(16);
+    else NVLLM_KV8_GENERIC(4);
+#undef NVLLM_KV8_GENERIC
     return hipGetLastError();
 }
 
@@ -217,12 +275,6 @@ __device__ __forceinline__ float quad_max(float x) {
 // Exponents are taken from a reference that moves only when a row's maximum has passed it by kSlack: p stays
 // below 2^8 (its rounding to bf16 is relative, the sums are f32), and most tiles rescale nothing.
 constexpr float kSlack = 8.0f;
-
-// block id as the kernels use it: inside the pool
-__device__ __forceinline__ int pool_id(int id, int64_t num_cache_blocks) {
-    const int most = (int)num_cache_blocks - 1;  // the C entries refuse larger pools
-    return id < 0 ? 0 : (id > most ? most : id);
-}
 
 // A kv head's rows of a cache block as a buffer: 16 bytes of it at lane_offset + row_offset, zeros without a
 // memory access if `valid` is false.  Tiles past the end are "loaded" that way, so that every step of a loop
@@ -336,6 +388,7 @@ __global__ __launch_bounds__(64 * W, NQT == 1 ? 2 : 1) void paged_attn_kv8_decod
     int ctx = context_lens[seq];
     const int64_t cap = (int64_t)max_blocks_per_seq * kBS;
     if (ctx > cap) ctx = (int)cap;  // never read past the table row
+    if (ctx < 0) ctx = 0;
     const int nblk_seq = ctx > 0 ? (int)(((int64_t)ctx + kBS - 1) / kBS) : 0;
     int blk_begin = split * blocks_per_split;
     int blk_end = blk_begin + blocks_per_split;
@@ -680,6 +733,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kv8_tile_kernel(
     int ctx = context_lens[seq];
     const int64_t cap = (int64_t)max_blocks_per_seq * kBS;
     if (ctx > cap) ctx = (int)cap;  // never read past the table row
+    if (ctx < 0) ctx = 0;
     const int row_last = row0 + kRows < R ? row0 + kRows - 1 : R - 1;
     // keys that some row of the tile sees: [0, keys); all its rows see [0, keys_all)
     const int64_t seen = (int64_t)ctx - T + row_last / G + 1;
@@ -1036,7 +1090,7 @@ hipError_t launch_tile(const PagedAttnArgs &a, const float *ks, const float *vs,
     float *ws_o, *ws_ml;
     if (!partials(a, splits, &ws_o, &ws_ml)) return hipErrorInvalidValue;
     const int64_t tiles = (query_rows(a) + rows - 1) / rows;
-    if (tiles > 65535) return hipErrorInvalidValue;
+    if (tiles > 65535 || (int64_t)a.num_seqs * a.num_kv_heads > 0x7fffffffLL) return hipErrorInvalidValue;
     paged_attn_kv8_tile_kernel<F, KG, STREAM>
         <<<dim3((unsigned)(a.num_seqs * a.num_kv_heads), (unsigned)tiles, splits), dim3(256), 0, stream>>>(
             static_cast<const __bf16 *>(a.q), static_cast<const unsigned char *>(a.k_cache),

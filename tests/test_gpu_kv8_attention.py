@@ -120,7 +120,7 @@ def test_rows_that_see_no_key_are_zero(dev, fmt, dtype, D, bs, T):
     rng = np.random.default_rng(T)
     lens = [0, 1, max(1, T - 1), T, 40]
     on, host = make(rng, fmt, dtype, lens, T, 4, 2, D, bs, dev)
-    on["lens"][0] = -3
+    on["lens"][0] = -2 ** 31 if T % 2 else -3
     got = call(on, 0.1)
     compare(got, host, 0.1, dtype)
     g = got.view(len(lens), T, -1)

@@ -8,6 +8,7 @@ import nano_vllm_rs_amd as nv
 
 C = nv.capi
 FAKE, ODD = ctypes.c_void_p(0x10000), ctypes.c_void_p(0x10001)
+KEY, VALUE = ctypes.c_void_p(0x80000), ctypes.c_void_p(0xa0000)
 
 
 def write(**kw):
@@ -18,7 +19,7 @@ def write(**kw):
 
 
 def producer(**kw):
-    a = dict(q=FAKE, k=FAKE, v=FAKE, q_out=FAKE, k_out=None, qw=FAKE, kw=FAKE, eps=1e-6, cos=FAKE, sin=FAKE, maxp=64, pos=FAKE, kc=FAKE,
+    a = dict(q=FAKE, k=KEY, v=VALUE, q_out=FAKE, k_out=None, qw=FAKE, kw=FAKE, eps=1e-6, cos=FAKE, sin=FAKE, maxp=64, pos=FAKE, kc=FAKE,
              vc=FAKE, ks=FAKE, vs=FAKE, slots=FAKE, ws=None, wsb=0, n=4, Hq=16, H=8, D=128, bs=16, nb=4, fmt=0, dt=0)
     a.update(kw)
     return C.lib().nvllm_qk_norm_rope_cache_kv8(*a.values(), None)
@@ -44,7 +45,8 @@ GEOMETRY = [("H", 0), ("H", -1), ("D", 0), ("bs", 0), ("nb", 0)]
 def test_geometry_formats_and_alignment(f):
     for name, x in GEOMETRY:
         assert f(**{name: x}) == C.NVLLM_ERR_CONFIG, name
-    for name, x in (("fmt", 2), ("fmt", -1), ("dt", 2), ("D", 257), ("D", 258), ("bs", 257)):
+    for name, x in (("fmt", 2), ("fmt", -1), ("dt", 2), ("D", 257), ("D", 258), ("bs", 257),
+                    ("H", 1 << 24)):
         assert f(**{name: x}) == C.NVLLM_ERR_UNSUPPORTED, (name, x)
     assert f(ks=ODD) == C.NVLLM_ERR_CONFIG and "aligned" in C.last_error()
     for name in ("kc", "ks"):
@@ -54,7 +56,9 @@ def test_geometry_formats_and_alignment(f):
 def test_write():
     assert write(n=0, key=None) == C.NVLLM_OK
     assert write(n=-1) == C.NVLLM_ERR_CONFIG
-    assert write(n=1 << 31) == C.NVLLM_ERR_UNSUPPORTED
+    for n in (1 << 62, (1 << 30) + 1):
+        for f in (write, producer):
+            assert f(n=n, wsb=1 << 40, ws=FAKE) == C.NVLLM_ERR_UNSUPPORTED
     for name in ("key", "value", "vc", "vs", "slots"):
         assert write(**{name: None}) == C.NVLLM_ERR_NULL
     assert write(key=ODD) == C.NVLLM_ERR_CONFIG and write(dt=1, value=ctypes.c_void_p(0x10002)) == C.NVLLM_ERR_CONFIG
@@ -77,9 +81,13 @@ def test_producer():
         assert producer(**{name: x}) == C.NVLLM_ERR_CONFIG, name
     for name in ("q", "k", "v", "q_out", "qw", "kw", "cos", "sin", "pos", "vc", "vs", "slots"):
         assert producer(**{name: None}) == C.NVLLM_ERR_NULL, name
-    far = ctypes.c_void_p(0x10000 + 4 * 8 * 128 * 2 - 2)
-    for bad in (FAKE, far):  # k_out on k, and on its last element
-        assert producer(k_out=bad) == C.NVLLM_ERR_CONFIG and "overlap" in C.last_error()
+    last = 4 * 8 * 128 * 2 - 2  # offset of the last element of k, v
+    for at in (KEY, VALUE):
+        for name in ("k_out", "q_out"):
+            for off in (0, last):
+                assert producer(**{name: ctypes.c_void_p(at.value + off)}) == C.NVLLM_ERR_CONFIG and "overlap" in C.last_error()
+        assert producer(q_out=ctypes.c_void_p(at.value - 4 * 16 * 128 * 2 + 2)) == C.NVLLM_ERR_CONFIG
+        assert "overlap" in C.last_error()
     assert producer(pos=ODD) == C.NVLLM_ERR_CONFIG and producer(cos=ODD) == C.NVLLM_ERR_CONFIG
 
 
@@ -87,15 +95,15 @@ def test_gather():
     assert gather(n=0) == C.NVLLM_ERR_CONFIG and "empty" in C.last_error()
     for name in ("ids", "ko", "vc", "vs"):
         assert gather(**{name: None}) == C.NVLLM_ERR_NULL
-    assert gather(H=1 << 24) == C.NVLLM_ERR_UNSUPPORTED
 
 
 def test_attend():
     assert attend(N=0) == C.NVLLM_OK
     for name, x in (("N", -1), ("T", 0), ("Hq", 0), ("Hq", 17), ("mb", 0)):
         assert attend(**{name: x}) == C.NVLLM_ERR_CONFIG, name
-    for name, x in (("N", 65536), ("T", 1 << 30)):
+    for name, x in (("N", 65536), ("T", 1 << 30), ("mb", (1 << 26) + 1)):
         assert attend(**{name: x}) == C.NVLLM_ERR_UNSUPPORTED, name
+    assert attend(Hq=1 << 17, H=1 << 17, D=8) == C.NVLLM_ERR_UNSUPPORTED
     for name in ("q", "vc", "vs", "bt", "cl", "out"):
         assert attend(**{name: None}) == C.NVLLM_ERR_NULL
     assert attend(q=ODD) == C.NVLLM_ERR_CONFIG and attend(dt=1, out=ctypes.c_void_p(0x10002)) == C.NVLLM_ERR_CONFIG
