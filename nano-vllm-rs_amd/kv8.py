@@ -19,37 +19,28 @@ def _refuse(message, code=capi.NVLLM_ERR_CONFIG):
     raise ConfigError(code, message)
 
 
-# the current stream's handle (the public way makes a Stream object each time, 2 us of a call's 10)
+# the current stream's handle and device (the public ways make a Stream object and look for an initialised
+# runtime each time, 2 us of a call's 10)
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 def _launch(tensors):
     """Checks what every tensor of a call has to be; -> the device index."""
     at = tensors[0].get_device()
     for t in tensors:
-        if t is None:
-            continue
-        if t.get_device() != at or at < 0:
-            if not t.is_cuda or at < 0:
-                raise RuntimeError("nano_vllm_rs_amd operators need HIP device tensors (no CPU fallback exists)")
+        if t is not None and (t.get_device() != at or not t.is_contiguous()):
+            break
+    else:
+        if at >= 0:
+            return at
+    for t in tensors:
+        if t is not None and not t.is_cuda:
+            raise RuntimeError("nano_vllm_rs_amd operators need HIP device tensors (no CPU fallback exists)")
+        if t is not None and t.get_device() != at:
             _refuse("tensors are on different devices: %d and %d" % (at, t.get_device()))
-        if not t.is_contiguous():
-            _refuse("tensor must be contiguous")
-    return at
-
-
-def _on_device(function):
-    """Launches happen with the tensors' device current: `function(index, ...)` is called under a guard if it
-    is not."""
-
-    def call(index, *args):
-        if index == torch.cuda.current_device():
-            return function(index, *args)
-        with torch.cuda.device(index):
-            return function(index, *args)
-
-    return call
+    _refuse("tensor must be contiguous")
 
 
 def _cache(key_cache, value_cache, key_scales, value_scales):
@@ -61,9 +52,9 @@ def _cache(key_cache, value_cache, key_scales, value_scales):
     if len(shape) != 4 or value_cache.shape != shape or value_cache.dtype != key_cache.dtype:
         _refuse("key and value cache must be [num_blocks, block_size, Hkv, D] of one dtype")
     nb, bs, hkv, d = shape
-    for s in (key_scales, value_scales):
-        if s.dtype != torch.float32 or s.shape != (nb, hkv):
-            _refuse("scales must be float32 [num_blocks, Hkv]")
+    if (key_scales.dtype != torch.float32 or value_scales.dtype != torch.float32 or
+            key_scales.shape != (nb, hkv) or value_scales.shape != (nb, hkv)):
+        _refuse("scales must be float32 [num_blocks, Hkv]")
     return nb, bs, hkv, d, fmt
 
 
@@ -78,12 +69,13 @@ def _dtype(t, *same):
     return code
 
 
-def _write_workspace(workspace, n, bs, nb, device):
+def _write_workspace(workspace, n, bs, nb, like):
     if workspace is None:
         need = capi.lib().nvllm_kv8_write_workspace_bytes(n, bs, nb)
-        if need:
-            workspace = torch.empty(need, dtype=torch.uint8, device=device)
-    return (workspace.data_ptr(), workspace.numel() * workspace.element_size()) if workspace is not None else (None, 0)
+        if not need:
+            return None, 0
+        workspace = like.new_empty((need,), dtype=torch.uint8)
+    return workspace.data_ptr(), workspace.numel() * workspace.element_size()
 
 
 def _p(t):
@@ -103,14 +95,11 @@ def reshape_and_cache_kv8(key, value, key_cache, value_cache, key_scales, value_
         _refuse("slot_mapping must be int64 [num_tokens]")
     dt = _dtype(key, value)
     index = _launch((key, value, key_cache, value_cache, key_scales, value_scales, slot_mapping, workspace))
-    _reshape_and_cache(index, key, value, key_cache, value_cache, key_scales, value_scales, slot_mapping, workspace,
-                       n, hkv, d, bs, nb, fmt, dt)
-
-
-@_on_device
-def _reshape_and_cache(index, key, value, key_cache, value_cache, key_scales, value_scales, slot_mapping, workspace,
-                       n, hkv, d, bs, nb, fmt, dt):
-    ws, size = _write_workspace(workspace, n, bs, nb, key.device)
+    if index != _current_device():
+        with torch.cuda.device(index):
+            return reshape_and_cache_kv8(key, value, key_cache, value_cache, key_scales, value_scales, slot_mapping,
+                                         workspace)
+    ws, size = _write_workspace(workspace, n, bs, nb, key)
     check(capi.lib().nvllm_reshape_and_cache_kv8(
         key.data_ptr(), value.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), key_scales.data_ptr(),
         value_scales.data_ptr(), slot_mapping.data_ptr(), ws, size, n, hkv, d, bs, nb, fmt, dt, _raw_stream(index)))
@@ -119,7 +108,7 @@ def _reshape_and_cache(index, key, value, key_cache, value_cache, key_scales, va
 def qk_norm_rope_cache_kv8(query, key, value, q_weight, k_weight, eps, rotary, positions, key_cache, value_cache,
                            key_scales, value_scales, slot_mapping, k_out=None, q_out=None, workspace=None):
     """nvllm_qk_norm_rope_cache_kv8: `qk_norm_rope_cache` with the rotated K and V going into the 8-bit
-    cache.  k_out must not be key.  Returns q_out (query itself unless q_out is given)."""
+    cache.  k_out must not overlap key or value, nor q_out.  Returns q_out (query itself unless q_out is given)."""
     nb, bs, hkv, d, fmt = _cache(key_cache, value_cache, key_scales, value_scales)
     n, hq = query.shape[0], query.shape[1]
     if query.shape != (n, hq, d) or key.shape != (n, hkv, d) or value.shape != key.shape:
@@ -140,20 +129,17 @@ def qk_norm_rope_cache_kv8(query, key, value, q_weight, k_weight, eps, rotary, p
     dt = _dtype(query, key, value, q_weight, k_weight, cos, sin, q_out, k_out)
     index = _launch((query, key, value, q_weight, k_weight, cos, sin, positions, key_cache, value_cache, key_scales,
                      value_scales, slot_mapping, k_out, q_out, workspace))
-    _qk_norm_rope_cache(index, query, key, value, q_weight, k_weight, eps, cos, sin, positions, key_cache, value_cache,
-                        key_scales, value_scales, slot_mapping, k_out, q_out, workspace, n, hq, hkv, d, bs, nb, fmt, dt)
-    return q_out
-
-
-@_on_device
-def _qk_norm_rope_cache(index, query, key, value, q_weight, k_weight, eps, cos, sin, positions, key_cache, value_cache,
-                        key_scales, value_scales, slot_mapping, k_out, q_out, workspace, n, hq, hkv, d, bs, nb, fmt, dt):
-    ws, size = _write_workspace(workspace, n, bs, nb, query.device)
+    if index != _current_device():
+        with torch.cuda.device(index):
+            return qk_norm_rope_cache_kv8(query, key, value, q_weight, k_weight, eps, rotary, positions, key_cache,
+                                          value_cache, key_scales, value_scales, slot_mapping, k_out, q_out, workspace)
+    ws, size = _write_workspace(workspace, n, bs, nb, query)
     check(capi.lib().nvllm_qk_norm_rope_cache_kv8(
         query.data_ptr(), key.data_ptr(), value.data_ptr(), q_out.data_ptr(), _p(k_out), q_weight.data_ptr(),
         k_weight.data_ptr(), float(eps), cos.data_ptr(), sin.data_ptr(), cos.shape[0], positions.data_ptr(),
         key_cache.data_ptr(), value_cache.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(),
         slot_mapping.data_ptr(), ws, size, n, hq, hkv, d, bs, nb, fmt, dt, _raw_stream(index)))
+    return q_out
 
 
 def gather_cache_blocks_kv8(key_cache, value_cache, key_scales, value_scales, block_ids, dtype=torch.bfloat16):
@@ -165,15 +151,12 @@ def gather_cache_blocks_kv8(key_cache, value_cache, key_scales, value_scales, bl
     if dtype not in _DT:
         _refuse("dtype must be bfloat16 or float32", capi.NVLLM_ERR_UNSUPPORTED)
     index = _launch((key_cache, value_cache, key_scales, value_scales, block_ids))
-    return _gather_cache_blocks(index, key_cache, value_cache, key_scales, value_scales, block_ids, dtype,
-                                block_ids.shape[0], nb, bs, hkv, d, fmt)
-
-
-@_on_device
-def _gather_cache_blocks(index, key_cache, value_cache, key_scales, value_scales, block_ids, dtype, n, nb, bs, hkv, d,
-                         fmt):
-    keys = torch.empty((n, bs, hkv, d), dtype=dtype, device=key_cache.device)
-    values = torch.empty_like(keys)
+    if index != _current_device():
+        with torch.cuda.device(index):
+            return gather_cache_blocks_kv8(key_cache, value_cache, key_scales, value_scales, block_ids, dtype)
+    n = block_ids.shape[0]
+    keys = key_cache.new_empty((n, bs, hkv, d), dtype=dtype)
+    values = key_cache.new_empty((n, bs, hkv, d), dtype=dtype)
     check(capi.lib().nvllm_gather_cache_blocks_kv8(
         key_cache.data_ptr(), value_cache.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(),
         block_ids.data_ptr(), n, keys.data_ptr(), values.data_ptr(), nb, bs, hkv, d, fmt, _DT[dtype],
@@ -199,31 +182,29 @@ def paged_attention_kv8(query, key_cache, value_cache, key_scales, value_scales,
     [num_seqs, max_blocks], context_lens int32 [num_seqs] -> [num_seqs, T, Hq*D].  `workspace`: uint8, of
     nvllm_paged_attn_kv8_workspace_bytes; made for the call if None."""
     nb, bs, hkv, d, fmt = _cache(key_cache, value_cache, key_scales, value_scales)
-    if query.dim() != 4 or query.shape[3] != d:
+    shape, table = query.shape, block_tables.shape
+    if len(shape) != 4 or shape[3] != d:
         _refuse("query must be [num_seqs, T, Hq, D] of the cache")
-    n, t, hq, _ = query.shape
+    n, t, hq, _ = shape
     if block_tables.dtype != torch.int32 or context_lens.dtype != torch.int32:
         _refuse("block_tables and context_lens must be int32")
-    if block_tables.dim() != 2 or block_tables.shape[0] != n or context_lens.shape != (n,):
+    if len(table) != 2 or table[0] != n or context_lens.shape != (n,):
         _refuse("block_tables must be [num_seqs, max_blocks], context_lens [num_seqs]")
-    dt = _dtype(query)
+    width, dt = table[1], _dtype(query)
     index = _launch((query, key_cache, value_cache, key_scales, value_scales, block_tables, context_lens, workspace))
-    return _paged_attention(index, query, key_cache, value_cache, key_scales, value_scales, block_tables, context_lens,
-                            float(scale), workspace, n, t, hq, hkv, d, bs, block_tables.shape[1], nb, fmt, dt)
-
-
-@_on_device
-def _paged_attention(index, query, key_cache, value_cache, key_scales, value_scales, block_tables, context_lens, scale,
-                     workspace, n, t, hq, hkv, d, bs, width, nb, fmt, dt):
+    if index != _current_device():
+        with torch.cuda.device(index):
+            return paged_attention_kv8(query, key_cache, value_cache, key_scales, value_scales, block_tables,
+                                       context_lens, scale, workspace)
     L = capi.lib()
-    out = torch.empty((n, t, hq * d), dtype=query.dtype, device=query.device)
+    out = query.new_empty((n, t, hq * d))
     if workspace is None:
         need = L.nvllm_paged_attn_kv8_workspace_bytes(n, t, hq, hkv, d, bs, width, dt)
         if need:
-            workspace = torch.empty(need, dtype=torch.uint8, device=query.device)
+            workspace = query.new_empty((need,), dtype=torch.uint8)
     size = workspace.numel() * workspace.element_size() if workspace is not None else 0
     check(L.nvllm_paged_attn_kv8(
         query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), key_scales.data_ptr(),
         value_scales.data_ptr(), block_tables.data_ptr(), context_lens.data_ptr(), out.data_ptr(), _p(workspace),
-        size, n, t, hq, hkv, d, bs, width, nb, scale, fmt, dt, _raw_stream(index)))
+        size, n, t, hq, hkv, d, bs, width, nb, float(scale), fmt, dt, _raw_stream(index)))
     return out
