@@ -316,3 +316,91 @@ pub fn reshape_and_cache(
                                           block_size as c_int, num_cache_blocks as i64, stream)
     })
 }
+
+/// Number format of an 8-bit cache.
+#[derive(Debug, Clone, Copy, PartialEq, Eq)]
+pub enum Kv8Format {
+    Int8 = 0,
+    E4M3 = 1,
+}
+
+/// One layer's 8-bit cache (no counterpart in the reference): codes [num_blocks, block_size, Hkv, D], one
+/// byte each, and f32 scales [num_blocks, Hkv], K and V apart; value = code * scale.
+pub struct Kv8Cache {
+    pub key_codes: *mut c_void,
+    pub value_codes: *mut c_void,
+    pub key_scales: *mut f32,
+    pub value_scales: *mut f32,
+    pub num_blocks: usize,
+    pub block_size: usize,
+    pub num_kv_heads: usize,
+    pub head_dim: usize,
+    pub format: Kv8Format,
+}
+
+/// Workspace of `reshape_and_cache_kv8` for `num_tokens` tokens (0 for small calls).
+pub fn kv8_write_workspace_bytes(num_tokens: usize, cache: &Kv8Cache) -> usize {
+    unsafe {
+        ffi::nvllm_kv8_write_workspace_bytes(num_tokens as i64, cache.block_size as c_int, cache.num_blocks as i64)
+    }
+}
+
+/// `reshape_and_cache` into an 8-bit cache: key/value [num_tokens,Hkv,D], device `slot_mapping` i64 [num_tokens].
+pub fn reshape_and_cache_kv8(
+    key: &DeviceTensor,
+    value: &DeviceTensor,
+    cache: &mut Kv8Cache,
+    slot_mapping: *const i64,
+    workspace: *mut c_void,
+    workspace_bytes: usize,
+    stream: ffi::Stream,
+) -> Result<()> {
+    let n = match key.shape[..] {
+        [n, h, d] if h == cache.num_kv_heads && d == cache.head_dim && value.shape == key.shape => n,
+        _ => return Err(Error::Tensor("key and value must be [num_tokens, Hkv, D] of the cache".into())),
+    };
+    check(unsafe {
+        ffi::nvllm_reshape_and_cache_kv8(key.ptr, value.ptr, cache.key_codes, cache.value_codes, cache.key_scales,
+                                         cache.value_scales, slot_mapping, workspace, workspace_bytes, n as i64,
+                                         cache.num_kv_heads as c_int, cache.head_dim as c_int,
+                                         cache.block_size as c_int, cache.num_blocks as i64, cache.format as c_int,
+                                         key.dtype as c_int, stream)
+    })
+}
+
+/// Workspace of `paged_attention_kv8` (with the launch device current).
+pub fn kv8_workspace_bytes(query: &DeviceTensor, cache: &Kv8Cache, max_blocks_per_seq: usize) -> Result<usize> {
+    let (n, t, hq, d) = query.dims4()?;
+    Ok(unsafe {
+        ffi::nvllm_paged_attn_kv8_workspace_bytes(n as c_int, t as c_int, hq as c_int, cache.num_kv_heads as c_int,
+                                                  d as c_int, cache.block_size as c_int,
+                                                  max_blocks_per_seq as c_int, query.dtype as c_int)
+    })
+}
+
+/// `paged_attention_batched` over an 8-bit cache: q [N,T,Hq,D] -> `out` [N,T,Hq*D].
+#[allow(clippy::too_many_arguments)]
+pub fn paged_attention_kv8(
+    query: &DeviceTensor,
+    cache: &Kv8Cache,
+    block_tables: *const i32,
+    context_lens: *const i32,
+    max_blocks_per_seq: usize,
+    scale: f32,
+    out: &mut DeviceTensor,
+    workspace: *mut c_void,
+    workspace_bytes: usize,
+    stream: ffi::Stream,
+) -> Result<()> {
+    let (n, t, hq, d) = query.dims4()?;
+    if d != cache.head_dim {
+        return Err(Error::Tensor("query must be [N, T, Hq, D] of the cache".into()));
+    }
+    check(unsafe {
+        ffi::nvllm_paged_attn_kv8(query.ptr, cache.key_codes, cache.value_codes, cache.key_scales, cache.value_scales,
+                                  block_tables, context_lens, out.ptr, workspace, workspace_bytes, n as c_int,
+                                  t as c_int, hq as c_int, cache.num_kv_heads as c_int, d as c_int,
+                                  cache.block_size as c_int, max_blocks_per_seq as c_int, cache.num_blocks as i64,
+                                  scale, cache.format as c_int, query.dtype as c_int, stream)
+    })
+}
