@@ -292,8 +292,8 @@ int nvllm_qk_norm_rope_cache_kv8(const void *q, const void *k, const void *v, vo
 
 /* nvllm_gather_cache_blocks, dequantised: k_out[i] = the values of block block_ids[i] (device int32
  * [num_ids]), [num_ids, block_size, num_kv_heads, head_dim] in dtype; v_out likewise unless NULL
- * (then v_cache and v_scales may be NULL too).  An id outside the pool gives zeros.  Exact in bf16
- * and f32 alike. */
+ * (then v_cache and v_scales may be NULL too).  An id outside the pool gives zeros.  Exact in f32,
+ * and in bf16 but for E4M3 values below its smallest number, 2^-133 (rounded to it or to 0). */
 int nvllm_gather_cache_blocks_kv8(const void *k_cache, const void *v_cache, const float *k_scales,
                                   const float *v_scales, const int32_t *block_ids, int64_t num_ids,
                                   void *k_out, void *v_out, int64_t num_cache_blocks,

@@ -297,7 +297,7 @@ class LayerKVCache:
         if len(block_ids) == 0:  # kv_cache.rs:124-126
             raise ConfigError(capi.NVLLM_ERR_CONFIG, "block_ids cannot be empty")
         c = self.config
-        if c.dtype in KV8_FORMATS:  # the values, in bfloat16 (which holds them exactly)
+        if c.dtype in KV8_FORMATS:  # the values, in bfloat16 (which holds them exactly from 2^-133 on)
             scales = self._key_scales if cache is self._key_cache else self._value_scales
             ids = torch.tensor([int(b) for b in block_ids], dtype=torch.int32, device=cache.device)
             out = torch.empty((len(block_ids), c.block_size, c.num_kv_heads, c.head_dim), dtype=torch.bfloat16,

@@ -9,7 +9,7 @@
 // (2) a block that is filled token by token and whose scale grows on the way is off by less than one
 // step of its final scale (1/2 + 1/4 + ... of it), where a free scale adds half a step at each growth,
 // (3) E4M3 loses nothing in a growth but what leaves its smallest binade, and (4) codes times scale
-// are exact in bf16.  It costs int8 up to one bit, half a bit on average; E4M3 nothing.
+// are exact in bf16 (from its smallest number on).  It costs int8 up to one bit, half a bit on average; E4M3 nothing.
 #pragma once
 
 #include <hip/hip_runtime.h>

@@ -517,7 +517,7 @@ bool fast_shape(DType dt, const Kv8WriteArgs &a) {
            at16(a.k_weight) && at16(a.cos_cache) && at16(a.sin_cache);
 }
 
-// Read-back of whole blocks: out[i] = codes of block ids[i] times its scales, in bf16 (exact) or f32.
+// Read-back of whole blocks: out[i] = codes of block ids[i] times its scales, in bf16 or f32 (exact where the type has the number).
 // Eight values a thread (D a multiple of 8), else one; blockIdx.y takes K and V.
 // Ids outside the pool give zeros.
 template <typename ET, Kv8Format F, int V>

@@ -144,7 +144,8 @@ def qk_norm_rope_cache_kv8(query, key, value, q_weight, k_weight, eps, rotary, p
 
 def gather_cache_blocks_kv8(key_cache, value_cache, key_scales, value_scales, block_ids, dtype=torch.bfloat16):
     """nvllm_gather_cache_blocks_kv8: the values of whole blocks, block_ids int32 [n] on the device ->
-    (keys, values), each [n, block_size, Hkv, D] in dtype (exact in either)."""
+    (keys, values), each [n, block_size, Hkv, D] in dtype (exact, but for values below
+    bfloat16's smallest number, 2^-133)."""
     nb, bs, hkv, d, fmt = _cache(key_cache, value_cache, key_scales, value_scales)
     if block_ids.dtype != torch.int32 or block_ids.dim() != 1:
         _refuse("block_ids must be int32 [n]")

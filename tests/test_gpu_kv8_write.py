@@ -177,6 +177,23 @@ def test_read_back_is_exact(dev, fmt, dtype, bs, H, D):
 
 
 @pytest.mark.parametrize("fmt", FMT)
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("D", [128, 6])
+def test_read_back_of_the_smallest_and_largest_scales(dev, fmt, dtype, D):
+    """every code at the scales' ends: exact in f32; in bf16 rounded to nearest where it has no such number"""
+    codes = np.arange(256, dtype=np.uint8)
+    codes[[0x7f, 0xff]] = 0  # E4M3's NaN
+    raw = np.resize(codes, (2, 16, 2, D))
+    raw[1] = np.resize(codes[::-1], (16, 2, D))
+    scales = np.array([[2.0 ** -126, 2.0 ** -124], [2.0 ** -120, 2.0 ** 119]])
+    on = to_dev(raw, fmt, dev)
+    s = torch.from_numpy(scales).float().to(dev)
+    k, v = nv.gather_cache_blocks_kv8(on, on, s, s, torch.arange(2, dtype=torch.int32, device=dev), ELEM[dtype])
+    want = torch.from_numpy(o.numbers(raw, fmt) * scales[:, None, :, None]).float().to(ELEM[dtype])
+    assert torch.equal(k.cpu(), want) and torch.equal(v, k)
+
+
+@pytest.mark.parametrize("fmt", FMT)
 def test_layer_cache_and_gather(dev, fmt):
     cfg = nv.KVCacheConfig(16, 16, 8, 128, 2, TORCH[fmt])
     cache = nv.KVCache(cfg, dev)
