@@ -377,7 +377,7 @@ __global__ __launch_bounds__(64 * W, NQT == 1 ? 2 : 1) void paged_attn_kv8_decod
     const int32_t *__restrict__ context_lens, __bf16 *__restrict__ out, float *__restrict__ ws_o,
     float *__restrict__ ws_ml, int T, int Hq, int Hkv, int max_blocks_per_seq, int64_t num_cache_blocks,
     float scale, int num_splits, int blocks_per_split) {
-    __shared__ __attribute__((aligned(16))) unsigned char lds_all[W * 2 * kImage];
+    __shared__ __attribute__((aligned(16))) unsigned char lds_all[W * NQT * 8192];  // images; parts to join
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4, c = lane & 15;
@@ -627,56 +627,58 @@ __global__ __launch_bounds__(64 * W, NQT == 1 ? 2 : 1) void paged_attn_kv8_decod
             }
         }
 
-    // join the waves' parts, one query tile after the other: (m, l) of each row, then O relative to the common
-    // maximum, chunk 4 dt + g of row c at chunk position (4 dt + g) ^ c of its 512 bytes
-    __shared__ float ml[W][16][2];
-    float *mine = reinterpret_cast<float *>(lds_all + wave * 2 * kImage);
+    // join the waves' parts: wave w sums the dims [128 / W w, ..) of all of them, so every wave leaves the others' dims
+    // (and each row's m and l) in LDS, a lane's 16 bytes where the same lane of the reader finds them
+    __shared__ float ml[W][NQT * 16][2];
+    constexpr int kOwn = 8 / W;  // dt a wave sums
+    const auto part_of = [&](int w, int qt, int dt) {
+        return reinterpret_cast<f32x4 *>(lds_all + ((w * NQT + qt) * 8 + dt) * 1024 + 16 * lane);
+    };
+    __syncthreads();  // the images have been read
 #pragma unroll
     for (int qt = 0; qt < NQT; ++qt) {
         float l = l_run[qt];
         l += __shfl_xor(l, 16);
         l += __shfl_xor(l, 32);
-        if (qt > 0) __syncthreads();  // the previous tile's sums have been read
         if (g == 0) {
-            ml[wave][c][0] = m_run[qt];
-            ml[wave][c][1] = l;
+            ml[wave][qt * 16 + c][0] = m_run[qt];
+            ml[wave][qt * 16 + c][1] = l;
         }
-        __syncthreads();
-        float m = ml[0][c][0];
-#pragma unroll
-        for (int w = 1; w < W; ++w) m = fmaxf(m, ml[w][c][0]);
-        const float f = m_run[qt] == -INFINITY ? 0.0f : fast_exp2(m_run[qt] - m);
 #pragma unroll
         for (int dt = 0; dt < 8; ++dt)
-            *reinterpret_cast<f32x4 *>(mine + 128 * c + 4 * ((4 * dt + g) ^ c)) = acc[qt][dt] * f;
-        __syncthreads();
+            if (dt / kOwn != wave) *part_of(wave, qt, dt) = acc[qt][dt];
+    }
+    __syncthreads();
 #pragma unroll
-        for (int i = threadIdx.x; i < 512; i += 64 * W) {
-            const int rr = i >> 5, chunk = i & 31, r = qt * 16 + rr;
-            if (r >= R) continue;
-            float mr = ml[0][rr][0], L = 0.0f;
+    for (int qt = 0; qt < NQT; ++qt) {
+        const int r = qt * 16 + c;
+        if (r >= R) continue;
+        float m = ml[0][r][0], L = 0.0f, f[W];
 #pragma unroll
-            for (int w = 1; w < W; ++w) mr = fmaxf(mr, ml[w][rr][0]);
+        for (int w = 1; w < W; ++w) m = fmaxf(m, ml[w][r][0]);
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            f[w] = ml[w][r][0] == -INFINITY ? 0.0f : fast_exp2(ml[w][r][0] - m);
+            L += ml[w][r][1] * f[w];
+        }
+        const int64_t orow = ((int64_t)seq * T + t_of_row[qt]) * Hq + kvh * G + (r - t_of_row[qt] * G);
+        const float inv = L == 0.0f ? 0.0f : 1.0f / L;  // no key seen: zeros
+#pragma unroll
+        for (int dt = 0; dt < 8; ++dt) {
+            if (dt / kOwn != wave) continue;
             f32x4 y = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int w = 0; w < W; ++w) {
-                L += ml[w][rr][0] == -INFINITY ? 0.0f : ml[w][rr][1] * fast_exp2(ml[w][rr][0] - mr);
-                y += *reinterpret_cast<const f32x4 *>(lds_all + w * 2 * kImage + 512 * rr + 16 * (chunk ^ rr));
-            }
-            const int t = r / G;
-            const int64_t orow = ((int64_t)seq * T + t) * Hq + kvh * G + (r - t * G);
+            for (int w = 0; w < W; ++w) y += (w == wave ? acc[qt][dt] : *part_of(w, qt, dt)) * f[w];
             if (num_splits == 1) {
-                const float inv = L == 0.0f ? 0.0f : 1.0f / L;  // no key seen: zeros
-                *reinterpret_cast<u32x2 *>(out + orow * kD + 4 * chunk) =
+                *reinterpret_cast<u32x2 *>(out + orow * kD + 16 * dt + 4 * g) =
                     u32x2{pack_bf16x2(y[0] * inv, y[1] * inv), pack_bf16x2(y[2] * inv, y[3] * inv)};
             } else {
-                const int64_t prow = orow * num_splits + split;
-                *reinterpret_cast<f32x4 *>(ws_o + prow * kD + 4 * chunk) = y;
-                if (chunk == 0) {
-                    ws_ml[2 * prow] = mr;
-                    ws_ml[2 * prow + 1] = L;
-                }
+                *reinterpret_cast<f32x4 *>(ws_o + (orow * num_splits + split) * kD + 16 * dt + 4 * g) = y;
             }
+        }
+        if (num_splits > 1 && wave == 0 && g == 0) {
+            ws_ml[2 * (orow * num_splits + split)] = m;
+            ws_ml[2 * (orow * num_splits + split) + 1] = L;
         }
     }
 }
@@ -701,6 +703,7 @@ __global__ __launch_bounds__(64 * W, NQT == 1 ? 2 : 1) void paged_attn_kv8_decod
 // staging with half the LDS conflicts and products interleaved with the exponentials by hand were each within 3 % or slower.
 // ---------------------------------------------------------------------------
 typedef __attribute__((ext_vector_type(16))) float f32x16;
+typedef __attribute__((ext_vector_type(2))) float f32x2;
 typedef __attribute__((ext_vector_type(4))) short s16x4;
 
 constexpr int kWideRow = 2 * kD;              // bytes of a widened row
@@ -766,10 +769,10 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kv8_tile_kernel(
 
     // staging: thread covers 16 dims (lch) of rows tid / 8 and 32 + tid / 8 of the tile
     const int64_t block_bytes = (int64_t)kBS * Hkv * kD;
-    const int sr = threadIdx.x >> 3, lch = threadIdx.x & 7;
+    const int sr = 16 * wave + (lane >> 3), lch = threadIdx.x & 7;
     const int head_bytes = (kBS - 1) * Hkv * kD + kD;
     const unsigned lane_off = (unsigned)(sr & 15) * (unsigned)(Hkv * kD) + 16u * lch;
-    const int sb = wave >> 1;  // block of the first row within its 32 keys
+    const int sb = wave;  // block of the first row within its 32 keys
     unsigned kw[2], vw[2];     // LDS positions of the two 16-byte chunks of the first row; the second: + 32 rows
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
@@ -786,9 +789,9 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kv8_tile_kernel(
         }
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const int64_t at = run.id_at(j + 2 * i + sb) * block_bytes + kvh * kD;
-            ck[i] = load16<STREAM>(block_rows(k_cache, at, head_bytes, t < ntiles), lane_off, 0);
-            cv[i] = load16<STREAM>(block_rows(v_cache, at, head_bytes, t < ntiles), lane_off, 0);
+            const int64_t at = run.id_at(j + sb) * block_bytes + kvh * kD;
+            ck[i] = load16<STREAM>(block_rows(k_cache, at, head_bytes, t < ntiles), lane_off, 8 * i * (unsigned)(Hkv * kD));
+            cv[i] = load16<STREAM>(block_rows(v_cache, at, head_bytes, t < ntiles), lane_off, 8 * i * (unsigned)(Hkv * kD));
         }
         if (j == kRun - kBigBlocks) run.advance(blk_begin + kBigBlocks * (t + 1));
     };
@@ -800,7 +803,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kv8_tile_kernel(
         if (key0 + kBigKeys > keys_all) {
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const int key = key0 + 32 * i + sr;
+                const int key = key0 + 8 * i + sr;
                 if (key >= keys || key >= blk_end * kBS) cv[i] = u32x4{0u, 0u, 0u, 0u};
                 if constexpr (F == Kv8Format::E4M3)
 #pragma unroll
@@ -815,8 +818,8 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kv8_tile_kernel(
         for (int i = 0; i < 2; ++i)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                *reinterpret_cast<bf16x8 *>(buf + kw[e] + 32 * kWideRow * i) = widen8<F>(ck[i][2 * e], ck[i][2 * e + 1]);
-                *reinterpret_cast<bf16x8 *>(buf + vw[e] + 32 * kWideRow * i) = widen8<F>(cv[i][2 * e], cv[i][2 * e + 1]);
+                *reinterpret_cast<bf16x8 *>(buf + (kw[e] ^ (i ? 128u : 0u)) + 8 * kWideRow * i) = widen8<F>(ck[i][2 * e], ck[i][2 * e + 1]);
+                *reinterpret_cast<bf16x8 *>(buf + vw[e] + 8 * kWideRow * i) = widen8<F>(cv[i][2 * e], cv[i][2 * e + 1]);
             }
     };
 
@@ -918,9 +921,12 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kv8_tile_kernel(
         // codes of tile t + 2 are on their way while tile t is multiplied and t + 1 goes into LDS
         u32x4 ck[2], cv[2];
         Scales sc[2];
-        load_tile(0, ck, cv, sc[0]);
-        stage_tile(0, lds, ck, cv);
-        load_tile(1, ck, cv, sc[1]);
+        {
+            u32x4 k0[2], v0[2];
+            load_tile(0, k0, v0, sc[0]);
+            load_tile(1, ck, cv, sc[1]);
+            stage_tile(0, lds, k0, v0);
+        }
         for (int t0 = 0; t0 < ntiles; t0 += 2)
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
@@ -947,17 +953,17 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kv8_tile_kernel(
                 __syncthreads();
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    const int key = key0 + 32 * i + sr;
+                    const int key = key0 + 8 * i + sr;
                     u32x4 one = {0u, 0u, 0u, 0u};
                     if (key < keys && key < blk_end * kBS) {
                         const int64_t at = pool_id(table[key / kBS], num_cache_blocks) * block_bytes + kvh * kD;
-                        one = *reinterpret_cast<const u32x4 *>(v_cache + at + lane_off);
+                        one = *reinterpret_cast<const u32x4 *>(v_cache + at + lane_off + 8 * i * (unsigned)(Hkv * kD));
 #pragma unroll
                         for (int e = 0; e < 4; ++e) one[e] = nan_bytes(one[e]) & 0x38383838u;  // 1.0
                     }
 #pragma unroll
                     for (int e = 0; e < 2; ++e)
-                        *reinterpret_cast<bf16x8 *>(lds + vw[e] + 32 * kWideRow * i) = widen8<F>(one[2 * e], one[2 * e + 1]);
+                        *reinterpret_cast<bf16x8 *>(lds + vw[e] + 8 * kWideRow * i) = widen8<F>(one[2 * e], one[2 * e + 1]);
                 }
                 __syncthreads();
 #pragma unroll 1
@@ -985,49 +991,67 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kv8_tile_kernel(
     }
 
     float l = half_sum(l_run);
-    if constexpr (KG == 2) {  // the second key half's waves hand theirs over: O [64 values a lane], m, l
+    constexpr int kOwn = 4 / KG;  // 32-dim tiles that the wave writes
+    const int dt0 = kOwn * kg;
+    if constexpr (KG == 2) {
+        // the two key halves' waves hand each other the dims that the other one sums, a lane's 16 bytes where the same
+        // lane of the reader finds them, and (m, l)
+        const auto part_of = [&](int w, int j) { return reinterpret_cast<f32x4 *>(lds + (8 * w + j) * 1024 + 16 * lane); };
+        f32x2 *ml = reinterpret_cast<f32x2 *>(lds + 32 * 1024);
         __syncthreads();
-        float *slot = reinterpret_cast<float *>(lds) + (wave & 1) * (66 * 64) + lane;
-        if (kg == 1) {
 #pragma unroll
-            for (int dt = 0; dt < 4; ++dt)
+        for (int j = 0; j < 8; ++j) {
+            const int q = 4 * (j & 3), d = j >> 2;
+            f32x4 x;
 #pragma unroll
-                for (int i = 0; i < 16; ++i) slot[64 * (16 * dt + i)] = acc[dt][i];
-            slot[64 * 64] = m_ref;
-            slot[64 * 65] = l;
+            for (int e = 0; e < 4; ++e) {
+                x[e] = kg == 0 ? acc[2 + d][q + e] : acc[d][q + e];
+                acc[d][q + e] = kg == 0 ? acc[d][q + e] : acc[2 + d][q + e];  // its own dims from here on
+            }
+            *part_of(wave, j) = x;
         }
+        ml[64 * wave + lane] = f32x2{m_ref, l};
         __syncthreads();
-        if (kg == 1) return;
-        const float m2 = slot[64 * 64], l2 = slot[64 * 65];
-        const float m = fmaxf(m_ref, m2);
-        const float a1 = m_ref == -INFINITY ? 0.0f : fast_exp2(m_ref - m), a2 = m2 == -INFINITY ? 0.0f : fast_exp2(m2 - m);
+        const f32x2 other = ml[64 * (wave ^ 2) + lane];
+        const float m = fmaxf(m_ref, other[0]);
+        const float a1 = m_ref == -INFINITY ? 0.0f : fast_exp2(m_ref - m);
+        const float a2 = other[0] == -INFINITY ? 0.0f : fast_exp2(other[0] - m);
 #pragma unroll
-        for (int dt = 0; dt < 4; ++dt)
+        for (int j = 0; j < 8; ++j) {
+            const f32x4 x = *part_of(wave ^ 2, j);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) acc[dt][i] = acc[dt][i] * a1 + slot[64 * (16 * dt + i)] * a2;
-        l = l * a1 + l2 * a2;
+            for (int e = 0; e < 4; ++e)
+                acc[j >> 2][4 * (j & 3) + e] = acc[j >> 2][4 * (j & 3) + e] * a1 + x[e] * a2;
+        }
+        l = l * a1 + other[1] * a2;
         m_ref = m;
     }
-    if (!live) return;
     if (num_splits == 1) {
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // no key seen: zeros
-        __bf16 *op = out + orow * kD + 4 * h;
+        __bf16 *op = out + orow * kD + 32 * dt0 + 8 * h;
 #pragma unroll
-        for (int dt = 0; dt < 4; ++dt)
+        for (int dt = 0; dt < kOwn; ++dt)
 #pragma unroll
-            for (int i = 0; i < 16; i += 4)
-                *reinterpret_cast<u32x2 *>(op + 32 * dt + 2 * i) =
-                    u32x2{pack_bf16x2(acc[dt][i] * inv, acc[dt][i + 1] * inv),
-                          pack_bf16x2(acc[dt][i + 2] * inv, acc[dt][i + 3] * inv)};
-    } else {
+            for (int i = 0; i < 16; i += 8) {
+                // lanes c and c + 32 have dims 4 h .. + 3 of two eights: trade for one eight each
+                float x[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    x[e] = __builtin_bit_cast(float, pack_bf16x2(acc[dt][i + 2 * e] * inv, acc[dt][i + 2 * e + 1] * inv));
+                swap_halves(x[0], x[2]);
+                swap_halves(x[1], x[3]);
+                if (live)
+                    *reinterpret_cast<f32x4 *>(op + 32 * dt + 2 * i) = f32x4{x[0], x[1], x[2], x[3]};
+            }
+    } else if (live) {
         const int64_t prow = orow * num_splits + split;
-        float *op = ws_o + prow * kD + 4 * h;
+        float *op = ws_o + prow * kD + 32 * dt0 + 4 * h;
 #pragma unroll
-        for (int dt = 0; dt < 4; ++dt)
+        for (int dt = 0; dt < kOwn; ++dt)
 #pragma unroll
             for (int i = 0; i < 16; i += 4)
                 *reinterpret_cast<f32x4 *>(op + 32 * dt + 2 * i) = f32x4{acc[dt][i], acc[dt][i + 1], acc[dt][i + 2], acc[dt][i + 3]};
-        if (h == 0) {
+        if (h == 0 && kg == 0) {
             ws_ml[2 * prow] = m_ref;
             ws_ml[2 * prow + 1] = l;
         }
