@@ -370,8 +370,11 @@ __device__ __forceinline__ unsigned nan_bytes(unsigned w) {
     return ((t & 0x80808080u) >> 7) * 0xffu;
 }
 
+// NQT query tiles of 16 rows.  One and two leave room for two waves a SIMD, two of them with NBUF 2 (against one wave and
+// NBUF 4 in workgroups of two waves: 256 x 2048 T = 8 213 -> 194 us, 128 x 512 38 -> 32, 4 x 4096 19 -> 15; 64 x 4096 99 ->
+// 104); three need a SIMD's registers.
 template <Kv8Format F, int NQT, int W, int NBUF, bool STREAM>
-__global__ __launch_bounds__(64 * W, NQT == 1 ? 2 : 1) void paged_attn_kv8_decode_kernel(
+__global__ __launch_bounds__(64 * W, NQT <= 2 ? 2 : 1) void paged_attn_kv8_decode_kernel(
     const __bf16 *__restrict__ q, const unsigned char *__restrict__ k_cache, const unsigned char *__restrict__ v_cache,
     const float *__restrict__ k_scales, const float *__restrict__ v_scales, const int32_t *__restrict__ block_tables,
     const int32_t *__restrict__ context_lens, __bf16 *__restrict__ out, float *__restrict__ ws_o,
@@ -1133,26 +1136,31 @@ hipError_t launch_tile_of(const PagedAttnArgs &a, const float *ks, const float *
     return streams(a) ? launch_tile<F, 2, true>(a, ks, vs, stream) : launch_tile<F, 2, false>(a, ks, vs, stream);
 }
 
-int decode_waves(const PagedAttnArgs &a) { return query_rows(a) <= 16 ? 4 : 2; }
+int decode_waves(const PagedAttnArgs &a) { return query_rows(a) <= 32 ? 4 : 2; }
 
-// Parts of the keys over workgroups: up to 1024 waves in all (4 a CU), each with 64 keys at least.  Two parts do not
-// pay for the merge launch (16 x 2048: 20.8 against 20.7 us, 16 x 512: 9.3 against 8.3), unless half the CUs would
-// stay without the one workgroup of two or more query tiles that they hold.
+// Parts of the keys over workgroups: up to 1024 waves in all (4 a CU), each with 64 keys at least; for the workgroups of
+// four waves up to 2048, where a part still has 4096 keys (16 x 16384: 141 us whole, 96 in four parts; 32 x 8192 104 and
+// 97 in two).  Two parts do not pay for the merge launch in short walks (16 x 2048: 20.8 against 20.7 us, 16 x 512 9.3
+// against 8.3; but 12 x 4096 T = 8 37 whole, 27 in two), unless half the CUs would stay without the one workgroup of
+// three query tiles that they hold.
 int decode_splits(const PagedAttnArgs &a) {
     const int w = decode_waves(a), forced = launch_policy().paged_splits;
-    int64_t splits = 4 * (int64_t)device_cus() / ((int64_t)a.num_seqs * a.num_kv_heads * w);
+    const int64_t waves = (int64_t)a.num_seqs * a.num_kv_heads * w, keys = (int64_t)a.max_blocks_per_seq * kBS;
+    const int64_t most = 8 * (int64_t)device_cus() / waves;
+    int64_t splits = 4 * (int64_t)device_cus() / waves;
+    if (w == 4 && most >= 2 && keys >= 4096 * most) splits = most;
+    else if (w == 4 && splits == 2 && keys < 4096) splits = 1;
     const int64_t cap = a.max_blocks_per_seq / (4 * w);
     if (forced > 0) splits = forced;
     if (splits > cap) splits = cap;
     if (splits > 64) splits = 64;  // the merge kernel holds one split's (m, l) per lane
-    if (splits < (w == 4 && forced <= 0 ? 3 : 2)) splits = 1;
-    return (int)splits;
+    return splits < 2 ? 1 : (int)splits;
 }
 
 template <Kv8Format F, int NQT, int W, bool STREAM>
 void launch_decode_as(const PagedAttnArgs &a, const float *ks, const float *vs, int splits, float *ws_o, float *ws_ml,
                       hipStream_t stream) {
-    paged_attn_kv8_decode_kernel<F, NQT, W, NQT == 1 ? 3 : 4, STREAM>
+    paged_attn_kv8_decode_kernel<F, NQT, W, NQT == 1 ? 3 : NQT == 2 ? 2 : 4, STREAM>
         <<<dim3(splits, a.num_seqs, a.num_kv_heads), dim3(64 * W), 0, stream>>>(
             static_cast<const __bf16 *>(a.q), static_cast<const unsigned char *>(a.k_cache),
             static_cast<const unsigned char *>(a.v_cache), ks, vs, a.block_tables, a.context_lens,
@@ -1172,7 +1180,7 @@ hipError_t launch_decode(const PagedAttnArgs &a, const float *ks, const float *v
         else launch_decode_as<F, NQT, W, false>(a, ks, vs, splits, ws_o, ws_ml, stream);        \
         break;
     switch ((int)((query_rows(a) + 15) / 16)) {
-        NVLLM_KV8_CASE(1, 4) NVLLM_KV8_CASE(2, 2) NVLLM_KV8_CASE(3, 2)
+        NVLLM_KV8_CASE(1, 4) NVLLM_KV8_CASE(2, 4) NVLLM_KV8_CASE(3, 2)
         default: return hipErrorInvalidValue;
     }
 #undef NVLLM_KV8_CASE
