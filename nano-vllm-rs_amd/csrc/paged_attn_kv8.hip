@@ -1138,18 +1138,21 @@ hipError_t launch_tile_of(const PagedAttnArgs &a, const float *ks, const float *
 
 int decode_waves(const PagedAttnArgs &a) { return query_rows(a) <= 32 ? 4 : 2; }
 
-// Parts of the keys over workgroups: up to 1024 waves in all (4 a CU), each with 64 keys at least; for the workgroups of
-// four waves up to 2048, where a part still has 4096 keys (16 x 16384: 141 us whole, 96 in four parts; 32 x 8192 104 and
-// 97 in two).  Two parts do not pay for the merge launch in short walks (16 x 2048: 20.8 against 20.7 us, 16 x 512 9.3
-// against 8.3; but 12 x 4096 T = 8 37 whole, 27 in two), unless half the CUs would stay without the one workgroup of
-// three query tiles that they hold.
+// Parts of the keys over workgroups: up to 1024 waves in all (4 a CU), each with 64 keys at least.  Two parts do not pay
+// for the merge launch in short walks (16 x 2048: 20.8 against 20.7 us, 16 x 512 9.3 against 8.3; but 16 x 4096 T = 8 44
+// whole, 33 in two), unless half the CUs would stay without the one workgroup of three query tiles that they hold.
+// One query tile and long walks that the chip holds at once: parts of 2048 keys, as the last workgroups then end closer
+// together (64 x 8192: 194 us whole, 177 in four parts; 32 x 16384 204 and 176; but 48 x 4096 70 and 74, 128 x 8192 with
+// two rounds of workgroups 338 and 348).
 int decode_splits(const PagedAttnArgs &a) {
-    const int w = decode_waves(a), forced = launch_policy().paged_splits;
-    const int64_t waves = (int64_t)a.num_seqs * a.num_kv_heads * w, keys = (int64_t)a.max_blocks_per_seq * kBS;
-    const int64_t most = 8 * (int64_t)device_cus() / waves;
-    int64_t splits = 4 * (int64_t)device_cus() / waves;
-    if (w == 4 && most >= 2 && keys >= 4096 * most) splits = most;
-    else if (w == 4 && splits == 2 && keys < 4096) splits = 1;
+    const int w = decode_waves(a), forced = launch_policy().paged_splits, cus = device_cus();
+    const int64_t units = (int64_t)a.num_seqs * a.num_kv_heads, keys = (int64_t)a.max_blocks_per_seq * kBS;
+    int64_t splits = 4 * cus / (units * w);
+    if (w == 4 && splits == 2 && keys < 4096) splits = 1;
+    if (query_rows(a) <= 16 && units <= 2 * cus && keys >= 8192) {
+        const int64_t parts = keys / 2048 < 8 * cus / units ? keys / 2048 : 8 * cus / units;
+        if (parts > splits) splits = parts;
+    }
     const int64_t cap = a.max_blocks_per_seq / (4 * w);
     if (forced > 0) splits = forced;
     if (splits > cap) splits = cap;
