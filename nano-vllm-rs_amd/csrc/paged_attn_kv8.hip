@@ -215,8 +215,8 @@ hipError_t launch_generic(const PagedAttnArgs &a, const float *ks, const float *
 //
 // Bound by HBM: a cached token costs 2 * Hkv * 128 bytes, half of the bf16 cache's.  A workgroup has one kv head
 // of one sequence, its W waves a part of the keys each (all query rows of the head), and they join through LDS at
-// the end: one launch, no workspace.  Only where (sequence, kv head) pairs are few are the keys split over
-// workgroups as well, with partials and a merge launch as in paged_attn.hip.  (Waves for the heads of a sequence
+// the end: one launch, no workspace.  Only where (sequence, kv head) pairs are few or walks long are the keys split
+// over workgroups as well, with partials and a merge launch as in paged_attn.hip.  (Waves for the heads of a sequence
 // instead, which read whole blocks together, as the bf16 kernel has them: 256 x 2048 int8 184 against 166 us,
 // 64 x 4096 with 4 splits 91 against 95; short walks even out better.)  What one byte a value changes:
 //   tile    32 keys (2 blocks), 8 KiB.  NBUF tiles in registers, all but one of them on their way;
@@ -701,9 +701,10 @@ __global__ __launch_bounds__(64 * W, NQT <= 2 ? 2 : 1) void paged_attn_kv8_decod
 // at ch ^ 2 (r & 7) (transposed reads of 4 rows x 16 dims).
 //
 // Bounds: with many rows the products and, between them, the exponentials (chunk of 4 x 1024 rows behind 7168 keys,
-// 2.6e11 operations: 282 us, 910 TFLOP/s); with few the way of the bytes into LDS (64 x 4096 T = 13, 537 MB: 123 us,
-// 4.4 TB/s; the same without the products 106, without the widening 125).  Two tiles in registers instead of one, 8-byte
-// staging with half the LDS conflicts and products interleaved with the exponentials by hand were each within 3 % or slower.
+// 2.6e11 operations: 279 us, 925 TFLOP/s); with few the loads (64 x 4096 T = 13, 537 MB: 121 us, 4.4 TB/s; the loads
+// alone 110) and a workgroup's start and end (256 x 64 T = 16: 35 us of the 248 of 256 x 2048).  Two to four tiles in
+// registers instead of one, three workgroups a CU, other orders of the workgroups, 8-byte staging with half the LDS
+// conflicts and products interleaved with the exponentials by hand were each within 3 % or slower.
 // ---------------------------------------------------------------------------
 typedef __attribute__((ext_vector_type(16))) float f32x16;
 typedef __attribute__((ext_vector_type(2))) float f32x2;
