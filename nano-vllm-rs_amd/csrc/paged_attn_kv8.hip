@@ -219,7 +219,8 @@ hipError_t launch_generic(const PagedAttnArgs &a, const float *ks, const float *
 // over workgroups as well, with partials and a merge launch as in paged_attn.hip.  (Waves for the heads of a sequence
 // instead, which read whole blocks together, as the bf16 kernel has them: 256 x 2048 int8 184 against 166 us,
 // 64 x 4096 with 4 splits 91 against 95; short walks even out better.)  What one byte a value changes:
-//   tile    32 keys (2 blocks), 8 KiB.  NBUF tiles in registers, all but one of them on their way;
+//   tile    32 keys (2 blocks), 8 KiB.  One in registers, the next on its way (two or three ahead: 256 x 2048 the
+//           same, 256 x 512 T = 12 92 against 84 us, 16 x 2048 17.8 against 16.3);
 //   K       8 lanes x 16 B read a 128-byte row, 8 rows an instruction; through the wave's LDS image (16-byte
 //           chunk ch of row r at position ch ^ (r & 7): 8 rows x 1 chunk and 1 row x 8 chunks both touch
 //           all banks once).  A lane reads chunks 4i + g of row c: 16 dims = two MFMA k-steps of 8, so the
@@ -370,10 +371,10 @@ __device__ __forceinline__ unsigned nan_bytes(unsigned w) {
     return ((t & 0x80808080u) >> 7) * 0xffu;
 }
 
-// NQT query tiles of 16 rows.  One and two leave room for two waves a SIMD, two of them with NBUF 2 (against one wave and
-// NBUF 4 in workgroups of two waves: 256 x 2048 T = 8 213 -> 194 us, 128 x 512 38 -> 32, 4 x 4096 19 -> 15; 64 x 4096 99 ->
-// 104); three need a SIMD's registers.
-template <Kv8Format F, int NQT, int W, int NBUF, bool STREAM>
+// NQT query tiles of 16 rows.  One and two leave room for two waves a SIMD and more (two in workgroups of four waves
+// against one wave a SIMD in workgroups of two: 256 x 2048 T = 8 213 -> 194 us, 128 x 512 38 -> 32, 4 x 4096 19 -> 15;
+// 64 x 4096 99 -> 104); three need a SIMD's registers.
+template <Kv8Format F, int NQT, int W, bool STREAM>
 __global__ __launch_bounds__(64 * W, NQT <= 2 ? 2 : 1) void paged_attn_kv8_decode_kernel(
     const __bf16 *__restrict__ q, const unsigned char *__restrict__ k_cache, const unsigned char *__restrict__ v_cache,
     const float *__restrict__ k_scales, const float *__restrict__ v_scales, const int32_t *__restrict__ block_tables,
@@ -578,13 +579,12 @@ __global__ __launch_bounds__(64 * W, NQT <= 2 ? 2 : 1) void paged_attn_kv8_decod
 
     if (ntiles > 0) {
         run.begin(blk_begin);
-        Tile tl[NBUF];
+        Tile tl[2];
+        load_tile(tl[0], 0);
+        for (int t = 0; t < ntiles; t += 2)
 #pragma unroll
-        for (int u = 0; u < NBUF - 1; ++u) load_tile(tl[u], u);
-        for (int t = 0; t < ntiles; t += NBUF)
-#pragma unroll
-            for (int u = 0; u < NBUF; ++u) {
-                load_tile(tl[(u + NBUF - 1) % NBUF], t + u + NBUF - 1);
+            for (int u = 0; u < 2; ++u) {
+                load_tile(tl[1 - u], t + u + 1);
                 if (t + u < ntiles) compute_tile(tl[u], t + u);
             }
     }
@@ -1164,7 +1164,7 @@ int decode_splits(const PagedAttnArgs &a) {
 template <Kv8Format F, int NQT, int W, bool STREAM>
 void launch_decode_as(const PagedAttnArgs &a, const float *ks, const float *vs, int splits, float *ws_o, float *ws_ml,
                       hipStream_t stream) {
-    paged_attn_kv8_decode_kernel<F, NQT, W, NQT == 1 ? 3 : NQT == 2 ? 2 : 4, STREAM>
+    paged_attn_kv8_decode_kernel<F, NQT, W, STREAM>
         <<<dim3(splits, a.num_seqs, a.num_kv_heads), dim3(64 * W), 0, stream>>>(
             static_cast<const __bf16 *>(a.q), static_cast<const unsigned char *>(a.k_cache),
             static_cast<const unsigned char *>(a.v_cache), ks, vs, a.block_tables, a.context_lens,
