@@ -251,6 +251,28 @@ def test_softmax_scales_without_a_plus(dev, fmt, dtype, D, bs, T, scale):
     compare(call(on, scale), host, scale, dtype)
 
 
+@pytest.mark.parametrize("splits", [0, 2, 5])
+@pytest.mark.parametrize("T", [1, 6, 12, 13, 50])
+def test_nothing_is_written_outside_output_and_workspace(dev, policy, T, splits):
+    """rows behind the last sequence and bytes behind the workspace that the entry asks for keep what they held"""
+    policy.setenv("NVLLM_PAGED_SPLITS", splits)
+    rng = np.random.default_rng(17)
+    Hq, H, D, N = 8, 2, 128, 3
+    on, host = make(rng, "e4m3", "bf16", [T, 600, 1500], T, Hq, H, D, 16, dev)
+    L, width = nv.capi.lib(), on["tables"].shape[1]
+    need = L.nvllm_paged_attn_kv8_workspace_bytes(N, T, Hq, H, D, 16, width, 0)
+    assert need > 0 or splits == 0
+    ws = torch.full((need + 4096,), 0xa5, dtype=torch.uint8, device=dev)
+    out = torch.full((N + 1, T, Hq * D), 7.0, dtype=torch.bfloat16, device=dev)
+    rc = L.nvllm_paged_attn_kv8(on["q"].data_ptr(), on["k"].data_ptr(), on["v"].data_ptr(), on["ks"].data_ptr(),
+                                on["vs"].data_ptr(), on["tables"].data_ptr(), on["lens"].data_ptr(), out.data_ptr(),
+                                ws.data_ptr(), need, N, T, Hq, H, D, 16, width, on["k"].shape[0], 0.1, 1, 0,
+                                torch.cuda.current_stream().cuda_stream)
+    assert rc == 0
+    compare(out[:N], host, 0.1, "bf16")
+    assert bool((out[N] == 7.0).all()) and bool((ws[need:] == 0xa5).all())
+
+
 @pytest.mark.parametrize("T,lens", [(1, [70, 300]), (1, [5000]), (5, [800, 9]), (40, [500, 77])])
 def test_same_bits_again_on_another_stream_and_in_a_graph(dev, T, lens):
     """no result depends on the order of anything: repeated, side by side on two streams, replayed from a
@@ -284,6 +306,31 @@ def test_same_bits_again_on_another_stream_and_in_a_graph(dev, T, lens):
         g.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, eager), cut
+
+
+def test_two_graphs_share_a_workspace(dev, policy):
+    """replayed in turn, with eager work of either shape between the replays"""
+    policy.setenv("NVLLM_PAGED_SPLITS", 3)
+    rng = np.random.default_rng(18)
+    cases = [make(rng, "int8", "bf16", lens, T, 16, 8, 128, 16, dev)[0] for T, lens in ((1, [900, 2000]), (20, [1500, 64]))]
+    need = max(nv.capi.lib().nvllm_paged_attn_kv8_workspace_bytes(2, c["q"].shape[1], 16, 8, 128, 16,
+                                                                 c["tables"].shape[1], 0) for c in cases)
+    assert need > 0
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    want = [call(c, 0.1) for c in cases]
+    graphs, outs = [], []
+    for c in cases:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(call(c, 0.1, workspace=ws))
+        graphs.append(g)
+    for _ in range(3):
+        for i in (0, 1, 1, 0):
+            outs[i].zero_()
+            call(cases[1 - i], 0.1, workspace=ws)
+            graphs[i].replay()
+            torch.cuda.synchronize()
+            assert torch.equal(outs[i], want[i])
 
 
 @pytest.mark.parametrize("fmt", FMT)

@@ -137,6 +137,41 @@ def test_values_at_the_edges(dev, fmt, dtype, D):
     _write_both(rng, fmt, dtype, 6, bs, H, D, list(range(16, 80)), dev, make=make)
 
 
+@pytest.mark.parametrize("n", [60, 3000])
+def test_nothing_is_written_outside(dev, n):
+    """a pool between guards, outputs and workspace with a tail: only what the call names changes"""
+    rng = np.random.default_rng(n)
+    bs, H, Hq, D, nb = 16, 2, 4, 128, 300
+    edge = bs * H * D
+    mem = [torch.full(((nb + 2) * edge,), 0x55, dtype=torch.uint8, device=dev) for _ in range(2)]
+    scale_mem = [torch.full(((nb + 2) * H,), 3.0, device=dev) for _ in range(2)]
+    kc, vc = (m[edge:-edge].view(nb, bs, H, D).view(torch.int8) for m in mem)
+    ks, vs = (m[H:-H].view(nb, H) for m in scale_mem)
+    q = torch.randn((n, Hq, D), device=dev).to(torch.bfloat16)
+    k, v = (torch.randn((n, H, D), device=dev).to(torch.bfloat16) for _ in range(2))
+    q_mem, k_mem = (torch.full((n + 1, h, D), 7.0, dtype=torch.bfloat16, device=dev) for h in (Hq, H))
+    need = nv.capi.lib().nvllm_kv8_write_workspace_bytes(n, bs, nb)
+    ws = torch.full((need + 4096,), 0xa5, dtype=torch.uint8, device=dev)
+    slots = torch.from_numpy(rng.permutation((nb // 2) * bs)[:n] + (nb // 2) * bs if n < 1000 else
+                             rng.permutation(nb * bs)[:n]).to(dev)
+    slots[0], slots[1] = -1, nb * bs
+    w = torch.ones(D, dtype=torch.bfloat16, device=dev)
+    rot = nv.RotaryEmbedding(D, 64, 1e6, torch.bfloat16, dev)
+    pos = torch.from_numpy(rng.integers(0, 64, n).astype(np.int32)).to(dev)
+    nv.qk_norm_rope_cache_kv8(q, k, v, w, w, 1e-6, rot, pos, kc, vc, ks, vs, slots, k_out=k_mem[:n], q_out=q_mem[:n],
+                              workspace=ws[:need] if need else None)
+    assert bool((q_mem[n] == 7.0).all()) and bool((k_mem[n] == 7.0).all()) and bool((ws[need:] == 0xa5).all())
+    for m in mem:
+        assert bool((m[:edge] == 0x55).all()) and bool((m[-edge:] == 0x55).all())
+    for m in scale_mem:
+        assert bool((m[:H] == 3.0).all()) and bool((m[-H:] == 3.0).all())
+    touched = torch.zeros(nb, dtype=torch.bool, device=dev)
+    live = slots[(slots >= 0) & (slots < nb * bs)]
+    touched[live // bs] = True
+    for c, s in ((kc, ks), (vc, vs)):
+        assert bool((c[~touched].view(torch.uint8) == 0x55).all()) and bool((s[~touched] == 3.0).all())
+
+
 def test_empty_call_and_untouched_blocks(dev):
     rng = np.random.default_rng(1)
     kc, ks, kw, ksw = _cache(rng, 4, 16, 2, 128, "int8", dev)
