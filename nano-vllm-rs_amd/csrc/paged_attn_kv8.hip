@@ -1074,15 +1074,15 @@ bool decode_path(DType dt, const PagedAttnArgs &a) { return fast_shape(dt, a) &&
 int tile_rows(const PagedAttnArgs &a) { return query_rows(a) <= 64 ? 64 : 128; }
 
 // Parts of the key walk: two workgroups on every CU, each part 256 keys at least.  One workgroup on every CU is more than
-// half as fast as two, so with as many as that a second part pays for the merge only where the walk is long (256
-// workgroups: 2048 keys 53 us whole, 81 us in two parts; 8192 keys 183 and 185; 16384 keys 270 and 247); fewer always do
-// (128 workgroups of 4096 keys: 69 us whole, 49 in two parts, 43 in four).
+// half as fast as two, so with as many as that a second part pays for the merge only in longer walks (256 workgroups: 2048
+// keys 51 us whole, 56 in two parts; 4096 71 and 67; 8192 137 and 126).  Fewer: 192 workgroups of 4096 keys
+// 69 and 58; 64 of 4096 keys in four parts 55, whole 90.
 int tile_splits(const PagedAttnArgs &a) {
     const int64_t rows = tile_rows(a);
     const int64_t units = (int64_t)a.num_seqs * a.num_kv_heads * ((query_rows(a) + rows - 1) / rows);
     const int forced = launch_policy().paged_splits;
     int64_t splits = forced > 0 ? forced : 2 * device_cus() / units;
-    if (forced <= 0 && splits == 2 && a.max_blocks_per_seq < 8192 / kBS) splits = 1;
+    if (forced <= 0 && splits == 2 && a.max_blocks_per_seq < 4096 / kBS) splits = 1;
     const int64_t most = a.max_blocks_per_seq / 16;
     if (splits > most) splits = most;
     if (splits > 64) splits = 64;  // the merge kernel holds one split's (m, l) per lane
@@ -1098,6 +1098,39 @@ bool partials(const PagedAttnArgs &a, int splits, float **ws_o, float **ws_ml) {
     *ws_o = static_cast<float *>(a.workspace);
     *ws_ml = *ws_o + rows * splits * kD;
     return true;
+}
+
+// Partials -> output, a half-wave a row, lane l dims 4 l .. + 3.
+__global__ __launch_bounds__(256) void paged_attn_kv8_merge_kernel(const float *__restrict__ ws_o,
+                                                                   const float *__restrict__ ws_ml,
+                                                                   __bf16 *__restrict__ out, int64_t rows, int splits) {
+    const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int l4 = 4 * (threadIdx.x & 31);
+    if (row >= rows) return;
+    const float *ml = ws_ml + 2 * row * splits, *o = ws_o + row * splits * kD + l4;
+    float m = -INFINITY, l = 0.0f;
+    for (int s = 0; s < splits; ++s) m = fmaxf(m, ml[2 * s]);
+    f32x4 y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int s = 0; s < splits; ++s) {
+        const float w = ml[2 * s] == -INFINITY ? 0.0f : fast_exp2(ml[2 * s] - m);
+        l += ml[2 * s + 1] * w;
+        y += *reinterpret_cast<const f32x4 *>(o + s * kD) * w;
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // no key seen: zeros
+    *reinterpret_cast<u32x2 *>(out + row * kD + l4) =
+        u32x2{pack_bf16x2(y[0] * inv, y[1] * inv), pack_bf16x2(y[2] * inv, y[3] * inv)};
+}
+
+// The kernel of paged_attn.hip takes a workgroup for a row and spreads the parts over it: best for few rows or many parts
+// (16384 rows of 4 parts: 19.3 us there, 7.3 here; 6656 rows of 4 9.3 and 4.9; 512 of 4 4.8 either way).
+hipError_t launch_merge(const PagedAttnArgs &a, const float *ws_o, const float *ws_ml, int splits, hipStream_t stream) {
+    const int64_t rows = (int64_t)a.num_seqs * a.num_new_tokens * a.num_heads;
+    if (splits > 8 || rows < 1024) return launch_paged_attn_merge(ws_o, ws_ml, a.out, rows, splits, stream);
+    if (rows > 8 * 0x7fffffffLL) return hipErrorInvalidValue;
+    paged_attn_kv8_merge_kernel<<<dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, stream>>>(
+        ws_o, ws_ml, static_cast<__bf16 *>(a.out), rows, splits);
+    return hipGetLastError();
 }
 
 int blocks_per_split(const PagedAttnArgs &a, int splits, int granule) {
@@ -1126,9 +1159,7 @@ hipError_t launch_tile(const PagedAttnArgs &a, const float *ks, const float *vs,
             static_cast<__bf16 *>(a.out), ws_o, ws_ml, a.num_new_tokens, a.num_heads, a.num_kv_heads,
             a.max_blocks_per_seq, a.num_cache_blocks, a.scale, splits, blocks_per_split(a, splits, kBigBlocks));
     const hipError_t err = hipGetLastError();
-    if (err != hipSuccess || splits == 1) return err;
-    return launch_paged_attn_merge(ws_o, ws_ml, a.out, (int64_t)a.num_seqs * a.num_new_tokens * a.num_heads, splits,
-                                   stream);
+    return err != hipSuccess || splits == 1 ? err : launch_merge(a, ws_o, ws_ml, splits, stream);
 }
 
 template <Kv8Format F>
@@ -1189,9 +1220,7 @@ hipError_t launch_decode(const PagedAttnArgs &a, const float *ks, const float *v
     }
 #undef NVLLM_KV8_CASE
     const hipError_t err = hipGetLastError();
-    if (err != hipSuccess || splits == 1) return err;
-    return launch_paged_attn_merge(ws_o, ws_ml, a.out, (int64_t)a.num_seqs * a.num_new_tokens * a.num_heads, splits,
-                                   stream);
+    return err != hipSuccess || splits == 1 ? err : launch_merge(a, ws_o, ws_ml, splits, stream);
 }
 
 int splits_of(DType dt, const PagedAttnArgs &a) {
