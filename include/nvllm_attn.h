@@ -301,7 +301,8 @@ int nvllm_gather_cache_blocks_kv8(const void *k_cache, const void *v_cache, cons
                                   int dtype, nvllm_stream_t stream);
 
 /* nvllm_paged_attn_* over the 8-bit cache: same tables, lengths, mask, clamps and output; a query that
- * sees no key (context_len < num_new_tokens) gives zeros.  Scales may be any finite numbers >= 0.
+ * sees no key (context_len < num_new_tokens) gives zeros.  Scales may be any finite numbers >= 0
+ * (and a K scale times `scale` finite): outputs are finite wherever the values are.
  * `workspace` as there, sized by nvllm_paged_attn_kv8_workspace_bytes for the same shape and dtype
  * with the launch device current. */
 int nvllm_paged_attn_kv8(const void *q, const void *k_cache, const void *v_cache,

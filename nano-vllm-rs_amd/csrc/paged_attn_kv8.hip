@@ -35,6 +35,14 @@ __device__ __forceinline__ int pool_id(int id, int64_t num_cache_blocks) {
     return id < 0 ? 0 : (id > most ? most : id);
 }
 
+// A tile with a V scale of 2^64 or more takes its exponents from a reference at least kLift (a power of two) above the
+// row's maximum, so that there p <= 2^-32.  Then nothing overflows, whatever the finite scales: values are below 2^128 and
+// a walk has 2^30 keys at most, so these tiles' sums stay below 2^(30 - 32 + 128), and the others', whose p may be 2^8
+// (kSlack below) and whose codes are below 2^9, below 2^(30 + 8 + 64 + 9).  The output is divided by the sum of
+// the same p, so their size cancels; lost is what is below 2^-94, p of the largest p or p * scale.
+constexpr float kLift = 32.0f;
+constexpr float kLarge = 0x1p64f;
+
 constexpr int kAtOnce = 8;  // rows of V that a group of lanes has on their way
 
 // what lanes of the wave wrote to LDS before, lanes of it may read after
@@ -117,7 +125,7 @@ __global__ __launch_bounds__(64 * W) void paged_attn_kv8_generic_kernel(
             for (int d = 0; d < D; ++d) acc += q_s[d] * decode1<F>(k_cache[row + d]);
         }
         const float s = key < keys ? acc * (scale * ks) : -INFINITY;
-        const float m_new = fmaxf(m, wave_max(s));
+        const float m_new = fmaxf(m, wave_max(s) + (__any(vs >= kLarge) ? kLift * 0.6931472f : 0.0f));
         const float m_safe = m_new == -INFINITY ? 0.0f : m_new;  // keys that all score -inf weigh nothing
         const float alpha = expf(m - m_safe);
         const float p = key < keys ? expf(s - m_safe) : 0.0f;
@@ -276,6 +284,14 @@ __device__ __forceinline__ float quad_max(float x) {
 // Exponents are taken from a reference that moves only when a row's maximum has passed it by kSlack: p stays
 // below 2^8 (its rounding to bf16 is relative, the sums are f32), and most tiles rescale nothing.
 constexpr float kSlack = 8.0f;
+
+// whether one of a tile's (wave-uniform) V scales is large: their bits order as the numbers do, none being negative
+template <int N> __device__ __forceinline__ bool has_large(const float (&scales)[N]) {
+    int most = 0;
+#pragma unroll
+    for (int b = 0; b < N; ++b) most = max(most, __builtin_bit_cast(int, scales[b]));
+    return most >= __builtin_bit_cast(int, kLarge);
+}
 
 // A kv head's rows of a cache block as a buffer: 16 bytes of it at lane_offset + row_offset, zeros without a
 // memory access if `valid` is false.  Tiles past the end are "loaded" that way, so that every step of a loop
@@ -538,6 +554,8 @@ __global__ __launch_bounds__(64 * W, NQT <= 2 ? 2 : 1) void paged_attn_kv8_decod
             for (int b = 0; b < kTileBlocks; ++b) f[b] = 1.0f;
         }
         bf16x8 pf[NQT];
+        const bool lift = has_large(tl.vs);
+        const float slack = lift ? -kLift : kSlack, above = lift ? kLift : 0.0f;
 #pragma unroll
         for (int qt = 0; qt < NQT; ++qt) {
             float mx = -INFINITY;
@@ -545,8 +563,8 @@ __global__ __launch_bounds__(64 * W, NQT <= 2 ? 2 : 1) void paged_attn_kv8_decod
             for (int b = 0; b < kTileBlocks; ++b)  // factors are >= 0
                 mx = fmaxf(mx, f[b] * fmaxf(fmaxf(s[qt][b][0], s[qt][b][1]), fmaxf(s[qt][b][2], s[qt][b][3])));
             mx = quad_max(mx);
-            if (__any(mx > m_run[qt] + kSlack)) {
-                const float m_new = fmaxf(m_run[qt], mx);
+            if (__any(mx > m_run[qt] + slack)) {
+                const float m_new = fmaxf(m_run[qt], mx + above);
                 const float alpha = m_new == -INFINITY ? 1.0f : fast_exp2(m_run[qt] - m_new);
                 m_run[qt] = m_new;
                 l_run[qt] *= alpha;
@@ -885,8 +903,9 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kv8_tile_kernel(
             mx = fmaxf(mx, x * f[b]);
         }
         mx = half_max(mx);
-        if (__any(mx > m_ref + kSlack)) {
-            const float m_new = fmaxf(m_ref, mx);
+        const bool lift = has_large(sc.v);
+        if (__any(mx > m_ref + (lift ? -kLift : kSlack))) {
+            const float m_new = fmaxf(m_ref, mx + (lift ? kLift : 0.0f));
             const float alpha = m_new == -INFINITY ? 1.0f : fast_exp2(m_ref - m_new);
             m_ref = m_new;
             l_run *= alpha;
