@@ -37,8 +37,8 @@ __device__ __forceinline__ int pool_id(int id, int64_t num_cache_blocks) {
 
 // A tile with a V scale of 2^64 or more takes its exponents from a reference at least kLift (a power of two) above the
 // row's maximum, so that there p <= 2^-32.  Then nothing overflows, whatever the finite scales: values are below 2^128 and
-// a walk has 2^30 keys at most, so these tiles' sums stay below 2^(30 - 32 + 128), and the others', whose p may be 2^8
-// (kSlack below) and whose codes are below 2^9, below 2^(30 + 8 + 64 + 9).  The output is divided by the sum of
+// a walk has 2^30 keys at most, so these tiles' sums stay below 2^(30 - 32 + 128), and the others', whose p may be 2^15
+// (kSlack below) and whose codes are below 2^9, below 2^(30 + 15 + 64 + 9).  The output is divided by the sum of
 // the same p, so their size cancels; lost is what is below 2^-94, p of the largest p or p * scale.
 constexpr float kLift = 32.0f;
 constexpr float kLarge = 0x1p64f;
@@ -281,16 +281,20 @@ __device__ __forceinline__ float quad_max(float x) {
     return half_max(fmaxf(a, b));
 }
 
-// Exponents are taken from a reference that moves only when a row's maximum has passed it by kSlack: p stays
-// below 2^8 (its rounding to bf16 is relative, the sums are f32), and most tiles rescale nothing.
-constexpr float kSlack = 8.0f;
+// Weights and values go to the matrix unit in f16.  The codes of both formats times a scale that is a power of two from
+// 2^-15 to 2^5 are f16 numbers, so V is exact, and a weight is off by 2^-11 of itself.  f16 has little range; p therefore
+// uses it to its end: exponents are taken from a reference that is moved to kRoom below a row's maximum, and only when
+// that has passed it by kSlack, so that the largest p is 2^7 .. 2^15, most tiles rescale nothing, and a p that f16 does
+// not hold in full is off by 2^-32 of the largest.  (In bf16, which needs none of this, a weight is off by
+// 2^-8 and the output's error against 64 bits a third larger: 2.3e-3 for 1.7e-3.)
+// A tile with another scale ("wild": not a power of two, or outside that range) takes bf16 instead, p times scale and
+// the bare code; so does every tile after one that lifted the reference, where p is small.
+constexpr float kSlack = 15.0f, kRoom = 7.0f;
 
-// whether one of a tile's (wave-uniform) V scales is large: their bits order as the numbers do, none being negative
-template <int N> __device__ __forceinline__ bool has_large(const float (&scales)[N]) {
-    int most = 0;
-#pragma unroll
-    for (int b = 0; b < N; ++b) most = max(most, __builtin_bit_cast(int, scales[b]));
-    return most >= __builtin_bit_cast(int, kLarge);
+// whether a block of this V scale goes through f16
+__device__ __forceinline__ bool tame(float scale) {
+    const unsigned b = __builtin_bit_cast(unsigned, scale), lo = 0x38000000u, hi = 0x42000000u;  // 2^-15, 2^5
+    return b == 0 || (b - lo <= hi - lo && (b & 0x7fffffu) == 0);
 }
 
 // A kv head's rows of a cache block as a buffer: 16 bytes of it at lane_offset + row_offset, zeros without a
@@ -315,6 +319,7 @@ struct Run {
     int64_t num_cache_blocks;
     int id, id_n, id_nn;               // id_nn: as the table has it
     float ks, vs, ks_n, vs_n;          // _n: as loaded
+    unsigned long long wild, large;    // bit l: V scale of block base + l is not tame / is kLarge or more
 
     __device__ __forceinline__ int raw_id(int base) const {
         const int j = base + lane;
@@ -330,12 +335,18 @@ struct Run {
         id_nn = raw_id(base + 2 * kRun);
         ask_scales(id, ks, vs);
         if (base + lane >= end) ks = vs = 0.0f;
+        look();
         ask_scales(id_n, ks_n, vs_n);
+    }
+    __device__ __forceinline__ void look() {
+        wild = __ballot(!tame(vs));
+        large = __ballot(vs >= kLarge);
     }
     __device__ __forceinline__ void advance(int base) {  // base: the run that begins
         id = id_n;
         ks = base + lane < end ? ks_n : 0.0f;
         vs = base + lane < end ? vs_n : 0.0f;
+        look();
         id_n = pool_id(id_nn, num_cache_blocks);
         ask_scales(id_n, ks_n, vs_n);
         id_nn = raw_id(base + 2 * kRun);
@@ -367,6 +378,41 @@ template <Kv8Format F> __device__ __forceinline__ bf16x8 widen8(unsigned w0, uns
     return __builtin_bit_cast(bf16x8, r);
 }
 
+typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
+typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
+
+// a tame block's codes times its scale, exact; `two`: the scale twice, in f16
+__device__ __forceinline__ f16x2 twice(float scale) { return f16x2{(_Float16)scale, (_Float16)scale}; }
+template <Kv8Format F> __device__ __forceinline__ void scaled4(unsigned w, float scale, f16x2 two, f16x2 &a, f16x2 &b) {
+    if constexpr (F == Kv8Format::E4M3) {
+        a = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, scale, false));
+        b = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, scale, true));
+    } else {
+        // 0x6400 + u is 1024 + u; u = code + 128
+        const f16x2 off = two * (_Float16)-1152.0f;
+        const unsigned u = w ^ 0x80808080u;
+        a = __builtin_elementwise_fma(__builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)), two, off);
+        b = __builtin_elementwise_fma(__builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)), two, off);
+    }
+}
+template <Kv8Format F> __device__ __forceinline__ f16x8 scaled8(unsigned w0, unsigned w1, const float (&scale)[2], const f16x2 (&two)[2]) {
+    f16x2 x[4];
+    scaled4<F>(w0, scale[0], two[0], x[0], x[1]);
+    scaled4<F>(w1, scale[1], two[1], x[2], x[3]);
+    return __builtin_bit_cast(f16x8, x);
+}
+
+// weights as the matrix unit takes them, in either type
+__device__ __forceinline__ u32x4 halves(const float (&p)[8]) {
+    f16x8 r;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = (_Float16)p[i];
+    return __builtin_bit_cast(u32x4, r);
+}
+__device__ __forceinline__ u32x4 bfloats(const float (&p)[8]) {
+    return u32x4{pack_bf16x2(p[0], p[1]), pack_bf16x2(p[2], p[3]), pack_bf16x2(p[4], p[5]), pack_bf16x2(p[6], p[7])};
+}
+
 // hipcc leaves too few wait states between the last matrix instruction of a basic block and a read of
 // its result in the next one (seen here as wrong values of one accumulator register; tests/mfma_waits.py
 // finds such places in the assembly).  Behind code whose results leave a block: 8 wait states.
@@ -379,6 +425,7 @@ __device__ __forceinline__ void settle() {
 struct Tile {
     u32x4 k[kTileBlocks][2], v[kTileBlocks][2];  // [block][rows 0-7, 8-15]
     float ks[kTileBlocks], vs[kTileBlocks];      // wave-uniform
+    bool wild, large;                            // and so are these: goes through bf16; lifts the reference
 };
 
 // byte c of the result is 0xff where byte c of w is an E4M3 NaN (0x7f, 0xff)
@@ -457,8 +504,12 @@ __global__ __launch_bounds__(64 * W, NQT <= 2 ? 2 : 1) void paged_attn_kv8_decod
     const unsigned tr_sw = (unsigned)(tr_row & 7);
 
     Run run{table, k_scales + kvh, v_scales + kvh, Hkv, blk_end, lane, num_cache_blocks};
+    bool lifted = false;
     auto load_tile = [&](Tile &tl, int t) {
         const int j = (kTileBlocks * t) & (kRun - 1);
+        tl.large = (run.large >> j & ((1u << kTileBlocks) - 1)) != 0;
+        lifted |= tl.large;
+        tl.wild = (run.wild >> j & ((1u << kTileBlocks) - 1)) != 0 || lifted;
 #pragma unroll
         for (int b = 0; b < kTileBlocks; ++b) {
             tl.ks[b] = run.k_at(j + b);
@@ -486,11 +537,13 @@ __global__ __launch_bounds__(64 * W, NQT <= 2 ? 2 : 1) void paged_attn_kv8_decod
     const int first_masked = ctx - (T - 1);  // first key that some query row cannot see
     unsigned nan_seen = 0;                   // among the values of the tiles from there on
 
-    // A operand of P.V: 8 keys (4g .. 4g+3 of both blocks) of dim 16 dt + c
-    auto v_fragment = [&](int dt) -> bf16x8 {
+    // A operand of P.V, as codes: 8 keys (4g .. 4g+3 of both blocks) of dim 16 dt + c
+    auto v_codes = [&](int dt) -> i32x2 {
         typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
-        const i32x2 w =
-            __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i32x2 *)(lds_v + tr_base + 16u * ((unsigned)dt ^ tr_sw)));
+        return __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i32x2 *)(lds_v + tr_base + 16u * ((unsigned)dt ^ tr_sw)));
+    };
+    auto v_fragment = [&](int dt) -> bf16x8 {
+        const i32x2 w = v_codes(dt);
         return widen8<F>((unsigned)w[0], (unsigned)w[1]);
     };
     auto compute_tile = [&](Tile &tl, int t) {
@@ -553,9 +606,7 @@ __global__ __launch_bounds__(64 * W, NQT <= 2 ? 2 : 1) void paged_attn_kv8_decod
 #pragma unroll
             for (int b = 0; b < kTileBlocks; ++b) f[b] = 1.0f;
         }
-        bf16x8 pf[NQT];
-        const bool lift = has_large(tl.vs);
-        const float slack = lift ? -kLift : kSlack, above = lift ? kLift : 0.0f;
+        const float slack = tl.large ? -kLift : kSlack, above = tl.large ? kLift : -kRoom;
 #pragma unroll
         for (int qt = 0; qt < NQT; ++qt) {
             float mx = -INFINITY;
@@ -571,26 +622,53 @@ __global__ __launch_bounds__(64 * W, NQT <= 2 ? 2 : 1) void paged_attn_kv8_decod
 #pragma unroll
                 for (int dt = 0; dt < 8; ++dt) acc[qt][dt] *= alpha;
             }
+        }
+        // weights of a query tile (their sum goes into l_run)
+        const auto weights = [&](int qt, float (&p)[8]) {
             const float m_safe = m_run[qt] == -INFINITY ? 0.0f : m_run[qt];
-            float p[8], sum = 0.0f;
+            float sum = 0.0f;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 p[j] = fast_exp2(fmaf(s[qt][j >> 2][j & 3], f[j >> 2], -m_safe));
                 sum += p[j];
-                p[j] *= tl.vs[j >> 2];
             }
             l_run[qt] += sum;
-            // the matrix unit takes p in bf16: each weight off by 2^-8 at most, as the output's own rounding
-            pf[qt] = __builtin_bit_cast(bf16x8, u32x4{pack_bf16x2(p[0], p[1]), pack_bf16x2(p[2], p[3]),
-                                                      pack_bf16x2(p[4], p[5]), pack_bf16x2(p[6], p[7])});
+        };
+        float vs[kTileBlocks] = {tl.vs[0], tl.vs[1]};
+        if (__builtin_expect(tl.wild, 0)) {  // (here, so that nothing cuts the weights off from the f16 product: T = 12 276 -> 261 us)
+#pragma unroll
+            for (int qt = 0; qt < NQT; ++qt) {
+                float p[8];
+                weights(qt, p);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) p[j] *= vs[j >> 2];
+                const bf16x8 pw = __builtin_bit_cast(bf16x8, bfloats(p));
+#pragma unroll
+                for (int dt = 0; dt < 8; ++dt)
+                    acc[qt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v_fragment(dt), pw, acc[qt][dt], 0, 0, 0);
+                // nothing is left for the rest of the tile's work
+#pragma unroll
+                for (int j = 0; j < 8; ++j) s[qt][j >> 2][j & 3] = -INFINITY;
+            }
+            f[0] = f[1] = vs[0] = vs[1] = 1.0f;
+            settle();
+        }
+        u32x4 pf[NQT];
+#pragma unroll
+        for (int qt = 0; qt < NQT; ++qt) {
+            float p[8];
+            weights(qt, p);
+            pf[qt] = halves(p);
         }
         // O^T += V^T P^T
+        const f16x2 two[2] = {twice(vs[0]), twice(vs[1])};
 #pragma unroll
         for (int dt = 0; dt < 8; ++dt) {
-            const bf16x8 a = v_fragment(dt);
+            const i32x2 w = v_codes(dt);
+            const f16x8 a = scaled8<F>((unsigned)w[0], (unsigned)w[1], vs, two);
 #pragma unroll
             for (int qt = 0; qt < NQT; ++qt)
-                acc[qt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, pf[qt], acc[qt][dt], 0, 0, 0);
+                acc[qt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, __builtin_bit_cast(f16x8, pf[qt]), acc[qt][dt], 0, 0, 0);
         }
         settle();
     };
@@ -712,9 +790,9 @@ __global__ __launch_bounds__(64 * W, NQT <= 2 ? 2 : 1) void paged_attn_kv8_decod
 //   KG = 1: 128 rows, 32 a wave, every wave all 64 keys;
 //   KG = 2: 64 rows; waves 0, 1 take the first 32 keys of each tile and waves 2, 3 the others, so that the
 //           four SIMDs share the work of few rows; the two halves join through LDS at the end.
-// Codes come in as in the decode kernel, but are widened to bf16 ONCE for all rows on their way into LDS
+// Codes come in as in the decode kernel, but are widened ONCE for all rows on their way into LDS
 // (two buffers of K and V, one barrier a tile); two tiles are on their way, one in registers and one in LDS,
-// while one is multiplied.  S^T = K Q^T and O^T = V^T P^T with mfma_f32_32x32x16_bf16: a query row lives in the lanes
+// while one is multiplied.  S^T = K Q^T and O^T = V^T P^T with mfma_f32_32x32x16: a query row lives in the lanes
 // c and c + 32, P needs no lane movement.  LDS: row r, 16-byte chunk ch of K at position ch ^ (r & 15), of V
 // at ch ^ 2 (r & 7) (transposed reads of 4 rows x 16 dims).
 //
@@ -735,18 +813,21 @@ constexpr int kWideImage = kBigKeys * kWideRow;  // 16 KiB
 
 struct Scales {  // of a tile's blocks, wave-uniform
     float k[kBigBlocks], v[kBigBlocks];
+    float staged;      // V scale of the block that this wave stages
+    bool large;        // lifts the reference
 };
 
-template <Kv8Format F, int KG, bool STREAM>
-__global__ __launch_bounds__(256, 2) void paged_attn_kv8_tile_kernel(
+// One walk.  HALF: in f16; false, the same in all waves and with nothing written, if it met a wild scale: then the
+// workgroup begins again in bf16.  (Both in one loop, as the decode kernel has them: 256 x 2048 T = 16 270 us, so 257.)
+template <Kv8Format F, int KG, bool STREAM, bool HALF>
+__device__ __forceinline__ bool tile_walk(
+    unsigned char *lds, int &nan_seen,  // lds: [buffer][K, V]
     const __bf16 *__restrict__ q, const unsigned char *__restrict__ k_cache, const unsigned char *__restrict__ v_cache,
     const float *__restrict__ k_scales, const float *__restrict__ v_scales, const int32_t *__restrict__ block_tables,
     const int32_t *__restrict__ context_lens, __bf16 *__restrict__ out, float *__restrict__ ws_o,
     float *__restrict__ ws_ml, int T, int Hq, int Hkv, int max_blocks_per_seq, int64_t num_cache_blocks, float scale,
     int num_splits, int blocks_per_split) {
     constexpr int kRows = 128 / KG, NS = 2 / KG;  // rows of the workgroup; 32-key score tiles of a wave
-    __shared__ __attribute__((aligned(16))) unsigned char lds[4 * kWideImage];  // [buffer][K, V]
-    __shared__ int nan_seen;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int h = lane >> 5, c = lane & 31;
@@ -802,8 +883,12 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kv8_tile_kernel(
         vw[e] = (unsigned)(kWideImage + sr * kWideRow + 16 * ((2 * lch + e) ^ (2 * (sr & 7))));
     }
     Run run{table, k_scales + kvh, v_scales + kvh, Hkv, blk_end, lane, num_cache_blocks};
+    bool wild = false;
     auto load_tile = [&](int t, u32x4 (&ck)[2], u32x4 (&cv)[2], Scales &sc) {
         const int j = (kBigBlocks * t) & (kRun - 1);
+        wild |= (run.wild >> j & ((1u << kBigBlocks) - 1)) != 0;
+        sc.large = (run.large >> j & ((1u << kBigBlocks) - 1)) != 0;
+        sc.staged = run.v_at(j + sb);
 #pragma unroll
         for (int b = 0; b < kBigBlocks; ++b) {
             sc.k[b] = run.k_at(j + b);
@@ -817,10 +902,10 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kv8_tile_kernel(
         }
         if (j == kRun - kBigBlocks) run.advance(blk_begin + kBigBlocks * (t + 1));
     };
-    // codes of tile t -> bf16 in LDS.  V rows that no row of the tile sees are zeros, and so is a NaN that only some
-    // rows see (below)
+    // codes of tile t -> bf16 (HALF: V in f16) in LDS.  V rows that no row of the tile sees are zeros, and
+    // so is a NaN that only some rows see (below)
     unsigned nan_here = 0;
-    auto stage_tile = [&](int t, unsigned char *buf, u32x4 (&ck)[2], u32x4 (&cv)[2]) {
+    auto stage_tile = [&](int t, unsigned char *buf, u32x4 (&ck)[2], u32x4 (&cv)[2], const Scales &sc) {
         const int key0 = (blk_begin + kBigBlocks * t) * kBS;
         if (key0 + kBigKeys > keys_all) {
 #pragma unroll
@@ -841,7 +926,11 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kv8_tile_kernel(
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 *reinterpret_cast<bf16x8 *>(buf + (kw[e] ^ (i ? 128u : 0u)) + 8 * kWideRow * i) = widen8<F>(ck[i][2 * e], ck[i][2 * e + 1]);
-                *reinterpret_cast<bf16x8 *>(buf + vw[e] + 8 * kWideRow * i) = widen8<F>(cv[i][2 * e], cv[i][2 * e + 1]);
+                if constexpr (HALF)
+                    *reinterpret_cast<f16x8 *>(buf + vw[e] + 8 * kWideRow * i) =
+                        scaled8<F>(cv[i][2 * e], cv[i][2 * e + 1], {sc.staged, sc.staged}, {twice(sc.staged), twice(sc.staged)});
+                else
+                    *reinterpret_cast<bf16x8 *>(buf + vw[e] + 8 * kWideRow * i) = widen8<F>(cv[i][2 * e], cv[i][2 * e + 1]);
             }
     };
 
@@ -857,15 +946,16 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kv8_tile_kernel(
     const int vr = 4 * h + ((lane & 15) >> 2);
     const unsigned vch = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
     const unsigned vrd = (unsigned)(kWideImage + (32 * kg + vr) * kWideRow + 8 * (lane & 1));
-    auto v_fragment = [&](const unsigned char *buf, int key16, int dt) -> bf16x8 {
+    auto v_fragment = [&](const unsigned char *buf, int key16, int dt) -> u32x4 {
         typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
         const unsigned at = vrd + (unsigned)(16 * key16 * kWideRow) + 16 * ((4 * dt + vch) ^ (2 * (unsigned)(vr & 7)));
         const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(buf + at));
         const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(buf + at + 8 * kWideRow));
-        return __builtin_bit_cast(bf16x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+        return __builtin_bit_cast(u32x4, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
     };
 
     auto compute_tile = [&](int t, const unsigned char *buf, const Scales &sc) {
+        const bool large = !HALF && sc.large;
         const int key0 = (blk_begin + kBigBlocks * t) * kBS + 32 * kg;
         f32x16 s[NS];
 #pragma unroll
@@ -903,9 +993,8 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kv8_tile_kernel(
             mx = fmaxf(mx, x * f[b]);
         }
         mx = half_max(mx);
-        const bool lift = has_large(sc.v);
-        if (__any(mx > m_ref + (lift ? -kLift : kSlack))) {
-            const float m_new = fmaxf(m_ref, mx + (lift ? kLift : 0.0f));
+        if (__any(mx > m_ref + (large ? -kLift : kSlack))) {
+            const float m_new = fmaxf(m_ref, mx + (large ? kLift : -kRoom));
             const float alpha = m_new == -INFINITY ? 1.0f : fast_exp2(m_ref - m_new);
             m_ref = m_new;
             l_run *= alpha;
@@ -916,26 +1005,35 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kv8_tile_kernel(
         }
         const float m_safe = m_ref == -INFINITY ? 0.0f : m_ref;
         float sum = 0.0f;
-        bf16x8 pf[2 * NS];  // P^T as B operand, 16 keys each
+        u32x4 pf[2 * NS];  // P^T as B operand, 16 keys each
 #pragma unroll
         for (int b = 0; b < 2 * NS; ++b) {
-            const float v_scale = kg == 0 ? sc.v[b] : sc.v[kBigBlocks - 2 * NS + b];
             float p[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 p[i] = fast_exp2(fmaf(s[b / 2][8 * (b % 2) + i], f[b], -m_safe));
                 sum += p[i];
-                p[i] *= v_scale;
             }
-            pf[b] = __builtin_bit_cast(bf16x8, u32x4{pack_bf16x2(p[0], p[1]), pack_bf16x2(p[2], p[3]),
-                                                     pack_bf16x2(p[4], p[5]), pack_bf16x2(p[6], p[7])});
+            if constexpr (HALF) {
+                pf[b] = halves(p);
+            } else {
+                const float v_scale = kg == 0 ? sc.v[b] : sc.v[kBigBlocks - 2 * NS + b];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) p[i] *= v_scale;
+                pf[b] = bfloats(p);
+            }
         }
         l_run += sum;
 #pragma unroll
         for (int b = 0; b < 2 * NS; ++b)
 #pragma unroll
-            for (int dt = 0; dt < 4; ++dt)
-                acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v_fragment(buf, b, dt), pf[b], acc[dt], 0, 0, 0);
+            for (int dt = 0; dt < 4; ++dt) {
+                const u32x4 v = v_fragment(buf, b, dt);
+                if constexpr (HALF)
+                    acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, v), __builtin_bit_cast(f16x8, pf[b]), acc[dt], 0, 0, 0);
+                else
+                    acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, v), __builtin_bit_cast(bf16x8, pf[b]), acc[dt], 0, 0, 0);
+            }
         settle();
     };
     if (F == Kv8Format::E4M3 && threadIdx.x == 0) nan_seen = 0;
@@ -948,20 +1046,24 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kv8_tile_kernel(
             u32x4 k0[2], v0[2];
             load_tile(0, k0, v0, sc[0]);
             load_tile(1, ck, cv, sc[1]);
-            stage_tile(0, lds, k0, v0);
+            stage_tile(0, lds, k0, v0, sc[0]);
         }
-        for (int t0 = 0; t0 < ntiles; t0 += 2)
+        for (int t0 = 0; t0 < ntiles && !(HALF && wild); t0 += 2)
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 const int t = t0 + u;
                 __syncthreads();
-                stage_tile(t + 1, lds + (1 - u) * 2 * kWideImage, ck, cv);
+                stage_tile(t + 1, lds + (1 - u) * 2 * kWideImage, ck, cv, sc[1]);
                 Scales next;
                 load_tile(t + 2, ck, cv, next);
                 if (works && t < ntiles) compute_tile(t, lds + u * 2 * kWideImage, sc[0]);
                 sc[0] = sc[1];
                 sc[1] = next;
             }
+    }
+    if (__builtin_expect(HALF && wild, 0)) {  // all waves have seen all scales
+        __syncthreads();  // the images have been read
+        return false;
     }
     if constexpr (F == Kv8Format::E4M3) {
         __syncthreads();
@@ -1002,7 +1104,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kv8_tile_kernel(
                         f32x16 z;
 #pragma unroll
                         for (int i = 0; i < 16; ++i) z[i] = 0.0f;
-                        z = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v_fragment(lds, b, dt),
+                        z = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, v_fragment(lds, b, dt)),
                                                                     __builtin_bit_cast(bf16x8, see), z, 0, 0, 0);
 #pragma unroll
                         for (int i = 0; i < 16; ++i) acc[dt][i] = z[i] > 0.0f ? __builtin_nanf("") : acc[dt][i];
@@ -1079,6 +1181,24 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kv8_tile_kernel(
             ws_ml[2 * prow + 1] = l;
         }
     }
+    return true;
+}
+
+template <Kv8Format F, int KG, bool STREAM>
+__global__ __launch_bounds__(256, 2) void paged_attn_kv8_tile_kernel(
+    const __bf16 *__restrict__ q, const unsigned char *__restrict__ k_cache, const unsigned char *__restrict__ v_cache,
+    const float *__restrict__ k_scales, const float *__restrict__ v_scales, const int32_t *__restrict__ block_tables,
+    const int32_t *__restrict__ context_lens, __bf16 *__restrict__ out, float *__restrict__ ws_o,
+    float *__restrict__ ws_ml, int T, int Hq, int Hkv, int max_blocks_per_seq, int64_t num_cache_blocks, float scale,
+    int num_splits, int blocks_per_split) {
+    __shared__ __attribute__((aligned(16))) unsigned char lds[4 * kWideImage];
+    __shared__ int nan_seen;
+#define NVLLM_KV8_WALK(HALF)                                                                                          \
+    tile_walk<F, KG, STREAM, HALF>(lds, nan_seen, q, k_cache, v_cache, k_scales, v_scales, block_tables,             \
+                                   context_lens, out, ws_o, ws_ml, T, Hq, Hkv, max_blocks_per_seq, num_cache_blocks, \
+                                   scale, num_splits, blocks_per_split)
+    if (!NVLLM_KV8_WALK(true)) NVLLM_KV8_WALK(false);
+#undef NVLLM_KV8_WALK
 }
 
 bool fast_shape(DType dt, const PagedAttnArgs &a) {
