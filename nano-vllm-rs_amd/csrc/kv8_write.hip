@@ -140,7 +140,7 @@ __device__ __forceinline__ void write_unit(const int *map, int bs, int D, int Hk
         const int t = map[o];
         if (t < 0) continue;
         const auto x = row(t);
-        for (int d = lane; d < D; d += 64) amax = fmaxf(amax, finite_abs(x(d)));
+        for (int d = lane; d < D; d += 64) amax = fmaxf(amax, finite_abs(narrow_odd(x(d))));  // past a border stays past it
     }
     const float need = scale_of<F>(wave_max(amax));
     const bool begins = map[0] >= 0;
