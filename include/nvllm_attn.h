@@ -261,7 +261,7 @@ int nvllm_qk_norm_rope_cache_f32(const void *q, const void *k, const void *v, vo
  * 0 in int8; what is infinite or beyond 2^127 saturates and takes no part in the scale.
  * The slot mapping may name slots in any order; of tokens that name the same slot the last one is
  * written; a negative slot, or one past the pool, skips its token.  Two calls that run at the same
- * time must not write the same block. */
+ * time must not write the same block, and a call's K and V caches (and their scales) must not overlap. */
 
 /* Workspace of the two writers below: 0 up to 1024 tokens, else 4 bytes per slot of the pool.  Its
  * contents need no preparation and mean nothing between calls; calls that overlap in time need one
@@ -277,8 +277,8 @@ int nvllm_reshape_and_cache_kv8(const void *key, const void *value, void *k_cach
                                 nvllm_stream_t stream);
 
 /* nvllm_qk_norm_rope_cache_* with quantisation: the rotated K and V go into the 8-bit cache, K computed in
- * f64 and rounded once (not by way of k_out); q_out and k_out in f32.  q_out may be q; neither it
- * nor k_out (optional) may overlap k or v. */
+ * f64 and rounded once (not by way of k_out); q_out and k_out in f32.  q_out is q, or overlaps none
+ * of q, k and v; k_out (optional) overlaps none of them, nor q_out (else NVLLM_ERR_CONFIG). */
 int nvllm_qk_norm_rope_cache_kv8(const void *q, const void *k, const void *v, void *q_out,
                                  void *k_out, const void *q_weight, const void *k_weight, float eps,
                                  const void *cos_cache, const void *sin_cache,

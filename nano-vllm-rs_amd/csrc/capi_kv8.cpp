@@ -66,6 +66,10 @@ int write_common(const char *who, const kernels::Kv8WriteArgs &a, size_t workspa
     }
     if (need > 0 && !aligned(a.workspace, 16))
         return fail(ErrorKind::Config, who, "workspace must be 16-byte aligned");
+    // K and V of a block are written by different waves
+    const std::int64_t scales = a.num_cache_blocks * a.num_kv_heads * 4, codes = scales / 4 * a.block_size * a.head_dim;
+    if (overlap(a.k_cache, codes, a.v_cache, codes) || overlap(a.k_scales, scales, a.v_scales, scales))
+        return fail(ErrorKind::Config, who, "caches of K and V must not overlap, nor their scales");
     return hip_status(kernels::launch_kv8_write(static_cast<kernels::DType>(dtype),
                                                 static_cast<kernels::Kv8Format>(format), a, as_stream(stream)),
                       who);
@@ -128,7 +132,7 @@ int nvllm_qk_norm_rope_cache_kv8(const void *q, const void *k, const void *v, vo
     for (const void *p : {q, (const void *)q_out, (const void *)k_out, q_weight, k_weight, cos_cache, sin_cache})
         if (!aligned(p, elt)) return fail(ErrorKind::Config, who, "pointer not aligned to its element type");
     if (!aligned(positions, 4)) return fail(ErrorKind::Config, who, "pointer not aligned to its element type");
-    // other waves read the rows of k and v while these are written
+    // other waves read rows of q, k and v while these are written
     const int64_t kv_bytes = num_tokens * num_kv_heads * head_dim * elt, q_bytes = num_tokens * num_heads * head_dim * elt;
     for (const void *p : {k, v}) {
         if (p && k_out && overlap(k_out, kv_bytes, p, kv_bytes))
@@ -136,6 +140,10 @@ int nvllm_qk_norm_rope_cache_kv8(const void *q, const void *k, const void *v, vo
         if (p && overlap(q_out, q_bytes, p, kv_bytes))
             return fail(ErrorKind::Config, who, "q_out must not overlap k or v");
     }
+    if (q_out != q && overlap(q_out, q_bytes, q, q_bytes))
+        return fail(ErrorKind::Config, who, "q_out must be q or not overlap it");
+    if (k_out && (overlap(k_out, kv_bytes, q, q_bytes) || overlap(k_out, kv_bytes, q_out, q_bytes)))
+        return fail(ErrorKind::Config, who, "k_out must not overlap q or q_out");
     kernels::Kv8WriteArgs a{};
     a.key = k;
     a.value = v;

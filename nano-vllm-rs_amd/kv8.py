@@ -108,7 +108,8 @@ def reshape_and_cache_kv8(key, value, key_cache, value_cache, key_scales, value_
 def qk_norm_rope_cache_kv8(query, key, value, q_weight, k_weight, eps, rotary, positions, key_cache, value_cache,
                            key_scales, value_scales, slot_mapping, k_out=None, q_out=None, workspace=None):
     """nvllm_qk_norm_rope_cache_kv8: `qk_norm_rope_cache` with the rotated K and V going into the 8-bit
-    cache.  k_out must not overlap key or value, nor q_out.  Returns q_out (query itself unless q_out is given)."""
+    cache.  q_out is query or overlaps none of query, key and value; k_out overlaps none of the four.  Returns q_out
+    (query itself unless q_out is given)."""
     nb, bs, hkv, d, fmt = _cache(key_cache, value_cache, key_scales, value_scales)
     n, hq = query.shape[0], query.shape[1]
     if query.shape != (n, hq, d) or key.shape != (n, hkv, d) or value.shape != key.shape:
