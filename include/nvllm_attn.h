@@ -250,7 +250,8 @@ int nvllm_qk_norm_rope_cache_f32(const void *q, const void *k, const void *v, vo
  *   value = code * scale
  * format 0 = int8: codes are integers in -127 .. 127; format 1 = E4M3 (OCP): codes are its numbers,
  * +-448 at most.  dtype (0 bf16, 1 f32) is that of the other tensors.  head_dim <= 256, block_size <=
- * 256.  A fresh cache is all zeros, codes and scales.
+ * 256; the writers take up to 2^30 tokens and 65535 heads.  A cache needs no initialisation where every
+ * block begins with a write of its row 0 (below); LayerKVCache's is all zeros, codes and scales.
  *
  * What a write does to a block.  Scales are powers of two, the smallest with max|x| <= top * scale
  * (top 127 or 448; 0 for zeros; 2^-126 at least).  A call that writes the block's row 0 BEGINS the

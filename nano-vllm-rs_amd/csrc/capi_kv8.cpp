@@ -48,6 +48,13 @@ int check_cache(const char *who, std::int64_t num_cache_blocks, int block_size, 
     return NVLLM_OK;
 }
 
+// what the writers count in 32 bits: tokens, and the pairs of block and head of 16 blocks
+int check_writer(const char *who, std::int64_t num_tokens, int num_heads, int num_kv_heads) {
+    if (num_heads > 65535 || num_kv_heads > 65535) return fail(ErrorKind::Unsupported, who, "more than 65535 heads");
+    if (num_tokens > (1 << 30)) return fail(ErrorKind::Unsupported, who, "more than 2^30 tokens");
+    return NVLLM_OK;
+}
+
 int write_common(const char *who, const kernels::Kv8WriteArgs &a, size_t workspace_bytes, int format, int dtype,
                  nvllm_stream_t stream) {
     if (!a.key || !a.value || !a.k_cache || !a.v_cache || !a.k_scales || !a.v_scales || !a.slot_mapping)
@@ -92,7 +99,7 @@ int nvllm_reshape_and_cache_kv8(const void *key, const void *value, void *k_cach
     static const char *who = "reshape_and_cache_kv8";
     if (num_tokens < 0) return fail(ErrorKind::Config, who, "negative or zero dimension");
     if (const int rc = check_cache(who, num_cache_blocks, block_size, num_kv_heads, head_dim, format, dtype)) return rc;
-    if (num_tokens > (1 << 30)) return fail(ErrorKind::Unsupported, who, "more than 2^30 tokens");
+    if (const int rc = check_writer(who, num_tokens, 0, num_kv_heads)) return rc;
     if (num_tokens == 0) return NVLLM_OK;
     kernels::Kv8WriteArgs a{};
     a.key = key;
@@ -122,9 +129,9 @@ int nvllm_qk_norm_rope_cache_kv8(const void *q, const void *k, const void *v, vo
     if (num_tokens < 0 || num_heads <= 0 || max_positions <= 0 || max_positions > 0x7fffffff)
         return fail(ErrorKind::Config, who, "negative or zero dimension");
     if (const int rc = check_cache(who, num_cache_blocks, block_size, num_kv_heads, head_dim, format, dtype)) return rc;
+    if (const int rc = check_writer(who, num_tokens, num_heads, num_kv_heads)) return rc;
     if (head_dim % 2 != 0)  // rope.rs:49 assert!(dim.is_multiple_of(2))
         return fail(ErrorKind::Config, who, "RoPE dimension must be even");
-    if (num_tokens > (1 << 30)) return fail(ErrorKind::Unsupported, who, "more than 2^30 tokens");
     if (num_tokens == 0) return NVLLM_OK;
     if (!q || !q_out || !q_weight || !k_weight || !cos_cache || !sin_cache || !positions)
         return fail(ErrorKind::Null, who, "null pointer");
@@ -179,6 +186,7 @@ int nvllm_gather_cache_blocks_kv8(const void *k_cache, const void *v_cache, cons
     static const char *who = "gather_cache_blocks_kv8";
     if (num_ids <= 0)  // kv_cache.rs:124-126
         return fail(ErrorKind::Config, who, "block_ids cannot be empty");
+    if (num_ids > 0x7fffffff) return fail(ErrorKind::Unsupported, who, "more than 2^31 - 1 block_ids");
     if (const int rc = check_cache(who, num_cache_blocks, block_size, num_kv_heads, head_dim, format, dtype)) return rc;
     if (!k_cache || !k_scales || !block_ids || !k_out || (v_out && (!v_cache || !v_scales)))
         return fail(ErrorKind::Null, who, "null pointer");
