@@ -1,9 +1,10 @@
 """Walks gfx950 assembly and lists the places where a matrix instruction's result is touched too soon.
 
 The hardware does not hold back a vector instruction that reads or overwrites the result of a matrix
-instruction still in flight: the compiler has to keep passes + 3 wait states between them (4 passes for
-16x16x32 bf16, 8 for 32x32x16; every instruction counts for one, s_nop n for n + 1).  hipcc has been seen
-to miss that across the end of a basic block, so this follows every path, through branches.
+instruction still in flight: the compiler has to keep passes + 4 wait states between them (passes + 3 on the
+parts before gfx950; 4 passes for 16x16x32 bf16, 8 for 32x32x16; every instruction counts for one, s_nop n
+for n + 1).  hipcc has been seen to miss that across the end of a basic block, so this follows every path,
+through branches.
 
   python mfma_waits.py FILE.s      exit status 1 if there is such a place"""
 import re
@@ -64,7 +65,7 @@ def violations(body):
         if not line.startswith("v_mfma"):
             continue
         shape = re.search(r"_(\d+x\d+x\d+)_?", line).group(1)
-        need = PASSES[shape] + 3
+        need = PASSES[shape] + 4
         dst = registers(line.split(None, 1)[1].split(",")[0])
         todo, seen = [(n, 0) for n in successors(i)], {}
         while todo:
