@@ -70,14 +70,16 @@ __global__ __launch_bounds__(256) void qk_norm_rope_cache_d128_kernel(
     const __bf16 *__restrict__ k_weight, float eps, const __bf16 *__restrict__ cos_cache,
     const __bf16 *__restrict__ sin_cache, int max_pos, const int32_t *__restrict__ positions,
     __bf16 *__restrict__ k_cache, __bf16 *__restrict__ v_cache,
-    const int64_t *__restrict__ slot_mapping, int64_t num_rows, int Hq, int Hkv,
+    const int64_t *__restrict__ slot_mapping, unsigned num_rows, int Hq, int Hkv,
     int64_t num_slots) {
-    constexpr int D = 128;
+    constexpr int64_t D = 128;
     const int li = threadIdx.x & 7;
-    const int64_t row = (int64_t)blockIdx.x * kRowsPerBlock + (threadIdx.x >> 3);
+    // rows are counted in 32 bits (a terabyte of them): with 64-bit division and products of indexes the kernel has 591
+    // instructions instead of 408, and 32768 tokens take 137.4 us instead of 131.4 (6.26 TB/s)
+    const unsigned row = blockIdx.x * kRowsPerBlock + (threadIdx.x >> 3);
     if (row >= num_rows) return;  // whole 8-lane groups leave together
-    const int R = Hq + 2 * Hkv;
-    const int64_t tok = row / R;
+    const unsigned R = Hq + 2 * Hkv;
+    const unsigned tok = row / R;
     const int j = (int)(row - tok * R);
     const int off_lo = 8 * li, off_hi = 64 + 8 * li;
 
@@ -85,7 +87,7 @@ __global__ __launch_bounds__(256) void qk_norm_rope_cache_d128_kernel(
         const int hv = j - Hq - Hkv;
         const int64_t slot = slot_mapping[tok];
         if (slot < 0 || slot >= num_slots) return;
-        const __bf16 *src = v + (tok * Hkv + hv) * D;
+        const __bf16 *src = v + (unsigned)(tok * Hkv + hv) * D;
         __bf16 *dst = v_cache + (slot * Hkv + hv) * D;
         const u32x4 lo = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(src + off_lo));
         const u32x4 hi = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(src + off_hi));
@@ -95,7 +97,8 @@ __global__ __launch_bounds__(256) void qk_norm_rope_cache_d128_kernel(
     }
     const bool is_q = j < Hq;
     const int hk = j - Hq;
-    const __bf16 *src = is_q ? q + (tok * Hq + j) * D : k + (tok * Hkv + hk) * D;
+    const int64_t at = (unsigned)(is_q ? tok * Hq + j : tok * Hkv + hk) * D;
+    const __bf16 *src = (is_q ? q : k) + at;
     const __bf16 *w = is_q ? q_weight : k_weight;
     int pos = positions[tok];
     pos = pos < 0 ? 0 : (pos >= max_pos ? max_pos - 1 : pos);  // never read outside the tables
@@ -124,7 +127,7 @@ __global__ __launch_bounds__(256) void qk_norm_rope_cache_d128_kernel(
     for (int i = 0; i < 8; ++i) ss += x1[i] * x1[i] + x2[i] * x2[i];
 #pragma unroll
     for (int m = 1; m < 8; m <<= 1) ss += __shfl_xor(ss, m);
-    const float inv = 1.0f / sqrtf(ss * (1.0f / D) + eps);
+    const float inv = 1.0f / sqrtf(ss * (1.0f / (float)D) + eps);
     u32x4 olo, ohi;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -140,12 +143,12 @@ __global__ __launch_bounds__(256) void qk_norm_rope_cache_d128_kernel(
         ohi[i] = pack_bf16x2(y2[0], y2[1]);
     }
     if (is_q) {
-        __bf16 *dst = q_out + (tok * Hq + j) * D;
+        __bf16 *dst = q_out + at;
         st16<NT>(dst + off_lo, olo);
         st16<NT>(dst + off_hi, ohi);
     } else {
         if (k_out) {
-            __bf16 *dst = k_out + (tok * Hkv + hk) * D;
+            __bf16 *dst = k_out + at;
             st16<NT>(dst + off_lo, olo);
             st16<NT>(dst + off_hi, ohi);
         }
@@ -225,8 +228,8 @@ hipError_t launch_qk_norm_rope_cache(DType dt, const QkNormRopeCacheArgs &a, hip
     const int64_t rows = a.num_tokens * (a.num_heads + 2 * a.num_kv_heads);
     const int64_t num_slots = a.num_cache_blocks * a.block_size;
     const auto al8 = [](const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; };
-    if (dt == DType::BF16 && a.head_dim == 128 && al8(a.q) && al8(a.k) && al8(a.v) && al8(a.q_out) &&
-        al8(a.k_out) && al8(a.q_weight) && al8(a.k_weight) && al8(a.cos_cache) &&
+    if (dt == DType::BF16 && a.head_dim == 128 && rows + kRowsPerBlock <= 0xffffffffLL && al8(a.q) &&
+        al8(a.k) && al8(a.v) && al8(a.q_out) && al8(a.k_out) && al8(a.q_weight) && al8(a.k_weight) && al8(a.cos_cache) &&
         al8(a.sin_cache) && al8(a.k_cache) && al8(a.v_cache)) {
         const dim3 grid((unsigned)((rows + kRowsPerBlock - 1) / kRowsPerBlock)), block(256);
         constexpr int64_t kStreamTokens = 2048;  // >= 48 MiB of outputs at Qwen3-4B shapes
@@ -237,7 +240,7 @@ hipError_t launch_qk_norm_rope_cache(DType dt, const QkNormRopeCacheArgs &a, hip
                 static_cast<__bf16 *>(a.k_out), static_cast<const __bf16 *>(a.q_weight),
                 static_cast<const __bf16 *>(a.k_weight), a.eps, static_cast<const __bf16 *>(a.cos_cache),
                 static_cast<const __bf16 *>(a.sin_cache), a.max_positions, a.positions,
-                static_cast<__bf16 *>(a.k_cache), static_cast<__bf16 *>(a.v_cache), a.slot_mapping, rows,
+                static_cast<__bf16 *>(a.k_cache), static_cast<__bf16 *>(a.v_cache), a.slot_mapping, (unsigned)rows,
                 a.num_heads, a.num_kv_heads, num_slots);
         else
             qk_norm_rope_cache_d128_kernel<false><<<grid, block, 0, stream>>>(
@@ -246,7 +249,7 @@ hipError_t launch_qk_norm_rope_cache(DType dt, const QkNormRopeCacheArgs &a, hip
                 static_cast<__bf16 *>(a.k_out), static_cast<const __bf16 *>(a.q_weight),
                 static_cast<const __bf16 *>(a.k_weight), a.eps, static_cast<const __bf16 *>(a.cos_cache),
                 static_cast<const __bf16 *>(a.sin_cache), a.max_positions, a.positions,
-                static_cast<__bf16 *>(a.k_cache), static_cast<__bf16 *>(a.v_cache), a.slot_mapping, rows,
+                static_cast<__bf16 *>(a.k_cache), static_cast<__bf16 *>(a.v_cache), a.slot_mapping, (unsigned)rows,
                 a.num_heads, a.num_kv_heads, num_slots);
         return hipGetLastError();
     }
