@@ -37,8 +37,8 @@ __device__ __forceinline__ int pool_id(int id, int64_t num_cache_blocks) {
 
 // A tile with a V scale of 2^64 or more takes its exponents from a reference at least kLift (a power of two) above the
 // row's maximum, so that there p <= 2^-32.  Then nothing overflows, whatever the finite scales: values are below 2^128 and
-// a walk has 2^30 keys at most, so these tiles' sums stay below 2^(30 - 32 + 128), and the others', whose p may be 2^15
-// (kSlack below) and whose codes are below 2^9, below 2^(30 + 15 + 64 + 9).  The output is divided by the sum of
+// a walk has 2^30 keys at most, so these tiles' sums stay below 2^(30 - 32 + 128), and the others', whose p may be 2^14
+// (kSlack below) and whose codes are below 2^9, below 2^(30 + 14 + 64 + 9).  The output is divided by the sum of
 // the same p, so their size cancels; lost is what is below 2^-94, p of the largest p or p * scale.
 constexpr float kLift = 32.0f;
 constexpr float kLarge = 0x1p64f;
@@ -281,20 +281,28 @@ __device__ __forceinline__ float quad_max(float x) {
     return half_max(fmaxf(a, b));
 }
 
-// Weights and values go to the matrix unit in f16.  The codes of both formats times a scale that is a power of two from
-// 2^-15 to 2^5 are f16 numbers, so V is exact, and a weight is off by 2^-11 of itself.  f16 has little range; p therefore
-// uses it to its end: exponents are taken from a reference that is moved to kRoom below a row's maximum, and only when
-// that has passed it by kSlack, so that the largest p is 2^7 .. 2^15, most tiles rescale nothing, and a p that f16 does
-// not hold in full is off by 2^-32 of the largest.  (In bf16, which needs none of this, a weight is off by
-// 2^-8 and the output's error against 64 bits a third larger: 2.3e-3 for 1.7e-3.)
-// A tile with another scale ("wild": not a power of two, or outside that range) takes bf16 instead, p times scale and
-// the bare code; so does every tile after one that lifted the reference, where p is small.
-constexpr float kSlack = 15.0f, kRoom = 7.0f;
+// Weights and values go to the matrix unit in f16.  The codes of both formats times a power of two from 2^-15 to 2^5 are
+// f16 numbers, so V is exact, and a weight is off by 2^-11 of itself.  f16 has little range; p therefore uses it to
+// its end: exponents are taken from a reference that is moved to kRoom below a row's maximum, and only when that has
+// passed it by kSlack, so that the largest p is 2^7 .. 2^14, most tiles rescale nothing, and a p that f16 does not hold
+// in full is off by 2^-32 of the largest.  (In bf16, which needs none of this, a weight is off by 2^-8 and the
+// output's error against 64 bits a third larger: 2.3e-3 for 1.7e-3.)
+// A V scale that is no power of two (no write makes one): the decode kernel multiplies p by its fraction, 1 .. 2 (to 2^15).
+// A tile with a scale out of the range ("wild"; to the tile kernel one that is no power of two, too) takes bf16 instead, p
+// times scale and the bare code; so does every tile after one that lifted the reference, where p is small.
+constexpr float kSlack = 14.0f, kRoom = 7.0f;
 
 // whether a block of this V scale goes through f16
-__device__ __forceinline__ bool tame(float scale) {
-    const unsigned b = __builtin_bit_cast(unsigned, scale), lo = 0x38000000u, hi = 0x42000000u;  // 2^-15, 2^5
-    return b == 0 || (b - lo <= hi - lo && (b & 0x7fffffu) == 0);
+template <bool POWERS> __device__ __forceinline__ bool tame(float scale) {
+    const unsigned b = __builtin_bit_cast(unsigned, scale), lo = 0x38000000u, hi = 0x42800000u;  // 2^-15, 2^6
+    return b == 0 || (b - lo < hi - lo && (!POWERS || (b & 0x7fffffu) == 0));
+}
+// scale = power * fraction, 1 <= fraction < 2 (a scale of 0: power 0)
+__device__ __forceinline__ float power_of(float scale) {
+    return __builtin_bit_cast(float, __builtin_bit_cast(unsigned, scale) & 0xff800000u);
+}
+__device__ __forceinline__ float fraction_of(float scale) {
+    return __builtin_bit_cast(float, (__builtin_bit_cast(unsigned, scale) & 0x7fffffu) | 0x3f800000u);
 }
 
 // A kv head's rows of a cache block as a buffer: 16 bytes of it at lane_offset + row_offset, zeros without a
@@ -312,7 +320,7 @@ template <bool STREAM> __device__ __forceinline__ u32x4 load16(Rows rows, unsign
 // A wave's view of its part of a block table: lane l holds id and scales of block `base + l` of a run of 64, and
 // the next run's are on their way.  What is loaded is looked at (clamped, masked) only when its run begins, so
 // that nothing waits for it before.  Past the part's end: the last id (read, and masked), scale 0.
-struct Run {
+template <bool POWERS> struct Run {
     const int32_t *table;
     const float *k_scales, *v_scales;  // of the kv head: + Hkv * id
     int Hkv, end, lane;
@@ -339,7 +347,7 @@ struct Run {
         ask_scales(id_n, ks_n, vs_n);
     }
     __device__ __forceinline__ void look() {
-        wild = __ballot(!tame(vs));
+        wild = __ballot(!tame<POWERS>(vs));
         large = __ballot(vs >= kLarge);
     }
     __device__ __forceinline__ void advance(int base) {  // base: the run that begins
@@ -503,7 +511,7 @@ __global__ __launch_bounds__(64 * W, NQT <= 2 ? 2 : 1) void paged_attn_kv8_decod
     const unsigned tr_base = (unsigned)(tr_row * kD + 8 * (c & 1));
     const unsigned tr_sw = (unsigned)(tr_row & 7);
 
-    Run run{table, k_scales + kvh, v_scales + kvh, Hkv, blk_end, lane, num_cache_blocks};
+    Run<false> run{table, k_scales + kvh, v_scales + kvh, Hkv, blk_end, lane, num_cache_blocks};
     bool lifted = false;
     auto load_tile = [&](Tile &tl, int t) {
         const int j = (kTileBlocks * t) & (kRun - 1);
@@ -654,13 +662,18 @@ __global__ __launch_bounds__(64 * W, NQT <= 2 ? 2 : 1) void paged_attn_kv8_decod
             settle();
         }
         u32x4 pf[NQT];
+        const float fraction[kTileBlocks] = {fraction_of(vs[0]), fraction_of(vs[1])};
 #pragma unroll
         for (int qt = 0; qt < NQT; ++qt) {
             float p[8];
             weights(qt, p);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) p[j] *= fraction[j >> 2];
             pf[qt] = halves(p);
         }
         // O^T += V^T P^T
+        vs[0] = power_of(vs[0]);
+        vs[1] = power_of(vs[1]);
         const f16x2 two[2] = {twice(vs[0]), twice(vs[1])};
 #pragma unroll
         for (int dt = 0; dt < 8; ++dt) {
@@ -882,7 +895,7 @@ __device__ __forceinline__ bool tile_walk(
         kw[e] = (unsigned)(sr * kWideRow + 16 * ((2 * lch + e) ^ (sr & 15)));
         vw[e] = (unsigned)(kWideImage + sr * kWideRow + 16 * ((2 * lch + e) ^ (2 * (sr & 7))));
     }
-    Run run{table, k_scales + kvh, v_scales + kvh, Hkv, blk_end, lane, num_cache_blocks};
+    Run<true> run{table, k_scales + kvh, v_scales + kvh, Hkv, blk_end, lane, num_cache_blocks};
     bool wild = false;
     auto load_tile = [&](int t, u32x4 (&ck)[2], u32x4 (&cv)[2], Scales &sc) {
         const int j = (kBigBlocks * t) & (kRun - 1);

@@ -84,7 +84,8 @@ def test_one_key_takes_nearly_all_the_weight(dev, fmt, T, below, sink):
 @pytest.mark.parametrize("T", TOKENS)
 @pytest.mark.parametrize("every", [1, 9])
 def test_scales_that_are_no_powers_of_two(dev, fmt, T, every):
-    """from a calibration: all blocks, or some of them; the weights times scale are then rounded to bf16"""
+    """from a calibration: all blocks, or some of them.  The decode kernel weighs as finely there (48 query rows a kv head
+    at most); the tile kernel rounds weights times scale to bf16"""
     rng = np.random.default_rng(T + every)
     on, host = make(rng, fmt, "bf16", [T, 1700, 333 + T], T, 8, 2, 128, 16, dev)
     vs, tables = host[4], host[5]
@@ -92,4 +93,4 @@ def test_scales_that_are_no_powers_of_two(dev, fmt, T, every):
         for j in range(every // 2, -(-n // 16), every):
             vs[tables[i, j]] = np.float32(rng.uniform(0.001, 0.1, 2))
     set_cache(on, fmt, vs=vs)
-    compare_fine(call(on, 128 ** -0.5), host, 128 ** -0.5, weight=2.0 ** -8)
+    compare_fine(call(on, 128 ** -0.5), host, 128 ** -0.5, weight=2.0 ** (-11 if 4 * T <= 48 else -8))
