@@ -280,8 +280,8 @@ hipError_t launch_generic(const Kv8WriteArgs &a, bool indexed, hipStream_t strea
 // A wave takes one (block, kv head) of K or V: 8 lanes a row, two rows a lane (o and o + 8), so the block is
 // read with four 16-byte loads a lane, its maximum found with six shuffles and written with two 16-byte
 // stores, all rows of the block at once.  Of a block that gets one or two rows (a decode step) a wave takes
-// eight heads instead, 8 lanes those of one head: the producer's decode step of 256 (32 and 8 heads) 9.4 -> 6.3
-// us, of 1024 30 -> 11.4.  `parts` workgroups share a chunk's units, so that few tokens still spread over the chip.
+// eight heads instead, 8 lanes those of one head: the producer's decode step of 256 (32 and 8 heads) 10.3 -> 7.3
+// us, of 1024 28.2 -> 12.5 (in a kernel trace).  `parts` workgroups share a chunk's units, so that few tokens still spread over the chip.
 // ---------------------------------------------------------------------------
 constexpr int kFastD = 128;
 constexpr int kFastBS = 16;

@@ -810,8 +810,8 @@ __global__ __launch_bounds__(64 * W, NQT <= 2 ? 2 : 1) void paged_attn_kv8_decod
 // at ch ^ 2 (r & 7) (transposed reads of 4 rows x 16 dims).
 //
 // Bounds: with many rows the products and, between them, the exponentials (chunk of 4 x 1024 rows behind 7168 keys,
-// 2.6e11 operations: 275 us, 940 TFLOP/s); with few the loads (64 x 4096 T = 13, 537 MB: 121 us, 4.4 TB/s; the loads
-// alone 110) and a workgroup's start and end (256 x 64 T = 16: 35 us of the 248 of 256 x 2048).  Two to four tiles in
+// 2.6e11 operations: 273 to 280 us, 920 to 945 TFLOP/s); with few the loads (64 x 4096 T = 13, 537 MB: 117 us, 4.6 TB/s;
+// the loads alone 110) and a workgroup's start and end (256 x 64 T = 16: 35 us of the 256 of 256 x 2048).  Two to four tiles in
 // registers instead of one, three workgroups a CU, other orders of the workgroups, 8-byte staging with half the LDS
 // conflicts and products interleaved with the exponentials by hand were each within 3 % or slower.
 // ---------------------------------------------------------------------------
@@ -1291,7 +1291,7 @@ int blocks_per_split(const PagedAttnArgs &a, int splits, int granule) {
 }
 
 // Loads that do not stay in the caches, unless what the tables reach fits the 256 MiB Infinity Cache, or other
-// workgroups read the keys too (more than one tile of rows).  64 x 4096 T = 13 (1 GiB) 134 us without, 123 with; a chunk
+// workgroups read the keys too (more than one tile of rows).  64 x 4096 T = 13 (512 MiB) 134 us without, 123 with; a chunk
 // of 4 x 1024 rows behind 7168 keys 276 without, 281 with.
 bool streams(const PagedAttnArgs &a) {
     return (int64_t)a.num_seqs * a.max_blocks_per_seq * 2 * kBS * a.num_kv_heads * kD > ((int64_t)256 << 20);

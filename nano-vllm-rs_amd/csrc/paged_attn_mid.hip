@@ -343,7 +343,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_attn_mid_kernel(
     };
     // p (bf16 pairs) of score elements e0 .. e0 + n - 1 (e < 16: sa, else sb), their sum added to psum
     auto exp_n = [&](const f32x16 &sa, const f32x16 &sb, int e0, int n, float mc, u32x4 (&pd)[4], f32x2 &psum2) {
-        // (two scores at a time: the scale-and-shift and the row sum as packed f32 instructions)
+        // (two scores at a time, in pairs of plain f32 instructions)
         const f32x2 sc2 = {scale_log2e, scale_log2e}, mc2 = {-mc, -mc};
 #pragma unroll
         for (int e = e0; e < e0 + n; e += 2) {
