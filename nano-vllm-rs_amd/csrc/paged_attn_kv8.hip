@@ -5,8 +5,8 @@
 // kv head), kv8_common.hpp:
 //   s_ij = softmax_scale * kscale[block of j] * (q_i . kcode_j),   p_ij = exp(s_ij - max_j s_ij)
 //   o_i  = sum_j (p_ij * vscale[block of j]) vcode_j / sum_j p_ij
-// A scale belongs to a token (its block), so it multiplies scores and probabilities and never the
-// codes: what is converted is one byte to the matrix unit's type, exactly.
+// A scale belongs to a token (its block), so K's multiplies scores.  What the matrix unit gets of K is the
+// code in its type, exactly; of V the code times the power of two in its scale, exactly too.
 #include <hip/hip_runtime.h>
 
 #include <cmath>
@@ -235,8 +235,8 @@ hipError_t launch_generic(const PagedAttnArgs &a, const float *ks, const float *
 //           dims are in an order of their own and Q's fragments follow it;
 //   V       the same image; ds_read_b64_tr_b8 gives a lane 8 keys of one dim.  Group g takes the keys that
 //           its scores are for (4g .. 4g+3 of two blocks), so P needs no lane movement;
-//   codes   become bf16 in registers, exactly (v_cvt_scalef32_pk_bf16_fp8, two a instruction; int8 by way of
-//           f32), and go to mfma_f32_16x16x32_bf16;
+//   codes   become bf16 (K) and f16 (V) in registers, exactly (v_cvt_scalef32_pk_bf16_fp8 and _f16_fp8, two a
+//           instruction; int8 by way of f32, or of f16's bits), and go to mfma_f32_16x16x32;
 //   scales  lane l of the wave holds id, K scale and V scale of block l of a run of 64; v_readlane makes
 //           them scalars at the tile that needs them.  The next run's are loaded 32 tiles ahead.
 // ---------------------------------------------------------------------------
@@ -643,7 +643,7 @@ __global__ __launch_bounds__(64 * W, NQT <= 2 ? 2 : 1) void paged_attn_kv8_decod
             l_run[qt] += sum;
         };
         float vs[kTileBlocks] = {tl.vs[0], tl.vs[1]};
-        if (__builtin_expect(tl.wild, 0)) {  // (here, so that nothing cuts the weights off from the f16 product: T = 12 276 -> 261 us)
+        if (__builtin_expect(tl.wild, 0)) {  // (here, so that no branch is between the weights and the f16 product: T = 12 281 -> 261 us)
 #pragma unroll
             for (int qt = 0; qt < NQT; ++qt) {
                 float p[8];
