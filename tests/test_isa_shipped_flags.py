@@ -88,4 +88,4 @@ def test_mid_kernel(assembly):
         assert lines[i].startswith("s_mov_b32 m0") and lines[i - 1].startswith("s_nop 4")
         assert lines[i + 1].startswith("s_nop 0") and [k for k in dma if i < k < i + 6] == list(range(i + 2, i + 6))
         offs = [re.search(r"offset:(\d+)", lines[k]) for k in range(i + 2, i + 6)]
-        assert [int(o.group(1)) if o else 0 for o in offs] == [0, 1024, 2048, 3072]
+        assert [int(o.group(1)) if o else 0 for o in offs] == [1024 * j for j in range(4)]
